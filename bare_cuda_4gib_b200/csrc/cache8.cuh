@@ -1,0 +1,42 @@
+// A paged cache of keys and values held as e4m3 codes.
+//
+// A page holds, for every cache of its group, keys then values, each [kv_heads][page_tokens][head_dim] codes; beside the pages
+// lie the scales, per page and cache keys' then values', each [kv_heads][page_tokens / SCALE_TOKENS] float32.  The number that a
+// code stands for is code * scale.  What the format keeps, and every kernel here counts on:
+//  - a scale is a power of two, 2^e with SCALE_LEAST <= e <= SCALE_MOST: code * scale is then exactly a bfloat16 (four bits of
+//    a bfloat16's eight, and its range), and a scale can grow without rounding the codes that it covered (but for those that fall
+//    below e4m3's normal range);
+//  - e is the smallest with 448 * 2^e no less than the block's largest entry in size;
+//  - codes are finite.  A block of SCALE_TOKENS positions that was given a NaN or an infinity, as key or value, has NaN as its keys'
+//    scale: every query that sees one of its keys gets NaN, a query to which all of them are hidden none.
+#pragma once
+
+#include "common.cuh"
+
+constexpr int SCALE_TOKENS = 16;
+constexpr int SCALE_LEAST = -100, SCALE_MOST = 119;
+
+struct Cache8 {
+  uint8_t* k;                  // this cache's part of page 0
+  uint8_t* v;
+  float* k_scale;              // this cache's scales of page 0
+  float* v_scale;
+  const int32_t* block_table;  // [batch sequences][table_stride]: page of a request's n-th block, -1 if none
+  long long page_stride;       // codes from one page to the next
+  long long scale_stride;      // scales from one page to the next
+  int table_stride;
+  int page_tokens;             // a multiple of SCALE_TOKENS
+  int kv_heads;
+  int head_dim;
+};
+
+// 2^e for -126 <= e <= 127.
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
+// The exponent of a normal positive power of two.
+__device__ __forceinline__ int exponent_of(float s) { return (__float_as_int(s) >> 23) - 127; }
+
+// The page that holds `position` of batch sequence `seq`, -1 if none does.
+__device__ __forceinline__ int page_of(const Cache8& c, int seq, int position) {
+  const int block = position / c.page_tokens;
+  return block < c.table_stride ? __ldg(c.block_table + (long long)seq * c.table_stride + block) : -1;
+}

@@ -1,0 +1,435 @@
+// Softmax attention of requests that bring very few rows (tokens x query heads of one key/value head: at most 16) over a cache of
+// e4m3 codes (cache8.cuh): the decode step, and steps of a few tokens.  It is to such a cache what attention_decode.cu is to a
+// bfloat16 one (cuongvng/bare-cuda-4gib engine/kernels/attention_qk.cu:49-68, softmax.cu:28-42, attention_av.cu:24-44).
+//
+//   s[k] = scale * 2^e_K(k) * (q . K_k)     p = softmax over the visible k     out = sum_k p[k] 2^e_V(k) V_k
+//
+// The codes are all that is worth bandwidth (2 head_dim bytes a key against a few hundred bytes for the rest), so the kernel is built
+// around their way into the tensor cores:
+//  * A warp takes 16 keys at a time: one scale block.  Keys and values go from memory straight into registers, 16 bytes a
+//    load, in the layout in which a matrix instruction wants them, so nothing passes through shared memory: the products are
+//    turned around (S^T = K Q^T and O^T = V^T P^T with the codes as the left operand, 16 keys or 16 channels, and up to 8 query
+//    rows as the right one), and the order of the inner dimension is free.  Of a key, thread t of four takes 16 neighbouring channels of every 64
+//    and uses them four at a time; of a value, the eight threads of a column take an eighth of the channels each.
+//    Two such products take 8 rows where the usual way round takes 16 with half of them empty (a group of 4 or 8 heads).
+//  * A code becomes a half by one conversion for two; halves hold e4m3 exactly.  The scale of the keys joins the factor of
+//    the scores; that of the values is applied to the 16 keys' sum in 32 bits (scaled weights would leave a half's range).  Queries become
+//    halves times a power of two of their row's own (exact but for entries 2^24 below the row's largest), the weights are at most 2^8.
+//  * The maximum that the exponentials are taken against moves only when a score has outgrown it by 2^8: until then 16 keys need no
+//    exchange between threads but one vote.
+//  * The key blocks of a request are dealt round-robin to the warps of a cluster of up to 8 thread blocks.  A block merges its
+//    warps' states in shared memory and sends row r to block r % n_splits of the cluster, which merges in index order: no
+//    scratch in global memory, no atomics, no second launch.
+//  * Blocks of keys that lie wholly below the step's first new position are asked for before the kernel waits for the one before it.
+// One B200, 32 / 8 heads of 128: 8 requests of 8,192 positions 27.9 us (4.8 TB/s), 64 of 2,000 to 8,192 149.5 us (4.5 TB/s).
+
+#include "cache8.cuh"
+
+#include <cuda_fp16.h>
+
+#ifndef HEAD_DIM
+#define HEAD_DIM 64
+#endif
+
+namespace {
+
+constexpr int D = HEAD_DIM;
+static_assert(D == 64 || D == 128, "HEAD_DIM must be 64 or 128");
+constexpr int WARPS = 8, THREADS = WARPS * 32;
+constexpr int UNIT = SCALE_TOKENS;             // keys a warp takes at a time
+constexpr int KG = D / 64;                     // 64-channel groups of a key
+constexpr int TILES = D / 16;                  // 16-channel tiles of the output
+constexpr int VW = D / 32;                     // 32-bit words of a value that a thread takes (an eighth of its channels)
+constexpr int FEW_ROWS = 16;
+constexpr float RESCALE_STEP = 8.0f;           // base-2 units
+constexpr int STATE = D + 4;                   // floats of a row's state: D sums, the maximum, the sum
+
+struct DecodeArgs {
+  const __nv_bfloat16* q;      // [rows][q_heads * D]
+  __nv_bfloat16* out;
+  Cache8 cache;
+  const int32_t *seq_q_start, *seq_q_len, *seq_kv_len;
+  int q_heads;
+  float scale_log2;
+  int window;
+  AttentionExtras extras;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ uint32_t peer_smem(uint32_t local, uint32_t rank) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
+  return remote;
+}
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two e4m3 codes (the lower half of `lo`, the upper half for the second) as two halves.
+__device__ __forceinline__ void halves(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi) : "r"(codes));
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {   // an 8 x 8 matrix of halves spread over the warp
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <int W>
+__device__ __forceinline__ void load_words(uint32_t (&w)[W], const uint8_t* p) {
+  if (W == 4) {
+    const uint4 v = __ldcg(reinterpret_cast<const uint4*>(p));
+    w[0] = v.x, w[1] = v.y, w[W > 2 ? 2 : 0] = v.z, w[W > 3 ? 3 : 0] = v.w;
+  } else {
+    const uint2 v = __ldcg(reinterpret_cast<const uint2*>(p));
+    w[0] = v.x, w[1] = v.y;
+  }
+}
+
+// NT: groups of 8 query rows.  EXTRAS: whether blocks of positions, a sink or a gate may be asked for.
+template <int NT, bool EXTRAS>
+__global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel(const DecodeArgs a) {
+  constexpr int ROWS = 8 * NT;
+  const AttentionExtras extras = EXTRAS ? a.extras : AttentionExtras{0, nullptr, nullptr, 0};
+  extern __shared__ __align__(16) float smem[];
+  const int n_splits = gridDim.z, split = blockIdx.z, owned_rows = (ROWS + n_splits - 1) / n_splits;
+  float* st = smem;                                       // [WARPS][ROWS][STATE]: this block's warps
+  float* recv = smem + WARPS * ROWS * STATE;              // [n_splits][owned_rows][STATE]: written by the cluster
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  pdl_launch_dependents();
+  const int seq = blockIdx.x, kvh = blockIdx.y;
+  const int group = a.q_heads / a.cache.kv_heads;
+  const int q_start = a.seq_q_start[seq], q_len = a.seq_q_len[seq], kv_len = a.seq_kv_len[seq], n_rows = q_len * group;
+  if (n_rows <= 0 || n_rows > FEW_ROWS) {                 // nothing, or the prompt kernel's: the same for the whole cluster
+    pdl_wait();
+    return;
+  }
+  if (n_splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this block runs: its memory may be written
+  const int pos0 = kv_len - q_len;
+  const int lo_key = first_visible_key(pos0, a.window, extras.chunk);
+  const int max_lo = first_visible_key(kv_len - 1, a.window, extras.chunk);   // from here on no row's bound hides a key
+  const int u_lo = lo_key / UNIT, u_hi = (kv_len - 1) / UNIT;
+  const int stride = WARPS * n_splits, first = u_lo + split * WARPS + warp;
+  const int n_units = first > u_hi ? 0 : (u_hi - first) / stride + 1;         // this warp's: first, first + stride, ...
+  const int closed = pos0 / UNIT;                                             // units from here on this step's append may write
+
+  // Where the warp's units lie, looked up 32 at a time: lane i knows unit i of the stretch.
+  long long where = -1;
+  float k_scale = 0.0f, v_scale = 0.0f;
+  auto look_up = [&](int from) {
+    const int unit = first + (from + lane) * stride;
+    where = -1;
+    if (from + lane < n_units) {
+      const int page = page_of(a.cache, seq, unit * UNIT);
+      if (page >= 0) {
+        const int in_page = unit * UNIT % a.cache.page_tokens;
+        where = (long long)page * a.cache.page_stride + ((long long)kvh * a.cache.page_tokens + in_page) * D;
+        const long long at = (long long)page * a.cache.scale_stride + (long long)kvh * (a.cache.page_tokens / UNIT) + in_page / UNIT;
+        k_scale = __ldcg(a.cache.k_scale + at);
+        v_scale = __ldcg(a.cache.v_scale + at);
+      }
+    }
+  };
+  uint32_t kc[2][KG][4], vc[4][VW];
+  auto load_keys = [&](long long at) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < KG; ++i) load_words<4>(kc[h][i], a.cache.k + at + (g + 8 * h) * D + i * 64 + 16 * t);
+  };
+  auto load_values = [&](long long at) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) load_words<VW>(vc[i], a.cache.v + at + (2 * t + (i & 1) + 8 * (i >> 1)) * D + g * (D / 8));
+  };
+  bool waited = false;
+  auto wait_once = [&]() {
+    if (!waited) pdl_wait(), waited = true;
+  };
+  if (n_units > 0) {
+    // the scale of an open block is the append's to write: only stretches below it may be looked up ahead of the wait
+    if (first + (min(n_units, 32) - 1) * stride >= closed) wait_once();
+    look_up(0);
+    const long long at = __shfl_sync(0xffffffffu, where, 0);
+    if (at >= 0) load_keys(at), load_values(at);
+  }
+  wait_once();
+
+  // ---- the query rows as halves, times a power of two that brings a row's largest entry to [2^10, 2^11)
+  uint32_t qf[NT][KG * 4][2];
+  float factor[NT][2];       // of rows 2 t and 2 t + 1: scale * log2(e) times that power back
+  int row_pos[NT][2], row_lo[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int R = n * 8 + g;
+    uint4 raw[KG][2];
+#pragma unroll
+    for (int i = 0; i < KG; ++i) raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
+    if (R < n_rows) {
+      const __nv_bfloat16* src = a.q + ((long long)(q_start + R / group) * a.q_heads + kvh * group + R % group) * D + 16 * t;
+#pragma unroll
+      for (int i = 0; i < KG; ++i) {
+        raw[i][0] = *reinterpret_cast<const uint4*>(src + i * 64);
+        raw[i][1] = *reinterpret_cast<const uint4*>(src + i * 64 + 8);
+      }
+    }
+    float most = 0.0f;
+    const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(raw);
+#pragma unroll
+    for (int i = 0; i < KG * 8; ++i) most = fmaxf(most, fmaxf(fabsf(__low2float(pairs[i])), fabsf(__high2float(pairs[i]))));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    const int e = most > 0.0f ? min(max(exponent_of(most) - 10, -100), 116) : 0;
+    const float down = power_of_two(-e);
+#pragma unroll
+    for (int i = 0; i < KG * 8; ++i)
+      qf[n][i >> 1][i & 1] = pack_half(__low2float(pairs[i]) * down, __high2float(pairs[i]) * down);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int col = 2 * t + h, C = n * 8 + col;
+      factor[n][h] = a.scale_log2 * power_of_two(__shfl_sync(0xffffffffu, e, col * 4));
+      row_pos[n][h] = C < n_rows ? pos0 + C / group : -1;
+      row_lo[n][h] = first_visible_key(row_pos[n][h], a.window, extras.chunk);
+    }
+  }
+
+  float m[NT][2], l[NT][2], o[NT][TILES][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    m[n][0] = m[n][1] = -INFINITY;
+    l[n][0] = l[n][1] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
+  }
+
+  for (int j = 0; j < n_units; ++j) {
+    const long long at = __shfl_sync(0xffffffffu, where, j & 31);
+    const float ks = __shfl_sync(0xffffffffu, k_scale, j & 31), vs = __shfl_sync(0xffffffffu, v_scale, j & 31);
+    if ((j & 31) == 31) look_up(j + 1);
+    const long long next = j + 1 < n_units ? __shfl_sync(0xffffffffu, where, (j + 1) & 31) : -1;
+    if (at < 0) {                   // a page that a window has given back: no row sees it
+      if (next >= 0) load_keys(next), load_values(next);
+      continue;
+    }
+    const int key0 = (first + j * stride) * UNIT;
+    float s[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < KG; ++i)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t a0, a1, a2, a3;
+        halves(kc[0][i][w], a0, a2);
+        halves(kc[1][i][w], a1, a3);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_f16(s[n], a0, a1, a2, a3, qf[n][i * 4 + w][0], qf[n][i * 4 + w][1]);
+      }
+    if (next >= 0) load_keys(next);
+    const bool all_visible = key0 + UNIT - 1 <= pos0 && key0 >= max_lo;
+    bool grown = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int h = e & 1;
+        float v = s[n][e] * (factor[n][h] * ks);
+        if (!all_visible) {
+          const int key = key0 + g + 8 * (e >> 1);
+          if (key > row_pos[n][h] || key < row_lo[n][h]) v = -INFINITY;
+        }
+        s[n][e] = v;
+        grown |= v > m[n][h] + RESCALE_STEP;
+      }
+    if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float top = fmaxf(s[n][h], s[n][h + 2]);
+#pragma unroll
+          for (int by = 4; by < 32; by <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, by));
+          const float m_new = fmaxf(m[n][h], top);
+          const float corr = m_new == -INFINITY ? 1.0f : fast_exp2(m[n][h] - m_new);
+          m[n][h] = m_new;
+          l[n][h] *= corr;
+#pragma unroll
+          for (int i = 0; i < TILES; ++i) o[n][i][h] *= corr, o[n][i][h + 2] *= corr;
+        }
+    }
+    uint32_t pf[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float m0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
+      const float p0 = fast_exp2(s[n][0] - m0), p1 = fast_exp2(s[n][1] - m1), p2 = fast_exp2(s[n][2] - m0), p3 = fast_exp2(s[n][3] - m1);
+      l[n][0] += p0 + p2;
+      l[n][1] += p1 + p3;
+      pf[n][0] = transposed(pack_half(p0, p1));
+      pf[n][1] = transposed(pack_half(p2, p3));
+    }
+    if (key0 + UNIT > kv_len) {     // behind the last key a page may hold anything, and zero times NaN is not zero
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (key0 + 2 * t + (i & 1) + 8 * (i >> 1) >= kv_len)
+#pragma unroll
+          for (int w = 0; w < VW; ++w) vc[i][w] = 0;
+    }
+#pragma unroll
+    for (int w = 0; w < VW; ++w)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        // channels 4 w + 2 half and + 1 of this thread's eighth, of its four keys
+        const uint32_t pick = half ? 0x7362u : 0x5140u;
+        uint32_t a0, a1, a2, a3;
+        halves(__byte_perm(vc[0][w], vc[1][w], pick), a0, a1);
+        halves(__byte_perm(vc[2][w], vc[3][w], pick), a2, a3);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          mma_f16(part, a0, a1, a2, a3, pf[n][0], pf[n][1]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][2 * w + half][e] = fmaf(part[e], vs, o[n][2 * w + half][e]);
+        }
+      }
+    if (next >= 0) load_values(next);
+  }
+
+  // ---- the warps' states into shared memory: row C of the tile, channels g * D / 8 + 2 i (+ 1)
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float sum = l[n][h];
+#pragma unroll
+      for (int by = 4; by < 32; by <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, by);
+      float* row = st + ((size_t)warp * ROWS + n * 8 + 2 * t + h) * STATE;
+#pragma unroll
+      for (int i = 0; i < TILES; i += 2)
+        *reinterpret_cast<float4*>(row + g * (D / 8) + 2 * i) = make_float4(o[n][i][h], o[n][i][h + 2], o[n][i + 1][h], o[n][i + 1][h + 2]);
+      if (g == 0) row[D] = m[n][h], row[D + 1] = sum;
+    }
+  __syncthreads();
+  if (n_splits > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");   // all blocks of the cluster have started
+  // ---- the block's warps merged, four channels a thread; row r goes to block r % n_splits
+  for (int i = threadIdx.x; i < ROWS * (D / 4); i += THREADS) {
+    const int r = i / (D / 4), c4 = i % (D / 4);
+    if (r >= n_rows) continue;
+    float M = -INFINITY, L = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) M = fmaxf(M, st[((size_t)w * ROWS + r) * STATE + D]);
+    const float M_use = M == -INFINITY ? 0.0f : M;        // (a row of NaN has no maximum, but sums)
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float* from = st + ((size_t)w * ROWS + r) * STATE;
+      const float f = from[D] == -INFINITY ? 1.0f : exp2f(from[D] - M_use);   // without a maximum: zeros, or NaN to be handed on
+      const float4 v = *reinterpret_cast<const float4*>(from + c4 * 4);
+      L += from[D + 1] * f;
+      acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+    }
+    const uint32_t local = smem_u32(recv + ((size_t)split * owned_rows + r / n_splits) * STATE);
+    const uint32_t dst = n_splits > 1 ? peer_smem(local, r % n_splits) : local;
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst + c4 * 16), "f"(acc.x), "f"(acc.y), "f"(acc.z), "f"(acc.w) : "memory");
+    if (c4 == 0) asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(dst + D * 4), "f"(M), "f"(L) : "memory");
+  }
+  if (n_splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  else __syncthreads();
+
+  // ---- the rows this block owns, merged over the blocks in index order
+  for (int i = threadIdx.x; i < owned_rows * (D / 4); i += THREADS) {
+    const int slot = i / (D / 4), c4 = i % (D / 4), r = slot * n_splits + split;
+    if (r >= n_rows) continue;
+    const int token = r / group, head = kvh * group + r % group;
+    const float sink = sink_log2(extras, head);            // joins the row's sum here, once
+    float M = sink;
+    for (int z = 0; z < n_splits; ++z) M = fmaxf(M, recv[((size_t)z * owned_rows + slot) * STATE + D]);
+    const float M_use = M == -INFINITY ? 0.0f : M;
+    float L = exp2f(sink - M_use);
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int z = 0; z < n_splits; ++z) {
+      const float* from = recv + ((size_t)z * owned_rows + slot) * STATE;
+      const float f = from[D] == -INFINITY ? 1.0f : exp2f(from[D] - M_use);
+      const float4 v = *reinterpret_cast<const float4*>(from + c4 * 4);
+      L += from[D + 1] * f;
+      acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+    }
+    const float inv = L == 0.0f ? 0.0f : head_gate<__nv_bfloat16>(extras, q_start + token, head) / L;
+    *reinterpret_cast<uint2*>(a.out + ((long long)(q_start + token) * a.q_heads + head) * D + c4 * 4) =
+        make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+  }
+}
+
+size_t smem_bytes(int rows, int n_splits) {
+  return (size_t)(WARPS * rows + n_splits * ((rows + n_splits - 1) / n_splits)) * STATE * 4;
+}
+
+template <int NT>
+int launch(const DecodeArgs& a, int n_seqs, int n_splits, cudaStream_t stream) {
+  static bool raised = false;
+  if (!raised) {
+    const int most = (int)((WARPS * 8 * NT + 8 * NT + 8) * STATE * 4);
+    if (cudaFuncSetAttribute(cache8_decode_kernel<NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess ||
+        cudaFuncSetAttribute(cache8_decode_kernel<NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess)
+      return launch_status();
+    raised = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(n_seqs, a.cache.kv_heads, n_splits);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem_bytes(8 * NT, n_splits);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n_attr = 0;
+  if (n_splits > 1) {
+    attr[n_attr].id = cudaLaunchAttributeClusterDimension;
+    attr[n_attr].val.clusterDim.x = 1;
+    attr[n_attr].val.clusterDim.y = 1;
+    attr[n_attr].val.clusterDim.z = n_splits;
+    ++n_attr;
+  }
+  if (pdl_enabled()) {
+    attr[n_attr].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n_attr].val.programmaticStreamSerializationAllowed = 1;
+    ++n_attr;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n_attr;
+  const AttentionExtras& x = a.extras;
+  cudaLaunchKernelEx(&cfg, x.chunk > 0 || x.sink || x.gate ? cache8_decode_kernel<NT, true> : cache8_decode_kernel<NT, false>, a);
+  return launch_status();
+}
+
+}  // namespace
+
+// Every request with 1 .. 16 packed rows (q_len * q_heads / kv_heads); the others' blocks return at once.  `rows`: the most packed rows
+// that such a request of the step brings (more than 8 take the kernel for 16).  n_splits (1, 2, 4 or 8) blocks share a
+// request's keys.  chunk, sink, gate and gate_stride: `AttentionExtras`; 0 and null: none.
+extern "C" int llm_cache8_attention_decode(const void* q, void* out, const Cache8* cache, const int32_t* seq_q_start,
+                                           const int32_t* seq_q_len, const int32_t* seq_kv_len, int n_seqs, int n_splits, int rows,
+                                           int q_heads, float scale, int window, int chunk, const float* sink, const void* gate,
+                                           long long gate_stride, cudaStream_t stream) {
+  if (n_seqs <= 0) return 0;
+  const Cache8& c = *cache;
+  if (c.head_dim != D || c.kv_heads <= 0 || q_heads <= 0 || q_heads % c.kv_heads || c.kv_heads > 65535 || c.page_tokens <= 0 ||
+      c.page_tokens % SCALE_TOKENS || (n_splits != 1 && n_splits != 2 && n_splits != 4 && n_splits != 8) || rows < 1 || rows > FEW_ROWS)
+    return ERR_BAD_SIZE;
+  const uintptr_t all = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(c.k) |
+                        reinterpret_cast<uintptr_t>(c.v) | (uintptr_t)c.page_stride;
+  if (all & 15) return ERR_BAD_ALIGN;
+  DecodeArgs a{reinterpret_cast<const __nv_bfloat16*>(q), reinterpret_cast<__nv_bfloat16*>(out), c, seq_q_start, seq_q_len, seq_kv_len,
+               q_heads, scale * 1.4426950408889634f, window, AttentionExtras{chunk, sink, gate, gate_stride}};
+  return rows <= 8 ? launch<1>(a, n_seqs, n_splits, stream) : launch<2>(a, n_seqs, n_splits, stream);
+}

@@ -1,0 +1,201 @@
+"""A paged cache held in 8 bits: e4m3 codes with a power-of-two scale for every 16 positions, key/value head and keys or values each
+(the format: `csrc/cache8.cuh`).  `append` writes a step's keys and values (`csrc/cache8_append.cu`), `attention` reads them
+(`csrc/cache8_attention_decode.cu` for requests that bring at most 16 packed rows, `csrc/cache8_attention_tcgen05.cu` for the others).
+Both go by the step's `StepMaps`.  Head sizes 64 and 128, bfloat16 queries and outputs."""
+
+from __future__ import annotations
+
+import ctypes
+from ctypes import c_float, c_int, c_longlong, c_void_p
+from typing import Dict, Optional
+
+import torch
+
+from . import build
+from ..errors import KernelLaunchError
+from .lib import AttentionExtras, CacheView, Partials, _check, _ptr, dtype_code, sm_count, stream_handle
+from .step_maps import SCALE_TOKENS, StepMaps
+
+DTYPE = torch.float8_e4m3fn
+HEAD_DIMS = (64, 128)
+FEW_ROWS = 16            # packed rows up to which the decode kernel takes a request
+DECODE_WARPS = 8         # warps of a block of the decode kernel, which a request's scale blocks are dealt to
+_append_lib = None
+_decode_libs: Dict[int, object] = {}
+_prompt_libs: Dict[int, object] = {}
+
+
+class _Cache8(ctypes.Structure):
+    """struct Cache8 of csrc/cache8.cuh."""
+
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p), ("block_table", c_void_p),
+                ("page_stride", c_longlong), ("scale_stride", c_longlong), ("table_stride", c_int), ("page_tokens", c_int),
+                ("kv_heads", c_int), ("head_dim", c_int)]
+
+
+def supports(head_dim: int, v_dim: Optional[int] = None, page_tokens: int = SCALE_TOKENS) -> bool:
+    return head_dim in HEAD_DIMS and (v_dim is None or v_dim == head_dim) and page_tokens > 0 and page_tokens % SCALE_TOKENS == 0
+
+
+def _append():
+    global _append_lib
+    if _append_lib is None:
+        l = build.load_library("cache8_append.cu")
+        P, I, L = c_void_p, c_int, c_longlong
+        l.llm_cache8_append.argtypes = [P, I, I, L, P, P, P, P, I, P, P, P, P, I, I, P]
+        l.llm_cache8_append.restype = c_int
+        _append_lib = l
+    return _append_lib
+
+
+def _decode(head_dim: int):
+    l = _decode_libs.get(head_dim)
+    if l is None:
+        l = build.load_library("cache8_attention_decode.cu", (f"-DHEAD_DIM={head_dim}",))
+        P, I, L, F = c_void_p, c_int, c_longlong, c_float
+        l.llm_cache8_attention_decode.argtypes = [P, P, P, P, P, P, I, I, I, I, F, I, I, P, P, L, P]
+        l.llm_cache8_attention_decode.restype = c_int
+        _decode_libs[head_dim] = l
+    return l
+
+
+def _prompt(head_dim: int):
+    l = _prompt_libs.get(head_dim)
+    if l is None:
+        l = build.load_library("cache8_attention_tcgen05.cu", (f"-DHEAD_DIM={head_dim}",))
+        P, I, L, F = c_void_p, c_int, c_longlong, c_float
+        l.llm_cache8_attention_prompt.argtypes = [P, P, P, P, P, P, P, P, I, I, F, I, I, P, P, L, P, P]
+        l.llm_cache8_attention_prompt.restype = c_int
+        l.llm_cache8_attention_prompt_rows.restype = c_int
+        _prompt_libs[head_dim] = l
+    return l
+
+
+def tile_rows(head_dim: int) -> int:
+    """The `tile_rows` that a `StepMaps` for this head size is made with."""
+    return int(_prompt(head_dim).llm_cache8_attention_prompt_rows())
+
+
+def prepare(head_dim: int) -> None:
+    """Builds and loads the kernels for this head size."""
+    _append(), _decode(head_dim), _prompt(head_dim)
+
+
+def view(codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, index: int = 0) -> CacheView:
+    """The cache that lies in `codes` (uint8 or float8_e4m3fn, [pages, (caches,) keys | values, kv heads, page tokens, head size])
+    and `scales` (float32, [pages, (caches,) keys | values, kv heads, page tokens / 16]): with caches, the one at `index`."""
+    if codes.dim() == 5:
+        codes, scales = codes.unsqueeze(1), scales.unsqueeze(1)
+    if codes.dim() != 6 or scales.dim() != 5 or codes.dtype not in (torch.uint8, DTYPE) or scales.dtype != torch.float32:
+        raise KernelLaunchError("cache8: codes must be uint8 or float8_e4m3fn with five or six axes, scales float32 with one less")
+    pages, caches, two, kv_heads, page_tokens, head_dim = codes.shape
+    if tuple(scales.shape) != (pages, caches, two, kv_heads, page_tokens // SCALE_TOKENS) or two != 2 or not 0 <= index < caches:
+        raise KernelLaunchError(f"cache8: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not belong together, or there is "
+                                f"no cache {index}")
+    if not codes.is_contiguous() or not scales.is_contiguous():
+        raise KernelLaunchError("cache8: codes and scales must be contiguous")
+    if not supports(head_dim, None, page_tokens):
+        raise KernelLaunchError(f"cache8: head size {head_dim} in pages of {page_tokens} positions is not supported (head sizes "
+                                f"{HEAD_DIMS}, pages of a multiple of {SCALE_TOKENS})")
+    if not codes.is_cuda or scales.device != codes.device or block_table.device != codes.device:
+        raise KernelLaunchError("cache8: codes, scales and block table must lie on one CUDA device")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
+        raise KernelLaunchError("cache8: the block table must be int32 with dense rows")
+    per_cache, per_cache_scales = 2 * kv_heads * page_tokens * head_dim, 2 * kv_heads * (page_tokens // SCALE_TOKENS)
+    k = codes.data_ptr() + index * per_cache
+    s = scales.data_ptr() + index * per_cache_scales * 4
+    return CacheView(k, k + per_cache // 2, block_table, caches * per_cache, block_table.stride(0), page_tokens, kv_heads, head_dim,
+                     DTYPE, codes.data_ptr(), codes.numel(), k_scale_ptr=s, v_scale_ptr=s + per_cache_scales // 2 * 4,
+                     scale_stride=caches * per_cache_scales)
+
+
+def _struct(cache: CacheView) -> int:
+    if cache.dtype != DTYPE:
+        raise KernelLaunchError(f"cache8: a cache of {cache.dtype} is not one of e4m3 codes")
+    if cache.struct is None:
+        cache.struct = _Cache8(cache.k_ptr, cache.v_ptr, cache.k_scale_ptr, cache.v_scale_ptr, cache.block_table.data_ptr(),
+                               cache.page_stride, cache.scale_stride, cache.table_stride, cache.page_tokens, cache.kv_heads, cache.head_dim)
+    return ctypes.addressof(cache.struct)
+
+
+def _check_step(what: str, cache: CacheView, maps: StepMaps, q_heads: int, *tensors) -> None:
+    if q_heads <= 0 or q_heads % cache.kv_heads:
+        raise KernelLaunchError(f"{what}: {q_heads} query heads cannot share {cache.kv_heads} key/value heads")
+    if maps.page_tokens != cache.page_tokens or maps.group * cache.kv_heads != q_heads:
+        raise KernelLaunchError(f"{what}: the step's maps are for pages of {maps.page_tokens} positions and {maps.group} heads a key/value head")
+    if maps.longest == 0:
+        raise KernelLaunchError(f"{what}: the step's maps have not been built")
+    if cache.block_table.shape[0] < maps.n_seqs:
+        raise KernelLaunchError(f"{what}: {maps.n_seqs} requests, and a block table of {cache.block_table.shape[0]} rows")
+    device = cache.block_table.device
+    if maps.device != device or any(t.device != device for t in tensors):
+        raise KernelLaunchError(f"{what}: maps, cache and tensors must lie on one CUDA device")
+    if device.index != torch.cuda.current_device():
+        raise KernelLaunchError(f"{what}: the tensors lie on {device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def append(qkv: Partials, q_out: torch.Tensor, cache: CacheView, maps: StepMaps, inv_freq: Optional[torch.Tensor], q_heads: int,
+           write_cache: bool = True, stream=None) -> None:
+    """Rows [q | k | v] of the step (`qkv`, dense, bfloat16 or float32, possibly a sum of partial results): q turned by
+    position into `q_out` (bfloat16 [rows, q_heads * head size]), k turned by position and v into the cache (left alone unless
+    `write_cache`).  `inv_freq` (float32 [head size / 2]) None: no rotation.  Positions of a written block that earlier steps filled
+    keep their numbers, but for a rounding where the new ones need a larger scale.  Rows of no request and idle ones are
+    left as they were in `q_out`."""
+    t = qkv.tensor
+    width, d = (q_heads + 2 * cache.kv_heads) * cache.head_dim, cache.head_dim
+    at = _struct(cache)
+    _check_step("cache8_append", cache, maps, q_heads, t, q_out)
+    if t.shape[-1] != width or t.shape[-2] < maps.n_rows or t.stride(-1) != 1 or t.stride(-2) != width or (qkv.n > 1 and t.shape[0] < qkv.n):
+        raise KernelLaunchError(f"cache8_append: projections of {tuple(t.shape)} for {maps.n_rows} dense rows of {width}")
+    if q_out.dtype != torch.bfloat16 or q_out.shape[-1] != q_heads * d or q_out.shape[0] < maps.n_rows or not q_out.is_contiguous():
+        raise KernelLaunchError(f"cache8_append: queries go to contiguous bfloat16 [rows, {q_heads * d}], not {tuple(q_out.shape)} of {q_out.dtype}")
+    if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.numel() != d // 2 or not inv_freq.is_contiguous()
+                                 or inv_freq.device != t.device):
+        raise KernelLaunchError(f"cache8_append: the inverse frequencies must be {d // 2} contiguous float32 numbers")
+    _check(_append().llm_cache8_append(
+        t.data_ptr(), dtype_code(t.dtype), qkv.n, qkv.stride, q_out.data_ptr(), at, maps.write_seq.data_ptr(), maps.write_block.data_ptr(),
+        maps.n_writes, maps.seq_q_start.data_ptr(), maps.seq_q_len.data_ptr(), maps.seq_kv_len.data_ptr(), _ptr(inv_freq), q_heads,
+        1 if write_cache else 0, stream if stream is not None else stream_handle()), "cache8_append")
+
+
+def decode_splits(n_seqs: int, kv_heads: int, max_keys: int) -> int:
+    """How many blocks of the decode kernel share a request's keys: a power of two up to 8, about two blocks an SM in all, and no more
+    than have a scale block for every warp."""
+    splits = 1
+    while splits < 8 and n_seqs * kv_heads * splits * 2 <= 2 * sm_count() and max_keys > splits * DECODE_WARPS * SCALE_TOKENS:
+        splits *= 2
+    return splits
+
+
+def attention(q: torch.Tensor, out: torch.Tensor, cache: CacheView, maps: StepMaps, q_heads: int, scale: float, window: int = 0,
+              extras: Optional[AttentionExtras] = None, stream=None) -> None:
+    """out = softmax(scale * q k^T) v over each request's cached positions up to the query's own (with `window` > 0 the newest
+    `window` of them), q and out contiguous bfloat16 [rows, q_heads * head size].  `extras`: blocks of positions, sink, gate.
+    Requests of few packed rows go to the decode kernel, the others to the prompt kernel, which a step may launch both of; rows
+    of no request and idle ones are left as they were in `out`, a row that sees no key is zero."""
+    at = _struct(cache)
+    _check_step("cache8_attention", cache, maps, q_heads, q, out)
+    for t in (q, out):
+        if t.dtype != torch.bfloat16 or t.shape[-1] != q_heads * cache.head_dim or t.shape[0] < maps.n_rows or not t.is_contiguous():
+            raise KernelLaunchError(f"cache8_attention: queries and outputs must be contiguous bfloat16 [{maps.n_rows} rows, "
+                                    f"{q_heads * cache.head_dim}], not {tuple(t.shape)} of {t.dtype}")
+    if not scale > 0.0 or window < 0:
+        raise KernelLaunchError(f"cache8_attention: scale {scale} and window {window} are not supported (above zero; zero or more)")
+    if maps.few_rows != FEW_ROWS or maps.tile_rows != tile_rows(cache.head_dim):
+        raise KernelLaunchError(f"cache8_attention: the step's maps must be made with few_rows {FEW_ROWS} and tile_rows "
+                                f"{tile_rows(cache.head_dim)}")
+    chunk, sink, gate, gate_stride = extras.arguments(q_heads, q.dtype) if extras is not None else (0, 0, 0, 0)
+    stream = stream if stream is not None else stream_handle()
+    group = maps.group
+    if maps.shortest * group <= FEW_ROWS:
+        rows = min(maps.longest * group, FEW_ROWS)
+        splits = decode_splits(maps.n_seqs, cache.kv_heads, cache.table_stride * cache.page_tokens)
+        _check(_decode(cache.head_dim).llm_cache8_attention_decode(
+            q.data_ptr(), out.data_ptr(), at, maps.seq_q_start.data_ptr(), maps.seq_q_len.data_ptr(), maps.seq_kv_len.data_ptr(),
+            maps.n_seqs, splits, rows, q_heads, scale, window, chunk, sink, gate, gate_stride, stream), "cache8_attention_decode")
+    if maps.longest * group > FEW_ROWS:
+        from . import gemm
+        _check(_prompt(cache.head_dim).llm_cache8_attention_prompt(
+            q.data_ptr(), out.data_ptr(), at, maps.seq_q_start.data_ptr(), maps.seq_q_len.data_ptr(), maps.seq_kv_len.data_ptr(),
+            maps.tile_seq.data_ptr(), maps.tile_index.data_ptr(), maps.n_tiles, q_heads, scale, window, chunk, sink, gate, gate_stride,
+            gemm.error_word(q.device).data_ptr(), stream), "cache8_attention_prompt")

@@ -60,7 +60,9 @@ def check_errors() -> None:
             role = {1: "gemm TMA producer", 2: "gemm MMA issuer", 3: "gemm epilogue", 11: "attention loader",
                     12: "attention MMA issuer", 13: "attention softmax",
                     14: "attention (shared memory not 1024-byte aligned)", 21: "few-token product, producer",
-                    22: "few-token product, consumer", 4: "gemm cluster exchange", 31: "decode attention"}.get(code, f"code {code}")
+                    22: "few-token product, consumer", 4: "gemm cluster exchange", 31: "decode attention",
+                    41: "attention over 8-bit codes, converters", 42: "attention over 8-bit codes, MMA issuer",
+                    43: "attention over 8-bit codes, softmax", 44: "attention over 8-bit codes (shared memory not 1024-byte aligned)"}.get(code, f"code {code}")
             raise KernelLaunchError(f"a kernel gave up ({role}): a bounded wait ran out; the result is invalid")
 
 

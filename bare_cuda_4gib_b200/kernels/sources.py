@@ -2,6 +2,7 @@
 needs at first use; `all_libraries()` is everything, for the build check."""
 
 ATTENTION_F32_HEAD_DIMS = (64, 128)
+CACHE8_HEAD_DIMS = (64, 128)
 ATTENTION_HEAD_DIMS = (16, 32, 48, 64, 80, 96, 112, 128)
 # (entries of one map, value entries) of differential attention on the tensor cores, as the presets have them
 DIFF_ATTENTION_SIZES = ((16, 16), (64, 128), (128, 256))
@@ -28,5 +29,7 @@ def all_libraries():
     jobs += [("attention_tcgen05.cu", (f"-DHEAD_DIM={d}",)) for d in (64, 128)]
     jobs += [("attention_decode.cu", (f"-DHEAD_DIM={d}",)) for d in (64, 128)]
     jobs += [("attention_decode.cu", ("-DHEAD_DIM=64", "-DDECODE_KEY_BLOCK=32"))]
+    jobs += [("step_maps.cu", ()), ("cache8_append.cu", ())]
+    jobs += [(f"cache8_attention_{kind}.cu", (f"-DHEAD_DIM={d}",)) for kind in ("decode", "tcgen05") for d in CACHE8_HEAD_DIMS]
     jobs += [("diff_attention.cu", (f"-DDA_DQ={d}", f"-DDA_DV={v}")) for d, v in DIFF_ATTENTION_SIZES]
     return jobs
