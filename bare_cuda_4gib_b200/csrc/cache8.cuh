@@ -30,6 +30,14 @@ struct Cache8 {
   int head_dim;
 };
 
+// What the kernels of a step go by: the arrays of llm_step_maps.
+struct StepLists {
+  const int32_t *seq_q_start, *seq_q_len, *seq_kv_len;   // per request: first row, new tokens, length after the step
+  const int32_t *write_seq, *write_block;                // blocks of SCALE_TOKENS positions that the step writes; -1, 0 behind the last
+  const int32_t *tile_seq, *tile_index;                  // tiles of the requests with many rows; -1, 0 behind the last
+  int n_seqs, n_writes, n_tiles;
+};
+
 // 2^e for -126 <= e <= 127.
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
 // The exponent of a normal positive power of two.

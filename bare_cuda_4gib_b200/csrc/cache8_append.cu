@@ -30,7 +30,7 @@ struct AppendArgs {
   long long partial_stride;
   __nv_bfloat16* q_out;        // [rows][q_heads * head_dim]
   Cache8 cache;
-  const int32_t *write_seq, *write_block, *seq_q_start, *seq_q_len, *seq_kv_len;
+  StepLists lists;
   const float* inv_freq;       // null: no rotation
   int q_heads, write_cache;
 };
@@ -106,13 +106,13 @@ __global__ void __launch_bounds__(TOKENS * (D / 8)) cache8_append_kernel(const A
   __shared__ float2 angles[TOKENS][HALF];
   __shared__ float largest[2][THREADS / 32];
   const int tid = threadIdx.x, group_of = tid / CHUNKS, c = tid % CHUNKS, kvh = blockIdx.y;
-  const int seq = a.write_seq[blockIdx.x];
+  const int seq = a.lists.write_seq[blockIdx.x];
   if (seq < 0) {
     pdl_wait();
     return;
   }
-  const int first = a.write_block[blockIdx.x] * TOKENS;
-  const int q_start = a.seq_q_start[seq], kv_len = a.seq_kv_len[seq], cached = kv_len - a.seq_q_len[seq];
+  const int first = a.lists.write_block[blockIdx.x] * TOKENS;
+  const int q_start = a.lists.seq_q_start[seq], kv_len = a.lists.seq_kv_len[seq], cached = kv_len - a.lists.seq_q_len[seq];
   const int lo = max(first, cached), n_new = min(first + TOKENS, kv_len) - lo;      // the block's new positions: lo ..
   const long long row0 = (long long)q_start + lo - cached;                            // their first row
   const int page = page_of(a.cache, seq, first);
@@ -207,8 +207,8 @@ __global__ void __launch_bounds__(TOKENS * (D / 8)) cache8_append_kernel(const A
 }
 
 template <int D, typename T>
-int launch(const AppendArgs& a, int n_writes, cudaStream_t stream) {
-  launch_kernel(cache8_append_kernel<D, T>, dim3(n_writes, a.cache.kv_heads), TOKENS * (D / 8), 0, stream, a);
+int launch(const AppendArgs& a, cudaStream_t stream) {
+  launch_kernel(cache8_append_kernel<D, T>, dim3(a.lists.n_writes, a.cache.kv_heads), TOKENS * (D / 8), 0, stream, a);
   return launch_status();
 }
 
@@ -218,10 +218,9 @@ int launch(const AppendArgs& a, int n_writes, cudaStream_t stream) {
 // rows of (q_heads + 2 kv_heads) * head_dim.  The lists are those of llm_step_maps.  Rows of no request, and idle ones, are left as they
 // were in q_out.  head_dim 64 or 128.
 extern "C" int llm_cache8_append(const void* qkv, int in_dtype, int n_partials, long long partial_stride, void* q_out,
-                                 const Cache8* cache, const int32_t* write_seq, const int32_t* write_block, int n_writes,
-                                 const int32_t* seq_q_start, const int32_t* seq_q_len, const int32_t* seq_kv_len,
-                                 const float* inv_freq, int q_heads, int write_cache, cudaStream_t stream) {
-  if (n_writes <= 0) return 0;
+                                 const Cache8* cache, const StepLists* lists, const float* inv_freq, int q_heads, int write_cache,
+                                 cudaStream_t stream) {
+  if (lists->n_writes <= 0) return 0;
   const Cache8& c = *cache;
   if (c.kv_heads <= 0 || q_heads <= 0 || q_heads % c.kv_heads || c.kv_heads > 65535 || n_partials < 1 || c.page_tokens % SCALE_TOKENS ||
       c.page_tokens <= 0 || (c.head_dim != 64 && c.head_dim != 128))
@@ -230,8 +229,7 @@ extern "C" int llm_cache8_append(const void* qkv, int in_dtype, int n_partials, 
   const uintptr_t all = reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(c.k) |
                         reinterpret_cast<uintptr_t>(c.v) | (uintptr_t)c.page_stride;
   if ((all & 15) || (n_partials > 1 && partial_stride % 4)) return ERR_BAD_ALIGN;
-  AppendArgs a{qkv, n_partials, partial_stride, reinterpret_cast<__nv_bfloat16*>(q_out), c, write_seq, write_block, seq_q_start,
-               seq_q_len, seq_kv_len, inv_freq, q_heads, write_cache};
-  if (c.head_dim == 64) return in_dtype == DT_F32 ? launch<64, float>(a, n_writes, stream) : launch<64, __nv_bfloat16>(a, n_writes, stream);
-  return in_dtype == DT_F32 ? launch<128, float>(a, n_writes, stream) : launch<128, __nv_bfloat16>(a, n_writes, stream);
+  AppendArgs a{qkv, n_partials, partial_stride, reinterpret_cast<__nv_bfloat16*>(q_out), c, *lists, inv_freq, q_heads, write_cache};
+  if (c.head_dim == 64) return in_dtype == DT_F32 ? launch<64, float>(a, stream) : launch<64, __nv_bfloat16>(a, stream);
+  return in_dtype == DT_F32 ? launch<128, float>(a, stream) : launch<128, __nv_bfloat16>(a, stream);
 }

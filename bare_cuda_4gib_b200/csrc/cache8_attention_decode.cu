@@ -13,8 +13,9 @@
 //    and uses them four at a time; of a value, the eight threads of a column take an eighth of the channels each.
 //    Two such products take 8 rows where the usual way round takes 16 with half of them empty (a group of 4 or 8 heads).
 //  * A code becomes a half by one conversion for two; halves hold e4m3 exactly.  The scale of the keys joins the factor of
-//    the scores; that of the values is applied to the 16 keys' sum in 32 bits (scaled weights would leave a half's range).  Queries become
-//    halves times a power of two of their row's own (exact but for entries 2^24 below the row's largest), the weights are at most 2^8.
+//    the scores.  A weight goes into P together with its block's value scale: P = 2^(s + e_V - m) with m the running maximum of s + e_V,
+//    while the sum takes P 2^-e_V; so a half of P is relative to what the row's keys can add to its output, and O needs no factor.
+//    Queries become halves times a power of two of their row's own (exact but for entries 2^24 below the row's largest).
 //  * The maximum that the exponentials are taken against moves only when a score has outgrown it by 2^8: until then 16 keys need no
 //    exchange between threads but one vote.
 //  * The key blocks of a request are dealt round-robin to the warps of a cluster of up to 8 thread blocks.  A block merges its
@@ -48,7 +49,7 @@ struct DecodeArgs {
   const __nv_bfloat16* q;      // [rows][q_heads * D]
   __nv_bfloat16* out;
   Cache8 cache;
-  const int32_t *seq_q_start, *seq_q_len, *seq_kv_len;
+  StepLists lists;
   int q_heads;
   float scale_log2;
   int window;
@@ -113,7 +114,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
   pdl_launch_dependents();
   const int seq = blockIdx.x, kvh = blockIdx.y;
   const int group = a.q_heads / a.cache.kv_heads;
-  const int q_start = a.seq_q_start[seq], q_len = a.seq_q_len[seq], kv_len = a.seq_kv_len[seq], n_rows = q_len * group;
+  const int q_start = a.lists.seq_q_start[seq], q_len = a.lists.seq_q_len[seq], kv_len = a.lists.seq_kv_len[seq], n_rows = q_len * group;
   if (n_rows <= 0 || n_rows > FEW_ROWS) {                 // nothing, or the prompt kernel's: the same for the whole cluster
     pdl_wait();
     return;
@@ -129,7 +130,8 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
 
   // Where the warp's units lie, looked up 32 at a time: lane i knows unit i of the stretch.
   long long where = -1;
-  float k_scale = 0.0f, v_scale = 0.0f;
+  float k_scale = 0.0f;
+  int v_exponent = 0;
   auto look_up = [&](int from) {
     const int unit = first + (from + lane) * stride;
     where = -1;
@@ -140,7 +142,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
         where = (long long)page * a.cache.page_stride + ((long long)kvh * a.cache.page_tokens + in_page) * D;
         const long long at = (long long)page * a.cache.scale_stride + (long long)kvh * (a.cache.page_tokens / UNIT) + in_page / UNIT;
         k_scale = __ldcg(a.cache.k_scale + at);
-        v_scale = __ldcg(a.cache.v_scale + at);
+        v_exponent = exponent_of(__ldcg(a.cache.v_scale + at));
       }
     }
   };
@@ -217,7 +219,8 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
 
   for (int j = 0; j < n_units; ++j) {
     const long long at = __shfl_sync(0xffffffffu, where, j & 31);
-    const float ks = __shfl_sync(0xffffffffu, k_scale, j & 31), vs = __shfl_sync(0xffffffffu, v_scale, j & 31);
+    const float ks = __shfl_sync(0xffffffffu, k_scale, j & 31);
+    const int ev = __shfl_sync(0xffffffffu, v_exponent, j & 31);
     if ((j & 31) == 31) look_up(j + 1);
     const long long next = j + 1 < n_units ? __shfl_sync(0xffffffffu, where, (j + 1) & 31) : -1;
     if (at < 0) {                   // a page that a window has given back: no row sees it
@@ -246,7 +249,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int h = e & 1;
-        float v = s[n][e] * (factor[n][h] * ks);
+        float v = fmaf(s[n][e], factor[n][h] * ks, (float)ev);
         if (!all_visible) {
           const int key = key0 + g + 8 * (e >> 1);
           if (key > row_pos[n][h] || key < row_lo[n][h]) v = -INFINITY;
@@ -275,8 +278,8 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
     for (int n = 0; n < NT; ++n) {
       const float m0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
       const float p0 = fast_exp2(s[n][0] - m0), p1 = fast_exp2(s[n][1] - m1), p2 = fast_exp2(s[n][2] - m0), p3 = fast_exp2(s[n][3] - m1);
-      l[n][0] += p0 + p2;
-      l[n][1] += p1 + p3;
+      l[n][0] = fmaf(p0 + p2, power_of_two(-ev), l[n][0]);
+      l[n][1] = fmaf(p1 + p3, power_of_two(-ev), l[n][1]);
       pf[n][0] = transposed(pack_half(p0, p1));
       pf[n][1] = transposed(pack_half(p2, p3));
     }
@@ -297,12 +300,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
         halves(__byte_perm(vc[0][w], vc[1][w], pick), a0, a1);
         halves(__byte_perm(vc[2][w], vc[3][w], pick), a2, a3);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          mma_f16(part, a0, a1, a2, a3, pf[n][0], pf[n][1]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[n][2 * w + half][e] = fmaf(part[e], vs, o[n][2 * w + half][e]);
-        }
+        for (int n = 0; n < NT; ++n) mma_f16(o[n][2 * w + half], a0, a1, a2, a3, pf[n][0], pf[n][1]);
       }
     if (next >= 0) load_values(next);
   }
@@ -377,7 +375,7 @@ size_t smem_bytes(int rows, int n_splits) {
 }
 
 template <int NT>
-int launch(const DecodeArgs& a, int n_seqs, int n_splits, cudaStream_t stream) {
+int launch(const DecodeArgs& a, int n_splits, cudaStream_t stream) {
   static bool raised = false;
   if (!raised) {
     const int most = (int)((WARPS * 8 * NT + 8 * NT + 8) * STATE * 4);
@@ -387,7 +385,7 @@ int launch(const DecodeArgs& a, int n_seqs, int n_splits, cudaStream_t stream) {
     raised = true;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(n_seqs, a.cache.kv_heads, n_splits);
+  cfg.gridDim = dim3(a.lists.n_seqs, a.cache.kv_heads, n_splits);
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = smem_bytes(8 * NT, n_splits);
   cfg.stream = stream;
@@ -417,11 +415,10 @@ int launch(const DecodeArgs& a, int n_seqs, int n_splits, cudaStream_t stream) {
 // Every request with 1 .. 16 packed rows (q_len * q_heads / kv_heads); the others' blocks return at once.  `rows`: the most packed rows
 // that such a request of the step brings (more than 8 take the kernel for 16).  n_splits (1, 2, 4 or 8) blocks share a
 // request's keys.  chunk, sink, gate and gate_stride: `AttentionExtras`; 0 and null: none.
-extern "C" int llm_cache8_attention_decode(const void* q, void* out, const Cache8* cache, const int32_t* seq_q_start,
-                                           const int32_t* seq_q_len, const int32_t* seq_kv_len, int n_seqs, int n_splits, int rows,
+extern "C" int llm_cache8_attention_decode(const void* q, void* out, const Cache8* cache, const StepLists* lists, int n_splits, int rows,
                                            int q_heads, float scale, int window, int chunk, const float* sink, const void* gate,
                                            long long gate_stride, cudaStream_t stream) {
-  if (n_seqs <= 0) return 0;
+  if (lists->n_seqs <= 0) return 0;
   const Cache8& c = *cache;
   if (c.head_dim != D || c.kv_heads <= 0 || q_heads <= 0 || q_heads % c.kv_heads || c.kv_heads > 65535 || c.page_tokens <= 0 ||
       c.page_tokens % SCALE_TOKENS || (n_splits != 1 && n_splits != 2 && n_splits != 4 && n_splits != 8) || rows < 1 || rows > FEW_ROWS)
@@ -429,7 +426,6 @@ extern "C" int llm_cache8_attention_decode(const void* q, void* out, const Cache
   const uintptr_t all = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(c.k) |
                         reinterpret_cast<uintptr_t>(c.v) | (uintptr_t)c.page_stride;
   if (all & 15) return ERR_BAD_ALIGN;
-  DecodeArgs a{reinterpret_cast<const __nv_bfloat16*>(q), reinterpret_cast<__nv_bfloat16*>(out), c, seq_q_start, seq_q_len, seq_kv_len,
-               q_heads, scale * 1.4426950408889634f, window, AttentionExtras{chunk, sink, gate, gate_stride}};
-  return rows <= 8 ? launch<1>(a, n_seqs, n_splits, stream) : launch<2>(a, n_seqs, n_splits, stream);
+  DecodeArgs a{reinterpret_cast<const __nv_bfloat16*>(q), reinterpret_cast<__nv_bfloat16*>(out), c, *lists, q_heads, scale * 1.4426950408889634f, window, AttentionExtras{chunk, sink, gate, gate_stride}};
+  return rows <= 8 ? launch<1>(a, n_splits, stream) : launch<2>(a, n_splits, stream);
 }

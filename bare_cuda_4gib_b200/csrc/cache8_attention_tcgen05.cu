@@ -3,28 +3,38 @@
 // head).  Nothing of cuongvng/bare-cuda-4gib's [heads, T, keys] score buffer exists (engine/kernels/attention_qk.cu:49-68,
 // softmax.cu:28-42, attention_av.cu:24-44).
 //
-// One thread block = two tiles of 128 packed rows of one request and one key/value head, which share every key and value
-// block.  Keys are visited in blocks of 128 positions:
-//   converter warps  (four) fetch a tile's codes from the request's pages, 16 bytes a load and one tile ahead, and write
-//                  code * scale as bfloat16 into 128-byte-swizzled shared memory.  A scale is a power of two, so that number is a
-//                  bfloat16 exactly, and everything behind it is the bfloat16 kernel.  Key tiles and value tiles go through
-//                  ONE ring of slots in the order K(0) V(0) K(1) V(1) ..., each slot given back by the commit of the last product that
-//                  reads it;
-//   MMA thread     S_g = Q_g K^T (M 128, N 128, K head size) into tile g's S columns of tensor memory;
-//   softmax warps  a group of four warps per tile; group g owns tile g and sees every key block of it.
-//                  First it stages Q_g with cp.async.  Then, one thread per row: read the row of S from tensor memory once, 64 columns
-//                  at a time, scale, mask, running maximum and sum in float32 (base 2), write P as bfloat16 into swizzled
-//                  shared memory (the A operand of the second product);
-//   MMA thread     O_g (+)= P_g V (M 128, N 64 per 64 value columns, K 128): O accumulates in tensor memory over all key blocks;
-//   softmax warps  the maximum that the exponentials are taken against follows the row's true maximum only when that
-//                  has grown by more than 2^8; at the end every thread divides its row of O by its sum and stores it.
+//   s[k] = scale * 2^e_K(k) * (q . K_k)     p = softmax over the visible k     out = sum_k p[k] 2^e_V(k) V_k
+//
+// One thread block = two tiles of 128 packed rows of one request and one key/value head, which share every key and value block of 128
+// positions.  Warps:
+//   converters (4) fetch a tile's codes from the request's pages, 16 bytes a load and a tile ahead, and write them as halves into
+//                  128-byte-swizzled shared memory.  Halves hold e4m3 exactly and one instruction converts two codes.  The scales
+//                  of a key block are split into 2^e of the block (the largest, which the softmax gets) and what is left for 16 positions, at most one, which
+//                  joins the halves (exactly down to 2^-15).  Key tiles and value tiles go through ONE ring of slots in the order K(0) V(0) K(1) ...;
+//   MMA issuer (1) S_g = Q_g K^T (M 128, N 128, K head size) into tile g's S columns of tensor memory, and
+//                  O_g (+)= P_g V with P_g as the operand in tensor memory and V as it lies ([key][channel], MN-major), in two halves of 64
+//                  keys, each as soon as its half of P is there: P never goes through shared memory, whose bandwidth
+//                  is what a block with P there is bound by (K and V tiles, two Q tiles and two P tiles a key block);
+//   softmax (8)    a group of four warps per tile, one thread per row.  First it stages Q_g as halves (times a power of two of
+//                  the row's own).  Then, per key block: read the row of S, 64 columns at a time, mask, running maximum and sum in
+//                  float32 (base 2), write P as halves back into tensor memory.
+// A weight goes into P together with the scale of its block's values: P = 2^(s + e_V - m) with m the running maximum of s + e_V, while the sum
+// takes P 2^-e_V.  So a half of P is relative to what the row's keys can add to its output, and O needs no factor of its own.
+// m follows the true maximum only when that has grown by more than 2^8 (a half reaches 2^15), so O is rescaled rarely.
+// At head size 128 a tile's P takes the columns of its S (S 2 x 128, O 2 x 128 columns of the 512): its next S is issued when P has been
+// read, and the other tile's softmax fills that time; at head size 64 P has columns of its own.
+// Few tiles (a question behind a long text): the key blocks are split among the blocks of a cluster, each with a softmax of its own; their
+// states are merged in index order through distributed shared memory.
 // A NaN scale (a block that was given a NaN) makes keys NaN, hence the scores of the rows that see them; hidden scores are replaced, not
 // multiplied, and values are finite always.  Values behind the request's last key are written as zeros.
 // Every mbarrier wait is bounded: on a timeout the thread sets the error word, all roles leave their loops, tensor memory is
 // released and the block returns.
-// One B200: a prompt of 2,048 tokens (32 / 4 heads of 64) 50.0 us, 2,048 tokens behind 2,048 (32 heads of 128) 231.7 us.
+// One B200: a prompt of 2,048 tokens (32 / 4 heads of 64) 51.6 us, 2,048 tokens behind 2,048 (32 heads of 128) 201 us, 61 tokens behind 3,001
+// (32 / 8 heads of 128) 30.1 us (97.6 with one block a tile).
 
 #include "cache8.cuh"
+
+#include <cuda_fp16.h>
 
 #ifndef HEAD_DIM
 #define HEAD_DIM 64
@@ -39,23 +49,28 @@ constexpr int BM = 128;          // packed rows per tile (one softmax group)
 constexpr int TILES = 2;         // tiles per block: both read every converted key and value tile
 constexpr int BLOCK_ROWS = TILES * BM;
 constexpr int BN = 128;          // keys per block
-constexpr int SUB = 128 * 128;   // bytes of a [128 rows x 64 bf16] swizzled sub-tile
+constexpr int SUB = 128 * 128;   // bytes of a [128 rows x 64 halves] swizzled sub-tile
 constexpr int Q_BYTES = KA * SUB;        // one tile's queries
 constexpr int TILE_BYTES = KA * SUB;     // one key tile or one value tile
-constexpr int P_BYTES = 2 * SUB;         // [128 rows x 128 keys] as two sub-tiles
-constexpr int SLOTS = HEAD_DIM == 64 ? 6 : 3;   // key and value tiles in flight (what shared memory allows)
+constexpr int SLOTS = HEAD_DIM == 64 ? 10 : 5;   // key and value tiles in flight (what shared memory allows)
 constexpr int SOFTMAX_THREADS = 128 * TILES, CONVERT_THREADS = 128;
-constexpr int MMA_WARP = SOFTMAX_THREADS / 32;
-constexpr int NUM_THREADS = SOFTMAX_THREADS + 32 + CONVERT_THREADS;   // warps 0-7 softmax, 8 MMA, 9-12 converters
-constexpr int TMEM_COLS = 256 * TILES;
-constexpr int O_COL = TILES * BN;  // first tensor-memory column of the P V results (the S buffers lie before it)
+constexpr int CONVERT_WARP = SOFTMAX_THREADS / 32, MMA_WARP = CONVERT_WARP + CONVERT_THREADS / 32;
+constexpr int NUM_THREADS = (MMA_WARP + 1) * 32;   // warps 0-7 softmax, 8-11 converters, 12 MMA
 constexpr int GROUP_THREADS = 128;
-constexpr int S_PIECE = 64;      // columns of S a softmax thread holds in registers at a time (one sub-tile of P)
+constexpr int S_PIECE = 64;      // columns of S a softmax thread holds in registers at a time
+constexpr bool SHARED_COLUMNS = HEAD_DIM == 128;   // whether P lies in the columns of S
+constexpr int TMEM_COLS = 512, O_COL = TILES * BN, P_COL = O_COL + TILES * D;
 constexpr unsigned long long WAIT_LIMIT_NS = 1000000000ull;
-constexpr size_t SMEM_BYTES = TILES * Q_BYTES + SLOTS * TILE_BYTES + TILES * P_BYTES + 256;   // 2 * SLOTS + 10 barriers, 2 words
+constexpr float RESCALE_STEP = 8.0f;
 // What a converter thread fetches of a tile: 16 codes (chunk ct % CHUNKS) of rows ct / CHUNKS + i * STRIDE, i < CHUNKS.
 constexpr int CHUNKS = D / 16, STRIDE = CONVERT_THREADS / CHUNKS;
 constexpr int BLOCKS = BN / SCALE_TOKENS;   // scale blocks of a key block
+constexpr int EXPONENTS = 8;                // key blocks whose exponents are kept (more than can be in flight)
+constexpr int STATE = D + 4;                // floats of a row's state in a merge: D sums, the maximum, the sum
+constexpr size_t TILES_BYTES = (size_t)TILES * Q_BYTES + (size_t)SLOTS * TILE_BYTES;
+static_assert((size_t)BLOCK_ROWS * STATE * 4 <= TILES_BYTES, "the states of a merge lie over the tiles");
+constexpr size_t SMEM_BYTES = TILES_BYTES + 512;
+static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
@@ -91,11 +106,6 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
-  const int bytes = valid ? 16 : 0;  // 0: the 16 bytes are filled with zeros
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-
 // Byte offset of the 16-byte chunk `chunk` (0..7) of row `row` inside a [rows x 64 bf16] sub-tile
 // with the 128-byte swizzle: rows are 128 bytes, groups of 8 rows are 1024 bytes, and the chunk
 // index is XORed with the row's index inside its group.
@@ -104,29 +114,35 @@ __device__ __forceinline__ uint32_t swizzled(int row, int chunk) {
 }
 
 // Shared-memory matrix descriptor, 128-byte swizzle, 1024 bytes between 8-row groups.
-__device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t addr) {
+__device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t addr, uint32_t leading = 16) {
   uint64_t d = 0;
   d |= (uint64_t)((addr & 0x3FFFF) >> 4);
-  d |= (uint64_t)1 << 16;
+  d |= (uint64_t)(leading >> 4) << 16;      // MN-major operands: bytes from one 64-wide sub-tile to the next
   d |= (uint64_t)(1024 >> 4) << 32;
   d |= (uint64_t)1 << 46;
   d |= (uint64_t)2 << 61;
   return d;
 }
 
-// float32 accumulator, bfloat16 operands, A K-major; B K-major or (b_mn = 1) MN-major.
+// float32 accumulator, half operands, A K-major; B K-major or (b_mn = 1) MN-major.
 __host__ __device__ constexpr uint32_t instr_desc(int m, int n, int b_mn) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) |
-         ((uint32_t)(m >> 4) << 24);
+  return (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-__device__ __forceinline__ void umma_bf16(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
-                                          uint32_t accumulate) {
+__device__ __forceinline__ void umma_ss(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
       ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// The A operand in tensor memory: lane = row, 32-bit column c = its elements 2 c and 2 c + 1.
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
 }
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
@@ -160,20 +176,44 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return y;
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&v);
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
 }
-
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// Four codes as four halves.
+__device__ __forceinline__ void halves(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi) : "r"(codes));
+}
+__device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+// 2^-d twice as a half (zero where a half has no such number).
+__device__ __forceinline__ uint32_t half_power(int d) {
+  const uint32_t h = d <= 14 ? (uint32_t)(15 - d) << 10 : d <= 24 ? 1u << (24 - d) : 0u;
+  return h | (h << 16);
+}
+__device__ __forceinline__ uint32_t peer_smem(uint32_t local, uint32_t rank) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
+  return remote;
+}
+__device__ __forceinline__ float4 load_peer4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
 
 struct AttnArgs {
   const __nv_bfloat16* q;      // [tokens, q_heads, D]
   __nv_bfloat16* out;          // [tokens, q_heads * D]
   Cache8 cache;
-  const int32_t* seq_q_start;
-  const int32_t* seq_q_len;
-  const int32_t* seq_kv_len;
-  const int32_t* tile_seq;     // per tile: batch sequence (-1: nothing to do)
-  const int32_t* tile_index;   // per tile: which tile of BLOCK_ROWS of the sequence's packed rows
+  StepLists lists;
   int q_heads;
   float scale_log2;
   int window;
@@ -181,23 +221,10 @@ struct AttnArgs {
   int* error_word;
 };
 
-// Four codes as bfloat16 numbers: a code's exponent and fraction four places to the right are a bfloat16 2^120 times too small
-// (its subnormals included), which the factor f1 = 2^(120 + e) mends; f2 (1 but for scales above 2^7) is the rest of the scale.
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-__device__ __forceinline__ void bf16_of_codes(uint32_t codes, uint32_t f1, uint32_t& lo, uint32_t& hi) {
-  const uint32_t a = __byte_perm(codes, 0, 0x1404), b = __byte_perm(codes, 0, 0x3424);
-  lo = mul_bf16x2((a & 0x80008000u) | ((a >> 4) & 0x07f007f0u), f1);
-  hi = mul_bf16x2((b & 0x80008000u) | ((b >> 4) & 0x07f007f0u), f1);
-}
-
 constexpr int ERR_CONVERT = 41, ERR_MMA = 42, ERR_SOFTMAX = 43, ERR_LAYOUT = 44;
 
 // EXTRAS: whether a window, blocks of positions, a sink or a gate may be asked for; without them their code is
-// not there.
+// not there.  gridDim.z blocks (a cluster) share a tile's key blocks.
 template <bool EXTRAS>
 __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const AttnArgs a) {
   const AttentionExtras extras = EXTRAS ? a.extras : AttentionExtras{0, nullptr, nullptr, 0};
@@ -205,59 +232,63 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const Att
   extern __shared__ __align__(1024) uint8_t smem[];   // swizzled tiles need 1024-byte alignment (checked below)
   uint8_t* q_smem = smem;                              // [TILES][KA sub-tiles]
   uint8_t* ring = q_smem + TILES * Q_BYTES;            // [SLOTS][KA sub-tiles]: key and value tiles in turn
-  uint8_t* p_smem = ring + SLOTS * TILE_BYTES;         // [TILES][two sub-tiles of 64 keys]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(p_smem + TILES * P_BYTES);
-  uint64_t* tile_full = bars;               // [SLOTS] converters -> MMA: the slot's tile is written
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + TILES_BYTES);
+  uint64_t* tile_full = bars;               // [SLOTS] converters -> MMA (and softmax): the slot's tile is written
   uint64_t* tile_empty = tile_full + SLOTS; // [SLOTS] MMA (commit) -> converters
   uint64_t* q_full = tile_empty + SLOTS;    // [2] softmax group -> MMA: Q_g staged
   uint64_t* s_full = q_full + 2;            // [2] MMA (commit) -> softmax, per group
-  uint64_t* p_full = s_full + 2;            // [2] softmax -> MMA: P written, per group
-  uint64_t* o_full = p_full + 2;            // [2] MMA (commit) -> softmax, per group: P(i) V is complete
-  uint64_t* s_free = o_full + 2;            // [2] softmax -> MMA: the group holds its S values in registers
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_free + 2);
+  uint64_t* s_free = s_full + 2;            // [2] softmax -> MMA: the group holds its S values in registers (P in columns of its own)
+  uint64_t* p_full = s_free + 2;            // [2][2] softmax -> MMA: half h of P written, per group
+  uint64_t* pv_done = p_full + 4;           // [2][2] MMA (commit) -> softmax: the product with half h is complete, per group
+  int2* exponents = reinterpret_cast<int2*>(pv_done + 4);   // [EXPONENTS] of a key block's keys and values
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(exponents + EXPONENTS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // ---- what this block works on (uniform across the cluster).  The step's lists are there before its kernels start, so they may
+  // be read ahead of pdl_wait().  Blocks are handed out with x fastest: all key/value heads of the latest tile first (it sees
+  // the most keys), then of the tile before it, ...
+  const int tile = gridDim.y - 1 - blockIdx.y, kvh = blockIdx.x;
+  const int seq = a.lists.tile_seq[tile];
+  if (seq < 0) {
+    pdl_wait();
+    return;
+  }
   if (smem_u32(smem) & 1023) {   // never seen; refuse rather than compute with a broken layout
     if (threadIdx.x == 0) atomicCAS(a.error_word, 0, ERR_LAYOUT);
     return;
   }
-  // ---- what this block works on (uniform across the block).  The tile list and the requests'
-  // lengths are written by the host before the step's first kernel, so they may be read ahead of
-  // pdl_wait(); their latency then hides behind the barrier set-up and the tensor-memory allocation.
-  // blocks are handed out with x fastest: all key/value heads of the latest tile first (it sees
-  // the most keys), then of the tile before it, ... so the longest blocks of the whole grid start first
-  const int tile = gridDim.y - 1 - blockIdx.y, kvh = blockIdx.x;
-  const int seq = a.tile_seq[tile];
-  int q_start = 0, q_len = 0, kv_len = 0, row0 = 0, n_rows = 0, pos0 = 0, group = 1;
+  const int group = a.q_heads / a.cache.kv_heads;
+  const int q_start = a.lists.seq_q_start[seq], q_len = a.lists.seq_q_len[seq], kv_len = a.lists.seq_kv_len[seq];
+  const int row0 = a.lists.tile_index[tile] * BLOCK_ROWS, n_rows = q_len * group, pos0 = kv_len - q_len;
   // per group (tile of 128 rows): its key blocks [g_lo, g_hi) and the positions of its first and last row
   int g_lo[TILES] = {}, g_hi[TILES] = {}, g_min_pos[TILES] = {}, g_max_pos[TILES] = {};
-  int kb_lo = 0, n_kb = 0;   // the union of the two ranges: what the converters bring
-  if (seq >= 0) {
-    group = a.q_heads / a.cache.kv_heads;
-    q_start = a.seq_q_start[seq];
-    q_len = a.seq_q_len[seq];
-    kv_len = a.seq_kv_len[seq];
-    row0 = a.tile_index[tile] * BLOCK_ROWS;
-    n_rows = q_len * group;
-    pos0 = kv_len - q_len;
-    int lo_all = 1 << 30, hi_all = 0;
+  int kb_lo = 1 << 30, kb_hi = 0;   // the union of the two ranges, then this block's share of it
+#pragma unroll
+  for (int g = 0; g < TILES; ++g) {
+    const int first_row = row0 + g * BM;
+    if (first_row >= n_rows) continue;
+    g_min_pos[g] = pos0 + first_row / group;
+    g_max_pos[g] = pos0 + min(q_len - 1, (first_row + BM - 1) / group);
+    g_lo[g] = first_visible_key(g_min_pos[g], window, extras.chunk) / BN;
+    g_hi[g] = g_max_pos[g] / BN + 1;
+    kb_lo = min(kb_lo, g_lo[g]);
+    kb_hi = max(kb_hi, g_hi[g]);
+  }
+  const int n_splits = gridDim.z, split = blockIdx.z;
+  if (n_splits > 1) {
+    const int n = kb_hi - kb_lo, from = kb_lo + n * split / n_splits;
+    kb_hi = kb_lo + n * (split + 1) / n_splits;
+    kb_lo = from;
 #pragma unroll
     for (int g = 0; g < TILES; ++g) {
-      const int first_row = row0 + g * BM;
-      if (first_row >= n_rows) continue;
-      const int first_token = first_row / group, last_token = min(q_len - 1, (first_row + BM - 1) / group);
-      g_min_pos[g] = pos0 + first_token;
-      g_max_pos[g] = pos0 + last_token;
-      const int lo_key = first_visible_key(g_min_pos[g], window, extras.chunk);
-      g_lo[g] = lo_key / BN;
-      g_hi[g] = g_max_pos[g] / BN + 1;
-      lo_all = min(lo_all, g_lo[g]);
-      hi_all = max(hi_all, g_hi[g]);
+      g_lo[g] = max(g_lo[g], kb_lo);
+      g_hi[g] = max(g_lo[g], min(g_hi[g], kb_hi));
     }
-    if (hi_all > 0) kb_lo = lo_all, n_kb = hi_all - lo_all;
   }
+  const int n_kb = kb_hi - kb_lo;
+
   if (threadIdx.x == 0) {
     for (int s = 0; s < SLOTS; ++s) {
       mbar_init(&tile_full[s], CONVERT_THREADS / 32);
@@ -266,9 +297,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const Att
     for (int b = 0; b < 2; ++b) {
       mbar_init(&q_full[b], GROUP_THREADS);
       mbar_init(&s_full[b], 1);
-      mbar_init(&p_full[b], GROUP_THREADS);
-      mbar_init(&o_full[b], 1);
       mbar_init(&s_free[b], GROUP_THREADS);
+    }
+    for (int b = 0; b < 4; ++b) {
+      mbar_init(&p_full[b], GROUP_THREADS);
+      mbar_init(&pv_done[b], 1);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -283,62 +316,74 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const Att
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = *tmem_slot;
   pdl_wait();      // (the MMA issuer too: the limit of its waits counts from here)
-  if (warp > MMA_WARP) {
+
+  // What a softmax thread carries to the end: its row's state.
+  const int g = (warp >> 2) & 1, r = (warp & 3) * 32 + lane, R = row0 + g * BM + r;     // warps 0-7
+  const bool row_valid = R < n_rows;
+  const int token = row_valid ? R / group : 0, head = row_valid ? kvh * group + R % group : 0;
+  const uint32_t lane_addr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16), o_addr = lane_addr + O_COL + g * D;
+  float m = -INFINITY, l = 0.0f;
+  const int my_lo = g ? g_lo[1] : g_lo[0], my_n = (g ? g_hi[1] : g_hi[0]) - my_lo;
+
+  if (warp >= CONVERT_WARP && warp < MMA_WARP) {
     // ------------------------------------------------------------------ converters
     // Tile n of the ring is the keys (n even) or the values (n odd) of key block n / 2.  A tile's codes are asked for one tile ahead of
-    // their conversion, and where a key block's scale blocks lie one tile before that.  Positions of no page (given back by a
+    // their conversion, and where a key block's scale blocks lie two tiles before that.  Positions of no page (given back by a
     // window) and behind the request's last key become zeros: their keys are masked, but zero times whatever lies there must be zero.
-    const int ct = threadIdx.x - (MMA_WARP + 1) * 32, chunk = ct % CHUNKS, row0 = ct / CHUNKS;
+    const int ct = threadIdx.x - CONVERT_WARP * 32, chunk = ct % CHUNKS, first_row = ct / CHUNKS;
+    auto find_page = [&](int jj) {      // of a key block, lane b: the page of its scale block b, -1 if none
+      const int key = (kb_lo + jj) * BN + lane * SCALE_TOKENS;
+      return lane < BLOCKS && jj < n_kb && key < kv_len ? page_of(a.cache, seq, key) : -1;
+    };
     struct Place {             // of a key block, lane b: its scale block b (the same for keys and values)
       long long at;            // codes from the cache's first, or -1
       float k_scale, v_scale;
     };
-    auto look_up = [&](int jj) {
+    auto place = [&](int jj, int page) {
       Place p{-1, 0.0f, 0.0f};
-      const int key = (kb_lo + jj) * BN + lane * SCALE_TOKENS;
-      if (lane < BLOCKS && jj < n_kb && key < kv_len) {
-        const int page = page_of(a.cache, seq, key);
-        if (page >= 0) {
-          const int in_page = key % a.cache.page_tokens;
-          p.at = (long long)page * a.cache.page_stride + ((long long)kvh * a.cache.page_tokens + in_page) * D;
-          const long long s = (long long)page * a.cache.scale_stride + (long long)kvh * (a.cache.page_tokens / SCALE_TOKENS) + in_page / SCALE_TOKENS;
-          p.k_scale = __ldcg(a.cache.k_scale + s);
-          p.v_scale = __ldcg(a.cache.v_scale + s);
-        }
+      if (page >= 0) {
+        const int in_page = ((kb_lo + jj) * BN + lane * SCALE_TOKENS) % a.cache.page_tokens;
+        p.at = (long long)page * a.cache.page_stride + ((long long)kvh * a.cache.page_tokens + in_page) * D;
+        const long long s = (long long)page * a.cache.scale_stride + (long long)kvh * (a.cache.page_tokens / SCALE_TOKENS) + in_page / SCALE_TOKENS;
+        p.k_scale = __ldcg(a.cache.k_scale + s);
+        p.v_scale = __ldcg(a.cache.v_scale + s);
       }
       return p;
     };
-    auto block_of = [&](int i) { return (row0 + i * STRIDE) / SCALE_TOKENS; };      // the same for a whole warp
+    auto block_of = [&](int i) { return (first_row + i * STRIDE) / SCALE_TOKENS; };      // the same for a whole warp
     auto fetch = [&](uint4 (&raw)[CHUNKS], const Place& p, int n) {
       const uint8_t* base = (n & 1) ? a.cache.v : a.cache.k;
       const int key0 = (kb_lo + (n >> 1)) * BN;
 #pragma unroll
       for (int i = 0; i < CHUNKS; ++i) {
-        const int row = row0 + i * STRIDE;
+        const int row = first_row + i * STRIDE;
         const long long at = __shfl_sync(0xffffffffu, p.at, block_of(i));
         raw[i] = make_uint4(0, 0, 0, 0);
         if (at >= 0 && key0 + row < kv_len) raw[i] = __ldcg(reinterpret_cast<const uint4*>(base + at + (row % SCALE_TOKENS) * D + chunk * 16));
       }
     };
-    auto convert = [&](const uint4 (&raw)[CHUNKS], const Place& p, int n) {
+    // What is left of a scale block's factor once the largest exponent of its key block is taken out, and that exponent.
+    auto split_scale = [&](const Place& p, float scale, int& most) {
+      const bool lost = isnan(scale), there = p.at >= 0 && !lost;
+      const int e = there ? exponent_of(scale) : -1000;
+      most = __reduce_max_sync(0xffffffffu, e);
+      if (most == -1000) most = 0;
+      return lost ? 0x7e007e00u : there ? half_power(most - e) : 0u;
+    };
+    auto convert = [&](const uint4 (&raw)[CHUNKS], uint32_t factors, int n) {
       const uint32_t base = smem_u32(ring) + (n % SLOTS) * TILE_BYTES + (chunk >> 2) * SUB;
-      const float scale = (n & 1) ? p.v_scale : p.k_scale;
 #pragma unroll
       for (int i = 0; i < CHUNKS; ++i) {
-        const int row = row0 + i * STRIDE;
-        const float s = __shfl_sync(0xffffffffu, scale, block_of(i));
-        const int e = exponent_of(s);
-        const float f = isnan(s) ? s : power_of_two(min(max(e, SCALE_LEAST), 7) + 120);
-        const uint32_t f1 = __byte_perm(__float_as_uint(f), 0, 0x3232);
+        const int row = first_row + i * STRIDE;
+        const uint32_t f = __shfl_sync(0xffffffffu, factors, block_of(i));
         uint32_t w[8];
-        bf16_of_codes(raw[i].x, f1, w[0], w[1]);
-        bf16_of_codes(raw[i].y, f1, w[2], w[3]);
-        bf16_of_codes(raw[i].z, f1, w[4], w[5]);
-        bf16_of_codes(raw[i].w, f1, w[6], w[7]);
-        if (e > 7) {           // rare, and the same for the whole warp
-          const uint32_t f2 = __byte_perm(__float_as_uint(power_of_two(min(e, 127) - 7)), 0, 0x3232);
+        halves(raw[i].x, w[0], w[1]);
+        halves(raw[i].y, w[2], w[3]);
+        halves(raw[i].z, w[4], w[5]);
+        halves(raw[i].w, w[6], w[7]);
+        if (f != 0x3c003c00u) {       // the same for the whole warp
 #pragma unroll
-          for (int k = 0; k < 8; ++k) w[k] = mul_bf16x2(w[k], f2);
+          for (int k = 0; k < 8; ++k) w[k] = mul_half2(w[k], f);
         }
         // two 16-byte chunks of the row; threads of odd sub-tiles store theirs the other way round, so that the eight that share a row
         // (or two rows, at head size 64) meet eight different groups of banks
@@ -349,25 +394,30 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const Att
       }
     };
     bool ok = true;
-    auto deliver = [&](const uint4 (&raw)[CHUNKS], const Place& p, int n) {
+    auto deliver = [&](const uint4 (&raw)[CHUNKS], uint32_t factors, int n) {
       const uint32_t use = (uint32_t)(n / SLOTS);   // how often the slot was filled before
       ok = ok && (use == 0 || mbar_wait(&tile_empty[n % SLOTS], (use - 1) & 1, abort_flag));
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) return;
-      convert(raw, p, n);
+      convert(raw, factors, n);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&tile_full[n % SLOTS]);
     };
     uint4 keys[CHUNKS], values[CHUNKS];
-    Place now = look_up(0);
+    Place now = place(0, find_page(0));
+    int page = find_page(1);
     if (n_kb > 0) fetch(keys, now, 0);
     for (int jj = 0; jj < n_kb && ok; ++jj) {
       fetch(values, now, 2 * jj + 1);
-      const Place next = look_up(jj + 1);
-      deliver(keys, now, 2 * jj);
+      const Place next = place(jj + 1, page);
+      page = find_page(jj + 2);
+      int ek, ev;
+      const uint32_t fk = split_scale(now, now.k_scale, ek), fv = split_scale(now, now.v_scale, ev);
+      if (warp == CONVERT_WARP && lane == 0) exponents[jj % EXPONENTS] = make_int2(ek, ev);
+      deliver(keys, fk, 2 * jj);
       if (jj + 1 < n_kb) fetch(keys, next, 2 * jj + 2);
-      deliver(values, now, 2 * jj + 1);
+      deliver(values, fv, 2 * jj + 1);
       now = next;
     }
     if (!ok && lane == 0) {
@@ -378,7 +428,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const Att
     // ------------------------------------------------------------------ MMA issuer
     if (n_kb > 0 && elect_one()) {
       constexpr uint32_t idesc_s = instr_desc(BM, BN, 0);
-      constexpr uint32_t idesc_o = instr_desc(BM, 64, 1);
+      constexpr uint32_t idesc_o = instr_desc(BM, D, 1);
       auto active = [&](int g, int jj) { return kb_lo + jj >= g_lo[g] && kb_lo + jj < g_hi[g]; };
       // S_g = Q_g K(jj)^T into group g's S buffer; `last`: no product after this one reads the key tile
       auto issue_s = [&](int g, int jj, bool last) {
@@ -389,46 +439,35 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const Att
         for (int at = 0; at < KA; ++at)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            umma_bf16(tmem_base + g * BN, smem_desc_sw128(q_addr + at * SUB) + 2 * k,
-                      smem_desc_sw128(k_addr + at * SUB) + 2 * k, idesc_s, (at > 0 || k > 0) ? 1u : 0u);
+            umma_ss(tmem_base + g * BN, smem_desc_sw128(q_addr + at * SUB) + 2 * k, smem_desc_sw128(k_addr + at * SUB) + 2 * k, idesc_s,
+                    (at > 0 || k > 0) ? 1u : 0u);
         umma_commit(&s_full[g]);
         if (last) umma_commit(&tile_empty[slot]);
       };
-      // O_g (+)= P_g V(jj): the group's O accumulates in tensor memory over its key blocks (`first`: overwrite)
-      auto issue_pv = [&](int g, int jj, bool last, int i) {     // i: the group's i-th key block
+      // O_g (+)= half h of P_g V(jj): the group's O accumulates in tensor memory over its key blocks (`first`: overwrite)
+      auto issue_pv = [&](int g, int jj, int h, bool last, bool first) {
         const int slot = (2 * jj + 1) % SLOTS;
-        const bool first = i == 0;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t v_addr = smem_u32(ring) + slot * TILE_BYTES;
-        const uint32_t p_addr = smem_u32(p_smem) + g * P_BYTES;
+        const uint32_t p_addr = tmem_base + (SHARED_COLUMNS ? g * BN + h * S_PIECE : P_COL + g * (BN / 2) + h * (S_PIECE / 2));
 #pragma unroll
-        for (int vt = 0; vt < KA; ++vt)
-#pragma unroll
-          for (int kk = 0; kk < BN / 16; ++kk)
-            umma_bf16(tmem_base + O_COL + g * D + vt * 64, smem_desc_sw128(p_addr + (kk >> 2) * SUB) + 2 * (kk & 3),
-                      smem_desc_sw128(v_addr + vt * SUB) + (uint64_t)(kk * 2048 >> 4), idesc_o, (kk > 0 || !first) ? 1u : 0u);
-        umma_commit(&o_full[g]);
+        for (int kk = 0; kk < S_PIECE / 16; ++kk)
+          umma_ts(tmem_base + O_COL + g * D, p_addr + kk * 8, smem_desc_sw128(v_addr, SUB) + (uint64_t)((h * (S_PIECE / 16) + kk) * 2048 >> 4),
+                  idesc_o, (kk > 0 || !first) ? 1u : 0u);
+        umma_commit(&pv_done[g * 2 + h]);
         if (last) umma_commit(&tile_empty[slot]);
       };
-      // The two groups are served as they come: a group's next S as soon as it reports that it holds the
-      // S before it in registers (and the key tile has landed), its P V as soon as it reports P (and has
-      // read the O_block before).  Nothing is waited for while the other group could be served.
+      // The two groups are served as they come.  Nothing is waited for while the other group could be served.
       bool ok = true;
-      int s_next[TILES] = {}, pv_next[TILES] = {};      // per group: its next block to issue S / P V for
+      int s_next[TILES] = {}, pv_next[TILES] = {};      // per group: its next block to issue S for, its next half block to issue P V for
       int n_g[TILES];
 #pragma unroll
       for (int g = 0; g < TILES; ++g) n_g[g] = g_hi[g] - g_lo[g];
-      auto unfinished = [&]() {
-        bool any = false;
-#pragma unroll
-        for (int g = 0; g < TILES; ++g) any = any || pv_next[g] < n_g[g];
-        return any;
-      };
       // Whether tile n has landed.  A barrier's parity tells one filling of a slot only from the one before it.
       // Groups that start with the same key block ask for the tiles as the slots are filled.  A group whose
       // first key block lies behind the other's (a window, or a later block of positions) would take an
       // earlier filling for its own: there the tiles are counted off in order.
-      const bool counted = EXTRAS && g_lo[0] != g_lo[TILES - 1];
+      const bool counted = EXTRAS && g_lo[0] != g_lo[1];
       int arrived = 0, arrived_slot = 0;
       uint32_t arrived_parity = 0;
       auto landed = [&](int n) {
@@ -442,29 +481,35 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const Att
         }
         return mbar_try_wait(&tile_full[n % SLOTS], (n / SLOTS) & 1);
       };
+      // whether group g's S buffer may be written for its block i
+      auto s_ready = [&](int g, int i) {
+        if (i == 0) return mbar_try_wait(&q_full[g], 0);
+        if (SHARED_COLUMNS) return pv_next[g] == 2 * i && mbar_try_wait(&pv_done[g * 2 + 1], (i - 1) & 1);   // (and with it half 0)
+        return mbar_try_wait(&s_free[g], (i - 1) & 1);
+      };
       unsigned long long idle_since = 0;
       unsigned idle_spins = 0;
-      while (ok && unfinished()) {
+      while (ok && (pv_next[0] < 2 * n_g[0] || pv_next[1] < 2 * n_g[1])) {
         bool progress = false;
 #pragma unroll
         for (int g = 0; g < TILES; ++g) {
           const int o = 1 - g;   // the other group
-          if (s_next[g] < n_g[g]) {
-            const int i = s_next[g], jj = g_lo[g] + i - kb_lo;
-            if ((i == 0 ? mbar_try_wait(&q_full[g], 0) : mbar_try_wait(&s_free[g], (i - 1) & 1)) && landed(2 * jj)) {
-              // the other group is done with K(jj) if it never reads it or has issued its S for it already
-              const bool last = !active(o, jj) || s_next[o] > kb_lo + jj - g_lo[o];
-              issue_s(g, jj, last);
-              s_next[g] = i + 1;
+          if (pv_next[g] < 2 * s_next[g]) {
+            const int i = pv_next[g] >> 1, h = pv_next[g] & 1, jj = g_lo[g] + i - kb_lo;
+            if (mbar_try_wait(&p_full[g * 2 + h], (uint32_t)i & 1u) && landed(2 * jj + 1)) {
+              // the other group is done with V(jj) if it never reads it or has issued its product already
+              const bool last = h == 1 && (!active(o, jj) || pv_next[o] > 2 * (kb_lo + jj - g_lo[o]) + 1);
+              issue_pv(g, jj, h, last, pv_next[g] == 0);
+              ++pv_next[g];
               progress = true;
             }
           }
-          if (pv_next[g] < s_next[g]) {
-            const int i = pv_next[g], jj = g_lo[g] + i - kb_lo;
-            if (mbar_try_wait(&p_full[g], (uint32_t)i & 1u) && landed(2 * jj + 1)) {
-              const bool last = !active(o, jj) || pv_next[o] > kb_lo + jj - g_lo[o];
-              issue_pv(g, jj, last, i);
-              pv_next[g] = i + 1;
+          if (s_next[g] < n_g[g]) {
+            const int i = s_next[g], jj = g_lo[g] + i - kb_lo;
+            if (s_ready(g, i) && landed(2 * jj)) {
+              const bool last = !active(o, jj) || s_next[o] > kb_lo + jj - g_lo[o];
+              issue_s(g, jj, last);
+              s_next[g] = i + 1;
               progress = true;
             }
           }
@@ -480,67 +525,65 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const Att
         *abort_flag = 1;
         atomicCAS(a.error_word, 0, ERR_MMA);
         for (int b = 0; b < TILES; ++b) umma_commit(&s_full[b]);   // release whoever waits
-        for (int b = 0; b < TILES; ++b) umma_commit(&o_full[b]);
+        for (int b = 0; b < 2 * TILES; ++b) umma_commit(&pv_done[b]);
       }
     }
   } else {
     // ------------------------------------------------------------------ softmax: group g owns tile g, one thread per row
-    const int quad = warp & 3, g = warp >> 2;        // tensor-memory lanes 32 * quad ..
-    const int gt = threadIdx.x & (GROUP_THREADS - 1);
-    const int tile_row0 = row0 + g * BM;
-    // Q_g: 128 rows x D in 16-byte chunks, staged by the group's threads (a few chunks each, so one
-    // round of global latency); rows past the request's packed rows are zero
-    for (int i = gt; i < BM * (D / 8); i += GROUP_THREADS) {
-      const int qr = i / (D / 8), c = i % (D / 8);
-      const int QR = tile_row0 + qr;
-      const bool valid = seq >= 0 && QR < n_rows;
-      const int token = valid ? QR / group : 0, head = valid ? kvh * group + QR % group : 0;
-      const __nv_bfloat16* src = a.q + ((long long)(q_start + token) * a.q_heads + head) * D + c * 8;
-      cp_async16(smem_u32(q_smem) + g * Q_BYTES + (c >> 3) * SUB + swizzled(qr, c & 7), src, valid);
+    float factor;       // scale * log2(e), times the power of two that was taken out of the row's queries
+    {
+      uint4 raw[D / 8];
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) raw[c] = make_uint4(0, 0, 0, 0);
+      if (row_valid) {
+        const uint4* src = reinterpret_cast<const uint4*>(a.q + ((long long)(q_start + token) * a.q_heads + head) * D);
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) raw[c] = __ldg(src + c);
+      }
+      const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(raw);
+      float most = 0.0f;
+#pragma unroll
+      for (int i = 0; i < D / 2; ++i) most = fmaxf(most, fmaxf(fabsf(__low2float(pairs[i])), fabsf(__high2float(pairs[i]))));
+      const int e = most > 0.0f ? min(max(exponent_of(most) - 10, -100), 116) : 0;     // the largest entry to [2^10, 2^11)
+      const float down = power_of_two(-e);
+      factor = a.scale_log2 * power_of_two(e);
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = pack_half(__low2float(pairs[4 * c + i]) * down, __high2float(pairs[4 * c + i]) * down);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(q_smem) + g * Q_BYTES + (c >> 3) * SUB + swizzled(r, c & 7)),
+                     "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+      }
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     mbar_arrive(&q_full[g]);
-    const int r = quad * 32 + lane;                  // row of the tile = tensor-memory lane
-    const int R = tile_row0 + r;
-    const bool row_valid = seq >= 0 && R < n_rows;
-    const int row_pos = row_valid ? pos0 + R / group : -1;
-    const uint32_t lane_addr = tmem_base + ((uint32_t)(quad * 32) << 16);
-    const uint32_t s_addr = lane_addr + g * BN, o_addr = lane_addr + O_COL + g * D;
-    const int my_lo = g_lo[g], my_n = g_hi[g] - g_lo[g];
+    const int row_pos = row_valid ? pos0 + token : -1;
+    const uint32_t s_addr = lane_addr + g * BN;
     const int row_lo = first_visible_key(row_pos, window, extras.chunk);
-    const int tile_min_pos = g_min_pos[g];
-    const int tile_max_lo = first_visible_key(g_max_pos[g], window, extras.chunk);   // from here on no row's bound hides a key
-    // Running softmax of the row.  `m` is the maximum the exponentials are taken against; it follows the
-    // true maximum only when that has grown by more than RESCALE_STEP (in base-2 units), so that O, which
-    // accumulates in tensor memory over all key blocks, has to be rescaled rarely: with a stale maximum
-    // the probabilities reach at most 2^RESCALE_STEP, and since sum and O are taken against the same `m`
-    // their quotient is exact either way.
-    constexpr float RESCALE_STEP = 8.0f;
-    float m = -INFINITY, l = 0.0f;
-    // this row of the group's P tiles (swizzled: chunk c of row r lies at c ^ (r % 8) inside the row's 128 bytes)
-    const uint32_t p_row = smem_u32(p_smem) + g * P_BYTES + (r >> 3) * 1024 + (r & 7) * 128, p_xor = (uint32_t)(r & 7) << 4;
-    // P(k) V of this group is complete
-    auto wait_pv = [&](int k) { return mbar_wait(&o_full[g], (uint32_t)k & 1u, abort_flag); };
+    const int tile_min_pos = g ? g_min_pos[1] : g_min_pos[0];
+    const int tile_max_lo = first_visible_key(g ? g_max_pos[1] : g_max_pos[0], window, extras.chunk);   // from here on no row's bound hides a key
+    // the product with half h of this group's block k is complete
+    auto wait_pv = [&](int k, int h) { return mbar_wait(&pv_done[g * 2 + h], (uint32_t)k & 1u, abort_flag); };
     bool ok = true;
     for (int i = 0; i < my_n && ok; ++i) {
-      const int key0 = (my_lo + i) * BN;
-      ok = mbar_wait(&s_full[g], i & 1, abort_flag) && !*abort_flag;
+      const int jj = my_lo + i - kb_lo, key0 = (my_lo + i) * BN, v_tile = 2 * jj + 1;
+      // the exponents were written ahead of the value tile (which stays until this group has read it)
+      ok = mbar_wait(&s_full[g], i & 1, abort_flag) && mbar_wait(&tile_full[v_tile % SLOTS], (uint32_t)(v_tile / SLOTS) & 1u, abort_flag) &&
+           !*abort_flag;
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const int2 e = exponents[jj % EXPONENTS];
+      const float c = factor * power_of_two(e.x), ev = (float)e.y;
       const bool all_visible = key0 + BN - 1 <= tile_min_pos && (!EXTRAS || key0 >= tile_max_lo);
-      // The row of S is read once, in two pieces of 64 columns (one sub-tile of P each).  Each piece
-      // settles the maximum for itself: should the second piece move it, the probabilities of the
-      // first, which this thread has just written, are rescaled where they lie (rare, as is every move).
       float l0 = 0.0f, l1 = 0.0f, l2 = 0.0f, l3 = 0.0f;
 #pragma unroll
-      for (int h = 0; h < BN / S_PIECE; ++h) {
+      for (int h = 0; h < 2; ++h) {
         uint32_t v[S_PIECE];
 #pragma unroll
-        for (int c = 0; c < S_PIECE; c += 32) tmem_load32_nowait(s_addr + h * S_PIECE + c, v + c);
+        for (int k = 0; k < S_PIECE; k += 32) tmem_load32_nowait(s_addr + h * S_PIECE + k, v + k);
         tmem_wait_loads();
-        if (h == BN / S_PIECE - 1) {   // the last read of S(i): the MMA thread may overwrite the buffer with S(i + 1)
+        if (!SHARED_COLUMNS && h == 1) {   // the last read of S(i): the MMA thread may overwrite the buffer with S(i + 1)
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
           mbar_arrive(&s_free[g]);
         }
@@ -560,12 +603,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const Att
           mx2 = fmaxf(mx2, fmaxf(__uint_as_float(v[k + 4]), __uint_as_float(v[k + 5])));
           mx3 = fmaxf(mx3, fmaxf(__uint_as_float(v[k + 6]), __uint_as_float(v[k + 7])));
         }
-        const float m_new = fmaxf(m, fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * a.scale_log2);   // scale > 0: the maximum commutes with it
+        const float m_new = fmaxf(m, fmaf(fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)), c, ev));   // c > 0: the maximum commutes with it
         // tensor-memory loads and stores are warp-wide: the warp moves its maxima together, as soon as one of
         // its rows has outgrown its own by the step (a row that has not may follow the true maximum just as well)
         const bool move = __any_sync(0xffffffffu, m_new > m + RESCALE_STEP);
-        // P(i) goes where P(i - 1) lay: the product that read it must be complete
-        if (h == 0 && i > 0 && !wait_pv(i - 1)) {
+        if (!SHARED_COLUMNS && i > 0 && !wait_pv(i - 1, h)) {   // half h of P(i) goes where that of P(i - 1) lay
           ok = false;
           break;
         }
@@ -573,22 +615,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const Att
           const float corr = fast_exp2(m - (m_new == -INFINITY ? 0.0f : m_new));   // m = -inf gives 0
           m = m_new;
           l *= corr;
-          if (h > 0) {   // this block's first piece: its partial sums, and its probabilities where this thread wrote them
-            l0 *= corr, l1 *= corr, l2 *= corr, l3 *= corr;
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              const uint32_t at = p_row + ((uint32_t)(c << 4) ^ p_xor);
-              uint32_t w[4];
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const __nv_bfloat162 pair = *reinterpret_cast<const __nv_bfloat162*>(&w[e]);
-                w[e] = pack_bf16(__low2float(pair) * corr, __high2float(pair) * corr);
-              }
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+          l0 *= corr, l1 *= corr, l2 *= corr, l3 *= corr;
+          if (i > 0 || h > 0) {     // O = O * corr in tensor memory, when every product issued so far is complete
+            if (!(h > 0 ? wait_pv(i, 0) : wait_pv(i - 1, 1))) {
+              ok = false;
+              break;
             }
-          }
-          if (i > 0) {     // O = O * corr in tensor memory, between two products (the one before is complete: see above)
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 32) {
@@ -599,49 +631,40 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const Att
               for (int k = 0; k < 32; ++k) t[k] = __float_as_uint(__uint_as_float(t[k]) * corr);
               tmem_store32(o_addr + c0, t);
             }
-            tmem_wait_stores();
           }
         }
-        const float m_use = m == -INFINITY ? 0.0f : m;
-        // probabilities into shared memory as the A operand of P V (sub-tile h of 64 keys); the row's sum
-        // in four independent partial sums
+        const float shift = ev - (m == -INFINITY ? 0.0f : m);
+        uint32_t packed[S_PIECE / 2];
 #pragma unroll
-        for (int c = 0; c < S_PIECE / 8; ++c) {
-          uint32_t packed[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float p0 = fast_exp2(fmaf(__uint_as_float(v[c * 8 + 2 * e]), a.scale_log2, -m_use));
-            const float p1 = fast_exp2(fmaf(__uint_as_float(v[c * 8 + 2 * e + 1]), a.scale_log2, -m_use));
-            if (e == 0) l0 += p0 + p1;
-            else if (e == 1) l1 += p0 + p1;
-            else if (e == 2) l2 += p0 + p1;
-            else l3 += p0 + p1;
-            packed[e] = pack_bf16(p0, p1);
-          }
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p_row + h * SUB + ((uint32_t)(c << 4) ^ p_xor)),
-                       "r"(packed[0]), "r"(packed[1]), "r"(packed[2]), "r"(packed[3]) : "memory");
+        for (int k = 0; k < S_PIECE; k += 2) {
+          const float p0 = fast_exp2(fmaf(__uint_as_float(v[k]), c, shift)), p1 = fast_exp2(fmaf(__uint_as_float(v[k + 1]), c, shift));
+          if ((k & 6) == 0) l0 += p0 + p1;
+          else if ((k & 6) == 2) l1 += p0 + p1;
+          else if ((k & 6) == 4) l2 += p0 + p1;
+          else l3 += p0 + p1;
+          packed[k / 2] = pack_half(p0, p1);
         }
+        tmem_store32(SHARED_COLUMNS ? s_addr + h * S_PIECE : lane_addr + P_COL + g * (BN / 2) + h * (S_PIECE / 2), packed);
+        tmem_wait_stores();
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        mbar_arrive(&p_full[g * 2 + h]);
       }
       if (!ok) break;
-      l += (l0 + l1) + (l2 + l3);
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mbar_arrive(&p_full[g]);
+      l = fmaf((l0 + l1) + (l2 + l3), power_of_two(-e.y), l);
     }
-    if (ok && my_n > 0) ok = wait_pv(my_n - 1) && !*abort_flag;
+    if (ok && my_n > 0) ok = wait_pv(my_n - 1, 1) && !*abort_flag;
     if (!ok) {
       *abort_flag = 1;
       atomicCAS(a.error_word, 0, ERR_SOFTMAX);
     }
-    // ---- every thread finishes its own row: O / l out of tensor memory, rounded to bfloat16, 64 bytes
-    // at a time.  Heads that share a key/value head lie side by side in a token's output row, as their
-    // rows do in the tile.  (The loads are warp-wide, so rows without an output still take part.)
-    if (ok && my_n > 0) {
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const int token = row_valid ? R / group : 0, head = row_valid ? kvh * group + R % group : 0;
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (n_splits == 1 && ok && my_n > 0) {
+      // ---- every thread finishes its own row: O / l out of tensor memory, rounded to bfloat16, 64 bytes
+      // at a time.  Heads that share a key/value head lie side by side in a token's output row, as their
+      // rows do in the tile.  (The loads are warp-wide, so rows without an output still take part.)
       // the sink joins the sum, taken against the same maximum (far above it the sum is infinite, the row zero)
       if (extras.sink && row_valid) l += exp2f(sink_log2(extras, head) - m);
-      const float inv = l > 0.0f ? (row_valid ? head_gate<__nv_bfloat16>(extras, q_start + token, head) : 1.0f) / l : 0.0f;
+      const float inv = l == 0.0f ? 0.0f : (row_valid ? head_gate<__nv_bfloat16>(extras, q_start + token, head) : 1.0f) / l;
       uint4* dst = reinterpret_cast<uint4*>(a.out + ((long long)(q_start + token) * a.q_heads + head) * D);
 #pragma unroll
       for (int c0 = 0; c0 < D; c0 += 32) {
@@ -650,14 +673,64 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const Att
         tmem_wait_loads();
         if (row_valid) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            dst[c0 / 8 + c] = make_uint4(pack_bf16(__uint_as_float(t[8 * c]) * inv, __uint_as_float(t[8 * c + 1]) * inv),
-                                         pack_bf16(__uint_as_float(t[8 * c + 2]) * inv, __uint_as_float(t[8 * c + 3]) * inv),
-                                         pack_bf16(__uint_as_float(t[8 * c + 4]) * inv, __uint_as_float(t[8 * c + 5]) * inv),
-                                         pack_bf16(__uint_as_float(t[8 * c + 6]) * inv, __uint_as_float(t[8 * c + 7]) * inv));
+          for (int k = 0; k < 4; ++k)
+            dst[c0 / 8 + k] = make_uint4(pack_bf16(__uint_as_float(t[8 * k]) * inv, __uint_as_float(t[8 * k + 1]) * inv),
+                                         pack_bf16(__uint_as_float(t[8 * k + 2]) * inv, __uint_as_float(t[8 * k + 3]) * inv),
+                                         pack_bf16(__uint_as_float(t[8 * k + 4]) * inv, __uint_as_float(t[8 * k + 5]) * inv),
+                                         pack_bf16(__uint_as_float(t[8 * k + 6]) * inv, __uint_as_float(t[8 * k + 7]) * inv));
         }
       }
     }
+  }
+  if (n_splits > 1) {
+    // ---- every row's state into this block's shared memory (over the tiles, which no product reads any more), then the rows
+    // r % n_splits == split merged over the cluster's blocks in index order
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    float* states = reinterpret_cast<float*>(smem);        // [BLOCK_ROWS][STATE]
+    if (warp < CONVERT_WARP) {
+      float* row = states + (size_t)(g * BM + r) * STATE;
+#pragma unroll
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t t[32];
+#pragma unroll
+        for (int k = 0; k < 32; ++k) t[k] = 0u;
+        if (my_n > 0) {      // the same for the whole group
+          tmem_load32_nowait(o_addr + c0, t);
+          tmem_wait_loads();
+        }
+#pragma unroll
+        for (int k = 0; k < 32; k += 4)
+          *reinterpret_cast<float4*>(row + c0 + k) = make_float4(__uint_as_float(t[k]), __uint_as_float(t[k + 1]), __uint_as_float(t[k + 2]),
+                                                                 __uint_as_float(t[k + 3]));
+      }
+      *reinterpret_cast<float4*>(row + D) = make_float4(m, l, 0.0f, 0.0f);
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    for (int i = threadIdx.x; i < BLOCK_ROWS / n_splits * (D / 4); i += NUM_THREADS) {
+      const int row = i / (D / 4) * n_splits + split, c4 = i % (D / 4), packed = row0 + row;
+      if (packed >= n_rows) continue;
+      const int tok = packed / group, hd = kvh * group + packed % group;
+      const uint32_t local = smem_u32(states + (size_t)row * STATE);
+      const float sink = sink_log2(extras, hd);
+      float M = sink;
+      for (int z = 0; z < n_splits; ++z) M = fmaxf(M, load_peer4(peer_smem(local, z) + D * 4).x);
+      const float M_use = M == -INFINITY ? 0.0f : M;
+      float L = exp2f(sink - M_use);
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int z = 0; z < n_splits; ++z) {
+        const uint32_t from = peer_smem(local, z);
+        const float4 ml = load_peer4(from + D * 4), v = load_peer4(from + c4 * 16);
+        const float f = ml.x == -INFINITY ? 1.0f : exp2f(ml.x - M_use);      // without a maximum: zeros, or NaN to be handed on
+        L += ml.y * f;
+        acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+      }
+      const float inv = L == 0.0f ? 0.0f : head_gate<__nv_bfloat16>(extras, q_start + tok, hd) / L;
+      *reinterpret_cast<uint2*>(a.out + ((long long)(q_start + tok) * a.q_heads + hd) * D + c4 * 4) =
+          make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");   // others may still read this block's states
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -671,17 +744,16 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const Att
 
 extern "C" int llm_cache8_attention_prompt_rows() { return BLOCK_ROWS; }
 
-// The tiles of llm_step_maps with tile_rows = llm_cache8_attention_prompt_rows() (entries of -1 return at once).  chunk, sink, gate and
-// gate_stride (elements): `AttentionExtras`; 0 and null: none.
-extern "C" int llm_cache8_attention_prompt(const void* q, void* out, const Cache8* cache, const int32_t* seq_q_start,
-                                           const int32_t* seq_q_len, const int32_t* seq_kv_len, const int32_t* tile_seq,
-                                           const int32_t* tile_index, int n_tiles, int q_heads, float scale, int window, int chunk,
-                                           const float* sink, const void* gate, long long gate_stride, int* error_word,
-                                           cudaStream_t stream) {
+// The tiles of llm_step_maps with tile_rows = llm_cache8_attention_prompt_rows() (entries of -1 return at once); n_splits (1, 2, 4 or 8)
+// blocks share a tile's keys.  chunk, sink, gate and gate_stride (elements): `AttentionExtras`; 0 and null: none.
+extern "C" int llm_cache8_attention_prompt(const void* q, void* out, const Cache8* cache, const StepLists* lists, int n_splits, int q_heads,
+                                           float scale, int window, int chunk, const float* sink, const void* gate,
+                                           long long gate_stride, int* error_word, cudaStream_t stream) {
+  const int n_tiles = lists->n_tiles;
   if (n_tiles <= 0) return 0;
   const Cache8& c = *cache;
   if (c.head_dim != D || c.kv_heads <= 0 || q_heads <= 0 || q_heads % c.kv_heads || c.page_tokens <= 0 || c.page_tokens % SCALE_TOKENS ||
-      n_tiles > 65535 || !(scale > 0.0f))
+      n_tiles > 65535 || !(scale > 0.0f) || (n_splits != 1 && n_splits != 2 && n_splits != 4 && n_splits != 8))
     return ERR_BAD_SIZE;
   const uintptr_t all = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(c.k) |
                         reinterpret_cast<uintptr_t>(c.v) | (uintptr_t)c.page_stride;
@@ -693,10 +765,29 @@ extern "C" int llm_cache8_attention_prompt(const void* q, void* out, const Cache
       return launch_status();
     configured = true;
   }
-  const AttnArgs a{reinterpret_cast<const __nv_bfloat16*>(q), reinterpret_cast<__nv_bfloat16*>(out), c, seq_q_start, seq_q_len,
-                   seq_kv_len, tile_seq, tile_index, q_heads, scale * 1.4426950408889634f, window,
-                   AttentionExtras{chunk, sink, gate, gate_stride}, error_word};
-  launch_kernel(window > 0 || chunk > 0 || sink || gate ? cache8_prompt_kernel<true> : cache8_prompt_kernel<false>,
-                dim3(c.kv_heads, n_tiles), NUM_THREADS, SMEM_BYTES, stream, a);
+  const AttnArgs a{reinterpret_cast<const __nv_bfloat16*>(q), reinterpret_cast<__nv_bfloat16*>(out), c, *lists, q_heads,
+                   scale * 1.4426950408889634f, window, AttentionExtras{chunk, sink, gate, gate_stride}, error_word};
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(c.kv_heads, n_tiles, n_splits);
+  cfg.blockDim = dim3(NUM_THREADS);
+  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n_attr = 0;
+  if (n_splits > 1) {
+    attr[n_attr].id = cudaLaunchAttributeClusterDimension;
+    attr[n_attr].val.clusterDim.x = 1;
+    attr[n_attr].val.clusterDim.y = 1;
+    attr[n_attr].val.clusterDim.z = n_splits;
+    ++n_attr;
+  }
+  if (pdl_enabled()) {
+    attr[n_attr].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n_attr].val.programmaticStreamSerializationAllowed = 1;
+    ++n_attr;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n_attr;
+  cudaLaunchKernelEx(&cfg, window > 0 || chunk > 0 || sink || gate ? cache8_prompt_kernel<true> : cache8_prompt_kernel<false>, a);
   return launch_status();
 }

@@ -24,6 +24,7 @@
 namespace {
 
 constexpr int THREADS = 256;
+constexpr int TABLE_CHUNK = 256;     // entries of a table row that a warp fills at a time
 constexpr int MAX_SEQS = 4096;       // the four sums of every request lie in shared memory
 
 struct MapsArgs {
@@ -122,10 +123,17 @@ __global__ void __launch_bounds__(THREADS) step_maps_kernel(const MapsArgs a) {
     a.tile_seq[i] = s < S ? s : -1;
     a.tile_index[i] = s < S ? i - tiles[s] : 0;
   }
-  for (int s = first >> 5; s < S; s += step >> 5) {       // a warp per table row
-    const int held = first_page[s + 1] - first_page[s], from = first_page[s];
+  // the tables: a warp takes a stretch of TABLE_CHUNK entries of a row at a time, all of its loads on their way at once
+  const int chunks = (a.max_blocks + TABLE_CHUNK - 1) / TABLE_CHUNK;
+  for (int c = first >> 5; c < S * chunks; c += step >> 5) {
+    const int s = c / chunks, b0 = (c - s * chunks) * TABLE_CHUNK + lane, from = first_page[s], held = min(first_page[s + 1], a.n_pages) - from;
     int32_t* row = a.block_table + (long long)s * a.max_blocks;
-    for (int b = lane; b < a.max_blocks; b += 32) row[b] = b < held && from + b < a.n_pages ? a.pages[from + b] : -1;
+    int page[TABLE_CHUNK / 32];
+#pragma unroll
+    for (int i = 0; i < TABLE_CHUNK / 32; ++i) page[i] = b0 + 32 * i < held ? a.pages[from + b0 + 32 * i] : -1;
+#pragma unroll
+    for (int i = 0; i < TABLE_CHUNK / 32; ++i)
+      if (b0 + 32 * i < a.max_blocks) row[b0 + 32 * i] = page[i];
   }
 }
 

@@ -19,6 +19,7 @@ from .step_maps import SCALE_TOKENS, StepMaps
 DTYPE = torch.float8_e4m3fn
 HEAD_DIMS = (64, 128)
 FEW_ROWS = 16            # packed rows up to which the decode kernel takes a request
+KEY_BLOCK = 128          # positions that the prompt kernel takes at a time
 DECODE_WARPS = 8         # warps of a block of the decode kernel, which a request's scale blocks are dealt to
 _append_lib = None
 _decode_libs: Dict[int, object] = {}
@@ -42,7 +43,7 @@ def _append():
     if _append_lib is None:
         l = build.load_library("cache8_append.cu")
         P, I, L = c_void_p, c_int, c_longlong
-        l.llm_cache8_append.argtypes = [P, I, I, L, P, P, P, P, I, P, P, P, P, I, I, P]
+        l.llm_cache8_append.argtypes = [P, I, I, L, P, P, P, P, I, I, P]
         l.llm_cache8_append.restype = c_int
         _append_lib = l
     return _append_lib
@@ -53,7 +54,7 @@ def _decode(head_dim: int):
     if l is None:
         l = build.load_library("cache8_attention_decode.cu", (f"-DHEAD_DIM={head_dim}",))
         P, I, L, F = c_void_p, c_int, c_longlong, c_float
-        l.llm_cache8_attention_decode.argtypes = [P, P, P, P, P, P, I, I, I, I, F, I, I, P, P, L, P]
+        l.llm_cache8_attention_decode.argtypes = [P, P, P, P, I, I, I, F, I, I, P, P, L, P]
         l.llm_cache8_attention_decode.restype = c_int
         _decode_libs[head_dim] = l
     return l
@@ -64,16 +65,17 @@ def _prompt(head_dim: int):
     if l is None:
         l = build.load_library("cache8_attention_tcgen05.cu", (f"-DHEAD_DIM={head_dim}",))
         P, I, L, F = c_void_p, c_int, c_longlong, c_float
-        l.llm_cache8_attention_prompt.argtypes = [P, P, P, P, P, P, P, P, I, I, F, I, I, P, P, L, P, P]
+        l.llm_cache8_attention_prompt.argtypes = [P, P, P, P, I, I, F, I, I, P, P, L, P, P]
         l.llm_cache8_attention_prompt.restype = c_int
         l.llm_cache8_attention_prompt_rows.restype = c_int
+        l.tile_rows = int(l.llm_cache8_attention_prompt_rows())
         _prompt_libs[head_dim] = l
     return l
 
 
 def tile_rows(head_dim: int) -> int:
     """The `tile_rows` that a `StepMaps` for this head size is made with."""
-    return int(_prompt(head_dim).llm_cache8_attention_prompt_rows())
+    return _prompt(head_dim).tile_rows
 
 
 def prepare(head_dim: int) -> None:
@@ -118,20 +120,25 @@ def _struct(cache: CacheView) -> int:
     return ctypes.addressof(cache.struct)
 
 
-def _check_step(what: str, cache: CacheView, maps: StepMaps, q_heads: int, *tensors) -> None:
-    if q_heads <= 0 or q_heads % cache.kv_heads:
-        raise KernelLaunchError(f"{what}: {q_heads} query heads cannot share {cache.kv_heads} key/value heads")
-    if maps.page_tokens != cache.page_tokens or maps.group * cache.kv_heads != q_heads:
-        raise KernelLaunchError(f"{what}: the step's maps are for pages of {maps.page_tokens} positions and {maps.group} heads a key/value head")
+def _check_step(what: str, cache: CacheView, maps: StepMaps, q_heads: int, a: torch.Tensor, b: torch.Tensor) -> None:
+    """Whether cache, maps and the two tensors belong together (this and what follows runs for every layer of a step)."""
+    if q_heads <= 0 or maps.group * cache.kv_heads != q_heads or maps.page_tokens != cache.page_tokens:
+        raise KernelLaunchError(f"{what}: the step's maps are for pages of {maps.page_tokens} positions and {maps.group} heads a key/value "
+                                f"head, the cache has pages of {cache.page_tokens} and {cache.kv_heads} key/value heads for {q_heads} heads")
     if maps.longest == 0:
         raise KernelLaunchError(f"{what}: the step's maps have not been built")
     if cache.block_table.shape[0] < maps.n_seqs:
         raise KernelLaunchError(f"{what}: {maps.n_seqs} requests, and a block table of {cache.block_table.shape[0]} rows")
-    device = cache.block_table.device
-    if maps.device != device or any(t.device != device for t in tensors):
+    index = maps.index
+    if cache.block_table.get_device() != index or a.get_device() != index or b.get_device() != index:
         raise KernelLaunchError(f"{what}: maps, cache and tensors must lie on one CUDA device")
-    if device.index != torch.cuda.current_device():
-        raise KernelLaunchError(f"{what}: the tensors lie on {device}, the current device is cuda:{torch.cuda.current_device()}")
+    if index != torch.cuda.current_device():
+        raise KernelLaunchError(f"{what}: the tensors lie on {maps.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _bf16_rows(t: torch.Tensor, rows: int, width: int) -> bool:
+    shape = t.shape
+    return t.dtype == torch.bfloat16 and shape[-1] == width and shape[0] >= rows and len(shape) == 2 and t.is_contiguous()
 
 
 def append(qkv: Partials, q_out: torch.Tensor, cache: CacheView, maps: StepMaps, inv_freq: Optional[torch.Tensor], q_heads: int,
@@ -145,16 +152,16 @@ def append(qkv: Partials, q_out: torch.Tensor, cache: CacheView, maps: StepMaps,
     width, d = (q_heads + 2 * cache.kv_heads) * cache.head_dim, cache.head_dim
     at = _struct(cache)
     _check_step("cache8_append", cache, maps, q_heads, t, q_out)
-    if t.shape[-1] != width or t.shape[-2] < maps.n_rows or t.stride(-1) != 1 or t.stride(-2) != width or (qkv.n > 1 and t.shape[0] < qkv.n):
-        raise KernelLaunchError(f"cache8_append: projections of {tuple(t.shape)} for {maps.n_rows} dense rows of {width}")
-    if q_out.dtype != torch.bfloat16 or q_out.shape[-1] != q_heads * d or q_out.shape[0] < maps.n_rows or not q_out.is_contiguous():
+    shape = t.shape
+    if shape[-1] != width or shape[-2] < maps.n_rows or t.stride(-1) != 1 or t.stride(-2) != width or (qkv.n > 1 and shape[0] < qkv.n):
+        raise KernelLaunchError(f"cache8_append: projections of {tuple(shape)} for {maps.n_rows} dense rows of {width}")
+    if not _bf16_rows(q_out, maps.n_rows, q_heads * d):
         raise KernelLaunchError(f"cache8_append: queries go to contiguous bfloat16 [rows, {q_heads * d}], not {tuple(q_out.shape)} of {q_out.dtype}")
     if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.numel() != d // 2 or not inv_freq.is_contiguous()
-                                 or inv_freq.device != t.device):
+                                 or inv_freq.get_device() != maps.index):
         raise KernelLaunchError(f"cache8_append: the inverse frequencies must be {d // 2} contiguous float32 numbers")
     _check(_append().llm_cache8_append(
-        t.data_ptr(), dtype_code(t.dtype), qkv.n, qkv.stride, q_out.data_ptr(), at, maps.write_seq.data_ptr(), maps.write_block.data_ptr(),
-        maps.n_writes, maps.seq_q_start.data_ptr(), maps.seq_q_len.data_ptr(), maps.seq_kv_len.data_ptr(), _ptr(inv_freq), q_heads,
+        t.data_ptr(), dtype_code(t.dtype), qkv.n, qkv.stride, q_out.data_ptr(), at, maps.lists, _ptr(inv_freq), q_heads,
         1 if write_cache else 0, stream if stream is not None else stream_handle()), "cache8_append")
 
 
@@ -167,6 +174,14 @@ def decode_splits(n_seqs: int, kv_heads: int, max_keys: int) -> int:
     return splits
 
 
+def prompt_splits(n_tiles: int, kv_heads: int, max_keys: int) -> int:
+    """How many blocks of the prompt kernel share a tile's keys: a power of two up to 8, as many as the SMs take at once."""
+    splits = 1
+    while splits < 8 and n_tiles * kv_heads * splits * 2 <= sm_count() and max_keys > splits * KEY_BLOCK:
+        splits *= 2
+    return splits
+
+
 def attention(q: torch.Tensor, out: torch.Tensor, cache: CacheView, maps: StepMaps, q_heads: int, scale: float, window: int = 0,
               extras: Optional[AttentionExtras] = None, stream=None) -> None:
     """out = softmax(scale * q k^T) v over each request's cached positions up to the query's own (with `window` > 0 the newest
@@ -175,10 +190,10 @@ def attention(q: torch.Tensor, out: torch.Tensor, cache: CacheView, maps: StepMa
     of no request and idle ones are left as they were in `out`, a row that sees no key is zero."""
     at = _struct(cache)
     _check_step("cache8_attention", cache, maps, q_heads, q, out)
-    for t in (q, out):
-        if t.dtype != torch.bfloat16 or t.shape[-1] != q_heads * cache.head_dim or t.shape[0] < maps.n_rows or not t.is_contiguous():
-            raise KernelLaunchError(f"cache8_attention: queries and outputs must be contiguous bfloat16 [{maps.n_rows} rows, "
-                                    f"{q_heads * cache.head_dim}], not {tuple(t.shape)} of {t.dtype}")
+    width = q_heads * cache.head_dim
+    if not _bf16_rows(q, maps.n_rows, width) or not _bf16_rows(out, maps.n_rows, width):
+        raise KernelLaunchError(f"cache8_attention: queries and outputs must be contiguous bfloat16 [{maps.n_rows} rows, {width}], not "
+                                f"{tuple(q.shape)} of {q.dtype} and {tuple(out.shape)} of {out.dtype}")
     if not scale > 0.0 or window < 0:
         raise KernelLaunchError(f"cache8_attention: scale {scale} and window {window} are not supported (above zero; zero or more)")
     if maps.few_rows != FEW_ROWS or maps.tile_rows != tile_rows(cache.head_dim):
@@ -191,11 +206,10 @@ def attention(q: torch.Tensor, out: torch.Tensor, cache: CacheView, maps: StepMa
         rows = min(maps.longest * group, FEW_ROWS)
         splits = decode_splits(maps.n_seqs, cache.kv_heads, cache.table_stride * cache.page_tokens)
         _check(_decode(cache.head_dim).llm_cache8_attention_decode(
-            q.data_ptr(), out.data_ptr(), at, maps.seq_q_start.data_ptr(), maps.seq_q_len.data_ptr(), maps.seq_kv_len.data_ptr(),
-            maps.n_seqs, splits, rows, q_heads, scale, window, chunk, sink, gate, gate_stride, stream), "cache8_attention_decode")
+            q.data_ptr(), out.data_ptr(), at, maps.lists, splits, rows, q_heads, scale, window, chunk, sink, gate, gate_stride, stream), "cache8_attention_decode")
     if maps.longest * group > FEW_ROWS:
         from . import gemm
         _check(_prompt(cache.head_dim).llm_cache8_attention_prompt(
-            q.data_ptr(), out.data_ptr(), at, maps.seq_q_start.data_ptr(), maps.seq_q_len.data_ptr(), maps.seq_kv_len.data_ptr(),
-            maps.tile_seq.data_ptr(), maps.tile_index.data_ptr(), maps.n_tiles, q_heads, scale, window, chunk, sink, gate, gate_stride,
-            gemm.error_word(q.device).data_ptr(), stream), "cache8_attention_prompt")
+            q.data_ptr(), out.data_ptr(), at, maps.lists, prompt_splits(maps.n_tiles, cache.kv_heads, cache.table_stride * cache.page_tokens),
+            q_heads, scale, window, chunk, sink, gate, gate_stride, gemm.error_word(q.device).data_ptr(), stream),
+            "cache8_attention_prompt")

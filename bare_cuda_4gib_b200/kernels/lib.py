@@ -68,7 +68,8 @@ def sm_count() -> int:
 
 
 def stream_handle() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """The current stream of the current device (what torch.cuda.current_stream().cuda_stream says, without the object)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 class CacheView:

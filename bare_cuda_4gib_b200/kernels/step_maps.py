@@ -6,6 +6,7 @@ every step; the arrays it then offers are what the kernels of that step read."""
 
 from __future__ import annotations
 
+import ctypes
 from ctypes import c_int, c_void_p
 
 import torch
@@ -28,6 +29,13 @@ def lib():
         l.llm_step_maps_max_seqs.restype = c_int
         _lib = l
     return _lib
+
+
+class StepLists(ctypes.Structure):
+    """struct StepLists of csrc/cache8.cuh."""
+
+    _fields_ = [(name, c_void_p) for name in ("seq_q_start", "seq_q_len", "seq_kv_len", "write_seq", "write_block", "tile_seq",
+                                              "tile_index")] + [(name, c_int) for name in ("n_seqs", "n_writes", "n_tiles")]
 
 
 class StepMaps:
@@ -70,6 +78,8 @@ class StepMaps:
         self._writes = torch.full((2, writes), -1, **i32)
         self._tiles = torch.full((2, tiles), -1, **i32)
         self.device = self._table.device
+        self.index = self.device.index
+        self.table = self._table                       # the block tables whole, at the address that `block_table` keeps
         self._out = tuple(t.data_ptr() for t in (*self._seqs, *self._rows, self._slots, self._table, *self._writes, *self._tiles))
         self._shape = None
         self.longest = self.shortest = 0
@@ -86,6 +96,10 @@ class StepMaps:
         self.write_seq, self.write_block = (t[:self.n_writes] for t in self._writes)
         self.tile_seq, self.tile_index = (t[:self.n_tiles] for t in self._tiles)
         self._shape = (seqs, rows)
+        self._lists = StepLists(*(t.data_ptr() for t in (self.seq_q_start, self.seq_q_len, self.seq_kv_len, self.write_seq,
+                                                         self.write_block, self.tile_seq, self.tile_index)),
+                                seqs, self.n_writes, self.n_tiles)
+        self.lists = ctypes.addressof(self._lists)      # what the launchers of the step's kernels hand on
 
     def build(self, cached: torch.Tensor, q_len: torch.Tensor, pages: torch.Tensor, n_rows: int, longest: int, shortest: int,
               stream=None) -> None:
@@ -102,9 +116,9 @@ class StepMaps:
         if not 0 < shortest <= longest <= n_rows:
             raise KernelLaunchError(f"step maps: requests of {shortest} to {longest} new tokens in a step of {n_rows}")
         for t in (cached, q_len, pages):
-            if t.dtype != torch.int32 or t.device != self.device or not t.is_contiguous():
+            if t.dtype != torch.int32 or t.get_device() != self.index or not t.is_contiguous():
                 raise KernelLaunchError(f"step maps: lengths and pages must be contiguous int32 on {self.device}")
-        if self.device.index != torch.cuda.current_device():
+        if self.index != torch.cuda.current_device():
             raise KernelLaunchError(f"step maps: made for {self.device}, the current device is cuda:{torch.cuda.current_device()}")
         if self._shape != (seqs, n_rows):
             self._arrays(seqs, n_rows)
