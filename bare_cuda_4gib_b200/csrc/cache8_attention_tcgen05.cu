@@ -7,10 +7,12 @@
 //
 // One thread block = two tiles of 128 packed rows of one request and one key/value head, which share every key and value block of 128
 // positions.  Warps:
-//   converters (4) fetch a tile's codes from the request's pages, 16 bytes a load and a tile ahead, and write them as halves into
-//                  128-byte-swizzled shared memory.  Halves hold e4m3 exactly and one instruction converts two codes.  The scales
-//                  of a key block are split into 2^e of the block (the largest, which the softmax gets) and what is left for 16 positions, at most one, which
-//                  joins the halves (exactly down to 2^-15).  Key tiles and value tiles go through ONE ring of slots in the order K(0) V(0) K(1) ...;
+//   loader (1)     copies a key block's codes, as they lie in the request's pages, into a ring of their own with TMA (one tensor map over the cache's
+//                  pool, a box per piece of a page), and splits the block's scales into 2^e (the largest, which the softmax gets) and what is
+//                  left for 16 positions, at most one, which the converters get;
+//   converters (4) write a tile's codes as halves, times what is left of their scale (exact down to 2^-15), into 128-byte-swizzled shared
+//                  memory.  Halves hold e4m3 exactly and one instruction converts two codes.  Key tiles and value tiles go through ONE ring
+//                  of slots in the order K(0) V(0) K(1) ...;
 //   MMA issuer (1) S_g = Q_g K^T (M 128, N 128, K head size) into tile g's S columns of tensor memory, and
 //                  O_g (+)= P_g V with P_g as the operand in tensor memory and V as it lies ([key][channel], MN-major), in two halves of 64
 //                  keys, each as soon as its half of P is there: P never goes through shared memory, whose bandwidth
@@ -29,12 +31,14 @@
 // multiplied, and values are finite always.  Values behind the request's last key are written as zeros.
 // Every mbarrier wait is bounded: on a timeout the thread sets the error word, all roles leave their loops, tensor memory is
 // released and the block returns.
-// One B200: a prompt of 2,048 tokens (32 / 4 heads of 64) 51.6 us, 2,048 tokens behind 2,048 (32 heads of 128) 201 us, 61 tokens behind 3,001
-// (32 / 8 heads of 128) 30.1 us (97.6 with one block a tile).
+// One B200: a prompt of 2,048 tokens (32 / 4 heads of 64) 46.8 us, 2,048 tokens behind 2,048 (32 heads of 128) 169 us, 61 tokens behind 3,001
+// (32 / 8 heads of 128) 26.2 us.
 
 #include "cache8.cuh"
 
+#include <cuda.h>
 #include <cuda_fp16.h>
+#include <string.h>
 
 #ifndef HEAD_DIM
 #define HEAD_DIM 64
@@ -52,24 +56,24 @@ constexpr int BN = 128;          // keys per block
 constexpr int SUB = 128 * 128;   // bytes of a [128 rows x 64 halves] swizzled sub-tile
 constexpr int Q_BYTES = KA * SUB;        // one tile's queries
 constexpr int TILE_BYTES = KA * SUB;     // one key tile or one value tile
-constexpr int SLOTS = HEAD_DIM == 64 ? 10 : 5;   // key and value tiles in flight (what shared memory allows)
+constexpr int RAW_BYTES = BN * D;        // one key tile or one value tile as codes
+constexpr int SLOTS = HEAD_DIM == 64 ? 6 : 3, RAW_SLOTS = HEAD_DIM == 64 ? 6 : 4;   // tiles in flight, as halves and as codes (what shared memory allows)
 constexpr int SOFTMAX_THREADS = 128 * TILES, CONVERT_THREADS = 128;
-constexpr int CONVERT_WARP = SOFTMAX_THREADS / 32, MMA_WARP = CONVERT_WARP + CONVERT_THREADS / 32;
-constexpr int NUM_THREADS = (MMA_WARP + 1) * 32;   // warps 0-7 softmax, 8-11 converters, 12 MMA
+constexpr int CONVERT_WARP = SOFTMAX_THREADS / 32, MMA_WARP = CONVERT_WARP + CONVERT_THREADS / 32, LOADER_WARP = MMA_WARP + 1;
+constexpr int NUM_THREADS = (LOADER_WARP + 1) * 32;   // warps 0-7 softmax, 8-11 converters, 12 MMA, 13 loader
 constexpr int GROUP_THREADS = 128;
 constexpr int S_PIECE = 64;      // columns of S a softmax thread holds in registers at a time
 constexpr bool SHARED_COLUMNS = HEAD_DIM == 128;   // whether P lies in the columns of S
 constexpr int TMEM_COLS = 512, O_COL = TILES * BN, P_COL = O_COL + TILES * D;
 constexpr unsigned long long WAIT_LIMIT_NS = 1000000000ull;
 constexpr float RESCALE_STEP = 8.0f;
-// What a converter thread fetches of a tile: 16 codes (chunk ct % CHUNKS) of rows ct / CHUNKS + i * STRIDE, i < CHUNKS.
-constexpr int CHUNKS = D / 16, STRIDE = CONVERT_THREADS / CHUNKS;
+constexpr int CHUNKS = D / 16;              // 16-byte chunks of a key's codes; also how many of them a converter thread takes of a tile
 constexpr int BLOCKS = BN / SCALE_TOKENS;   // scale blocks of a key block
-constexpr int EXPONENTS = 8;                // key blocks whose exponents are kept (more than can be in flight)
+constexpr int EXPONENTS = 16;               // key blocks whose exponents are kept (more than can be in flight)
 constexpr int STATE = D + 4;                // floats of a row's state in a merge: D sums, the maximum, the sum
-constexpr size_t TILES_BYTES = (size_t)TILES * Q_BYTES + (size_t)SLOTS * TILE_BYTES;
+constexpr size_t TILES_BYTES = (size_t)TILES * Q_BYTES + (size_t)SLOTS * TILE_BYTES + (size_t)RAW_SLOTS * RAW_BYTES;
 static_assert((size_t)BLOCK_ROWS * STATE * 4 <= TILES_BYTES, "the states of a merge lie over the tiles");
-constexpr size_t SMEM_BYTES = TILES_BYTES + 512;
+constexpr size_t SMEM_BYTES = TILES_BYTES + 768;
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -111,6 +115,20 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
 // index is XORed with the row's index inside its group.
 __device__ __forceinline__ uint32_t swizzled(int row, int chunk) {
   return (uint32_t)((row >> 3) * 1024 + (row & 7) * 128 + ((chunk ^ (row & 7)) << 4));
+}
+
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y) : "memory");
+}
+// Byte offset of chunk `chunk` of row `row` in a tile of codes as TMA writes it: 128-byte swizzle for rows of 128 bytes, 64-byte swizzle
+// for rows of 64.
+__device__ __forceinline__ uint32_t raw_swizzled(int row, int chunk) {
+  return (uint32_t)(row * D + ((D == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) << 4));
 }
 
 // Shared-memory matrix descriptor, 128-byte swizzle, 1024 bytes between 8-row groups.
@@ -213,6 +231,8 @@ struct AttnArgs {
   const __nv_bfloat16* q;      // [tokens, q_heads, D]
   __nv_bfloat16* out;          // [tokens, q_heads * D]
   Cache8 cache;
+  long long page_rows, k_row0, v_row0;   // the pool seen as rows of D codes: row = page * page_rows + k_row0 (or v_row0) + kv head * page_tokens + ...
+  int box_rows;                // rows of the tensor map's box: divides the page size and BN
   StepLists lists;
   int q_heads;
   float scale_log2;
@@ -221,27 +241,31 @@ struct AttnArgs {
   int* error_word;
 };
 
-constexpr int ERR_CONVERT = 41, ERR_MMA = 42, ERR_SOFTMAX = 43, ERR_LAYOUT = 44;
+constexpr int ERR_CONVERT = 41, ERR_MMA = 42, ERR_SOFTMAX = 43, ERR_LAYOUT = 44, ERR_LOADER = 45;
 
 // EXTRAS: whether a window, blocks of positions, a sink or a gate may be asked for; without them their code is
 // not there.  gridDim.z blocks (a cluster) share a tile's key blocks.
 template <bool EXTRAS>
-__global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __grid_constant__ CUtensorMap pool_map, const AttnArgs a) {
   const AttentionExtras extras = EXTRAS ? a.extras : AttentionExtras{0, nullptr, nullptr, 0};
   const int window = EXTRAS ? a.window : 0;
   extern __shared__ __align__(1024) uint8_t smem[];   // swizzled tiles need 1024-byte alignment (checked below)
   uint8_t* q_smem = smem;                              // [TILES][KA sub-tiles]
   uint8_t* ring = q_smem + TILES * Q_BYTES;            // [SLOTS][KA sub-tiles]: key and value tiles in turn
+  uint8_t* raw_ring = ring + SLOTS * TILE_BYTES;       // [RAW_SLOTS]: the same tiles as codes
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + TILES_BYTES);
   uint64_t* tile_full = bars;               // [SLOTS] converters -> MMA (and softmax): the slot's tile is written
   uint64_t* tile_empty = tile_full + SLOTS; // [SLOTS] MMA (commit) -> converters
-  uint64_t* q_full = tile_empty + SLOTS;    // [2] softmax group -> MMA: Q_g staged
+  uint64_t* raw_full = tile_empty + SLOTS;  // [RAW_SLOTS] loader -> converters: the slot's codes have landed
+  uint64_t* raw_empty = raw_full + RAW_SLOTS; // [RAW_SLOTS] converters -> loader
+  uint64_t* q_full = raw_empty + RAW_SLOTS; // [2] softmax group -> MMA: Q_g staged
   uint64_t* s_full = q_full + 2;            // [2] MMA (commit) -> softmax, per group
   uint64_t* s_free = s_full + 2;            // [2] softmax -> MMA: the group holds its S values in registers (P in columns of its own)
   uint64_t* p_full = s_free + 2;            // [2][2] softmax -> MMA: half h of P written, per group
   uint64_t* pv_done = p_full + 4;           // [2][2] MMA (commit) -> softmax: the product with half h is complete, per group
   int2* exponents = reinterpret_cast<int2*>(pv_done + 4);   // [EXPONENTS] of a key block's keys and values
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(exponents + EXPONENTS);
+  uint32_t* factors = reinterpret_cast<uint32_t*>(exponents + EXPONENTS);   // [RAW_SLOTS][BLOCKS] what is left of a scale, twice as a half; 0: zeros
+  uint32_t* tmem_slot = factors + RAW_SLOTS * BLOCKS;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   pdl_launch_dependents();
@@ -290,9 +314,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const Att
   const int n_kb = kb_hi - kb_lo;
 
   if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&pool_map)) : "memory");
     for (int s = 0; s < SLOTS; ++s) {
       mbar_init(&tile_full[s], CONVERT_THREADS / 32);
       mbar_init(&tile_empty[s], 1);
+    }
+    for (int s = 0; s < RAW_SLOTS; ++s) {
+      mbar_init(&raw_full[s], 1);
+      mbar_init(&raw_empty[s], CONVERT_THREADS / 32);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&q_full[b], GROUP_THREADS);
@@ -327,102 +356,133 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const Att
 
   if (warp >= CONVERT_WARP && warp < MMA_WARP) {
     // ------------------------------------------------------------------ converters
-    // Tile n of the ring is the keys (n even) or the values (n odd) of key block n / 2.  A tile's codes are asked for one tile ahead of
-    // their conversion, and where a key block's scale blocks lie two tiles before that.  Positions of no page (given back by a
-    // window) and behind the request's last key become zeros: their keys are masked, but zero times whatever lies there must be zero.
-    const int ct = threadIdx.x - CONVERT_WARP * 32, chunk = ct % CHUNKS, first_row = ct / CHUNKS;
-    auto find_page = [&](int jj) {      // of a key block, lane b: the page of its scale block b, -1 if none
+    // A thread takes 16 codes (a chunk) of CHUNKS rows.  The eight threads whose accesses share a turn of the banks hold four chunks of two rows
+    // that meet eight different bank groups, in the codes as they lie and in the halves as they are written: neighbours at head size 64, rows
+    // that differ in bits 0 and 2 at 128.
+    const int cw = warp - CONVERT_WARP;
+    const int chunk = D == 128 ? (cw >> 1) * 4 + (lane & 3) : lane & 3;
+    const int row_in = D == 128 ? (cw & 1) * 8 + ((lane >> 3) ^ ((lane >> 2) & 1) * 5) : cw * 8 + (lane >> 2);
+    constexpr int STEP = BN / CHUNKS;             // rows from one of a thread's chunks to the next: one or two scale blocks
+    bool ok = true;
+    for (int n = 0; n < 2 * n_kb; ++n) {
+      const int raw_slot = n % RAW_SLOTS, slot = n % SLOTS, use = n / SLOTS;
+      ok = mbar_wait(&raw_full[raw_slot], (uint32_t)(n / RAW_SLOTS) & 1u, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      uint4 raw[CHUNKS];
+      uint32_t factor[CHUNKS];
+      const uint32_t from = smem_u32(raw_ring) + raw_slot * RAW_BYTES;
+#pragma unroll
+      for (int i = 0; i < CHUNKS; ++i) {
+        const int row = row_in + i * STEP;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(raw[i].x), "=r"(raw[i].y), "=r"(raw[i].z), "=r"(raw[i].w) : "r"(from + raw_swizzled(row, chunk)) : "memory");
+        factor[i] = factors[raw_slot * BLOCKS + row / SCALE_TOKENS];      // the same for the whole warp
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&raw_empty[raw_slot]);
+      ok = use == 0 || mbar_wait(&tile_empty[slot], (uint32_t)(use - 1) & 1u, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const uint32_t to = smem_u32(ring) + slot * TILE_BYTES + (chunk >> 2) * SUB;
+      const int behind = kv_len - (kb_lo + (n >> 1)) * BN;       // rows from here on lie behind the request's last key
+#pragma unroll
+      for (int i = 0; i < CHUNKS; ++i) {
+        const int row = row_in + i * STEP;
+        uint32_t w[8];
+        halves(raw[i].x, w[0], w[1]);
+        halves(raw[i].y, w[2], w[3]);
+        halves(raw[i].z, w[4], w[5]);
+        halves(raw[i].w, w[6], w[7]);
+        if (factor[i] != 0x3c003c00u) {
+          // (where no page is held, or a scale is lost beside a far larger one, zeros; whatever lay there may be NaN)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) w[k] = factor[i] ? mul_half2(w[k], factor[i]) : 0u;
+        }
+        if (row >= behind) {     // masked as keys, but as values zero times whatever lies there must be zero
+#pragma unroll
+          for (int k = 0; k < 8; ++k) w[k] = 0u;
+        }
+        const int first = (chunk & 3) * 2;
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + swizzled(row, first)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + swizzled(row, first + 1)), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tile_full[slot]);
+    }
+    if (!ok && lane == 0) {
+      *abort_flag = 1;
+      atomicCAS(a.error_word, 0, ERR_CONVERT);
+    }
+  } else if (warp == LOADER_WARP) {
+    // ------------------------------------------------------------------ loader
+    // Lane b looks after the key block's scale block b.  Pages are looked up two key blocks ahead and scales one, so that neither is waited for.
+    auto find_page = [&](int jj) {      // -1: not held, or wholly behind the request's last key
       const int key = (kb_lo + jj) * BN + lane * SCALE_TOKENS;
       return lane < BLOCKS && jj < n_kb && key < kv_len ? page_of(a.cache, seq, key) : -1;
     };
-    struct Place {             // of a key block, lane b: its scale block b (the same for keys and values)
-      long long at;            // codes from the cache's first, or -1
+    struct Place {
+      long long row;           // of the pool, without the cache's own offset, or -1
       float k_scale, v_scale;
     };
     auto place = [&](int jj, int page) {
       Place p{-1, 0.0f, 0.0f};
       if (page >= 0) {
         const int in_page = ((kb_lo + jj) * BN + lane * SCALE_TOKENS) % a.cache.page_tokens;
-        p.at = (long long)page * a.cache.page_stride + ((long long)kvh * a.cache.page_tokens + in_page) * D;
-        const long long s = (long long)page * a.cache.scale_stride + (long long)kvh * (a.cache.page_tokens / SCALE_TOKENS) + in_page / SCALE_TOKENS;
-        p.k_scale = __ldcg(a.cache.k_scale + s);
-        p.v_scale = __ldcg(a.cache.v_scale + s);
+        p.row = (long long)page * a.page_rows + (long long)kvh * a.cache.page_tokens + in_page;
+        const long long at = (long long)page * a.cache.scale_stride + (long long)kvh * (a.cache.page_tokens / SCALE_TOKENS) + in_page / SCALE_TOKENS;
+        p.k_scale = __ldcg(a.cache.k_scale + at);
+        p.v_scale = __ldcg(a.cache.v_scale + at);
       }
       return p;
     };
-    auto block_of = [&](int i) { return (first_row + i * STRIDE) / SCALE_TOKENS; };      // the same for a whole warp
-    auto fetch = [&](uint4 (&raw)[CHUNKS], const Place& p, int n) {
-      const uint8_t* base = (n & 1) ? a.cache.v : a.cache.k;
-      const int key0 = (kb_lo + (n >> 1)) * BN;
-#pragma unroll
-      for (int i = 0; i < CHUNKS; ++i) {
-        const int row = first_row + i * STRIDE;
-        const long long at = __shfl_sync(0xffffffffu, p.at, block_of(i));
-        raw[i] = make_uint4(0, 0, 0, 0);
-        if (at >= 0 && key0 + row < kv_len) raw[i] = __ldcg(reinterpret_cast<const uint4*>(base + at + (row % SCALE_TOKENS) * D + chunk * 16));
-      }
-    };
-    // What is left of a scale block's factor once the largest exponent of its key block is taken out, and that exponent.
+    // What is left of the lane's scale once the largest exponent of the key block is taken out, and that exponent.
     auto split_scale = [&](const Place& p, float scale, int& most) {
-      const bool lost = isnan(scale), there = p.at >= 0 && !lost;
+      const bool lost = isnan(scale), there = p.row >= 0 && !lost;
       const int e = there ? exponent_of(scale) : -1000;
       most = __reduce_max_sync(0xffffffffu, e);
       if (most == -1000) most = 0;
-      return lost ? 0x7e007e00u : there ? half_power(most - e) : 0u;
+      return p.row < 0 ? 0u : lost ? 0x7e007e00u : half_power(most - e);
     };
-    auto convert = [&](const uint4 (&raw)[CHUNKS], uint32_t factors, int n) {
-      const uint32_t base = smem_u32(ring) + (n % SLOTS) * TILE_BYTES + (chunk >> 2) * SUB;
-#pragma unroll
-      for (int i = 0; i < CHUNKS; ++i) {
-        const int row = first_row + i * STRIDE;
-        const uint32_t f = __shfl_sync(0xffffffffu, factors, block_of(i));
-        uint32_t w[8];
-        halves(raw[i].x, w[0], w[1]);
-        halves(raw[i].y, w[2], w[3]);
-        halves(raw[i].z, w[4], w[5]);
-        halves(raw[i].w, w[6], w[7]);
-        if (f != 0x3c003c00u) {       // the same for the whole warp
-#pragma unroll
-          for (int k = 0; k < 8; ++k) w[k] = mul_half2(w[k], f);
-        }
-        // two 16-byte chunks of the row; threads of odd sub-tiles store theirs the other way round, so that the eight that share a row
-        // (or two rows, at head size 64) meet eight different groups of banks
-        const int first = (chunk & 3) * 2, swap = (chunk >> 2) & 1;
-        const uint32_t at0 = base + swizzled(row, first + swap), at1 = base + swizzled(row, first + 1 - swap);
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at0), "r"(swap ? w[4] : w[0]), "r"(swap ? w[5] : w[1]), "r"(swap ? w[6] : w[2]), "r"(swap ? w[7] : w[3]) : "memory");
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at1), "r"(swap ? w[0] : w[4]), "r"(swap ? w[1] : w[5]), "r"(swap ? w[2] : w[6]), "r"(swap ? w[3] : w[7]) : "memory");
-      }
-    };
+    const int per_piece = a.box_rows / SCALE_TOKENS;
+    const bool leads = lane < BLOCKS && lane % per_piece == 0;      // a piece of a page is its first scale block's lane's to copy
     bool ok = true;
-    auto deliver = [&](const uint4 (&raw)[CHUNKS], uint32_t factors, int n) {
-      const uint32_t use = (uint32_t)(n / SLOTS);   // how often the slot was filled before
-      ok = ok && (use == 0 || mbar_wait(&tile_empty[n % SLOTS], (use - 1) & 1, abort_flag));
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) return;
-      convert(raw, factors, n);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&tile_full[n % SLOTS]);
-    };
-    uint4 keys[CHUNKS], values[CHUNKS];
+    int issued = 0;
     Place now = place(0, find_page(0));
     int page = find_page(1);
-    if (n_kb > 0) fetch(keys, now, 0);
     for (int jj = 0; jj < n_kb && ok; ++jj) {
-      fetch(values, now, 2 * jj + 1);
       const Place next = place(jj + 1, page);
       page = find_page(jj + 2);
       int ek, ev;
       const uint32_t fk = split_scale(now, now.k_scale, ek), fv = split_scale(now, now.v_scale, ev);
-      if (warp == CONVERT_WARP && lane == 0) exponents[jj % EXPONENTS] = make_int2(ek, ev);
-      deliver(keys, fk, 2 * jj);
-      if (jj + 1 < n_kb) fetch(keys, next, 2 * jj + 2);
-      deliver(values, fv, 2 * jj + 1);
+      if (lane == 0) exponents[jj % EXPONENTS] = make_int2(ek, ev);
+      const uint32_t copies = __popc(__ballot_sync(0xffffffffu, leads && now.row >= 0));
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        const int n = 2 * jj + which, slot = n % RAW_SLOTS, use = n / RAW_SLOTS;
+        ok = ok && (use == 0 || mbar_wait(&raw_empty[slot], (uint32_t)(use - 1) & 1u, abort_flag));
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane < BLOCKS) factors[slot * BLOCKS + lane] = which ? fv : fk;
+        __syncwarp();
+        if (lane == 0) mbar_expect_tx(&raw_full[slot], copies * a.box_rows * D);   // also the one arrival
+        __syncwarp();
+        if (leads && now.row >= 0)
+          tma_load_2d(smem_u32(raw_ring) + slot * RAW_BYTES + lane * SCALE_TOKENS * D, &pool_map, &raw_full[slot], 0,
+                      (int)(now.row + (which ? a.v_row0 : a.k_row0)));
+        issued = n + 1;
+      }
       now = next;
     }
-    if (!ok && lane == 0) {
-      *abort_flag = 1;
-      atomicCAS(a.error_word, 0, ERR_CONVERT);
+    if (!ok) {
+      if (lane == 0) {
+        *abort_flag = 1;
+        atomicCAS(a.error_word, 0, ERR_LOADER);
+        // this block's copies in flight land before it leaves (the waits of the others end at the flag)
+        volatile int never = 0;
+        for (int n = max(0, issued - RAW_SLOTS); n < issued; ++n) mbar_wait(&raw_full[n % RAW_SLOTS], (uint32_t)(n / RAW_SLOTS) & 1u, &never);
+      }
+      __syncwarp();
     }
   } else if (warp == MMA_WARP) {
     // ------------------------------------------------------------------ MMA issuer
@@ -742,11 +802,45 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const Att
 
 }  // namespace
 
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiledFn encode_tiled_fn() {
+  static EncodeTiledFn fn = nullptr;
+  if (!fn) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(p);
+  }
+  return fn;
+}
+
 extern "C" int llm_cache8_attention_prompt_rows() { return BLOCK_ROWS; }
 
+// Writes the 128-byte tensor map of a pool of `rows` rows of D codes starting at `base` (16-byte aligned), boxes of `box_rows` whole rows
+// (the largest power of two that divides the page size, up to 128), swizzled as raw_swizzled says.
+extern "C" int llm_cache8_prompt_pool_map(void* map_out, const void* base, long long rows, int box_rows) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return 1000 + (int)cudaErrorNotSupported;
+  if ((reinterpret_cast<uintptr_t>(base) & 15) || rows <= 0 || rows > 0x7fffffffLL || box_rows < SCALE_TOKENS || BN % box_rows) return ERR_BAD_SIZE;
+  cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)D};
+  cuuint32_t box[2] = {(cuuint32_t)D, (cuuint32_t)box_rows};
+  cuuint32_t elem[2] = {1, 1};
+  CUresult r = fn(reinterpret_cast<CUtensorMap*>(map_out), CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : 2000 + (int)r;
+}
+
 // The tiles of llm_step_maps with tile_rows = llm_cache8_attention_prompt_rows() (entries of -1 return at once); n_splits (1, 2, 4 or 8)
-// blocks share a tile's keys.  chunk, sink, gate and gate_stride (elements): `AttentionExtras`; 0 and null: none.
-extern "C" int llm_cache8_attention_prompt(const void* q, void* out, const Cache8* cache, const StepLists* lists, int n_splits, int q_heads,
+// blocks share a tile's keys.  `pool_map`: llm_cache8_prompt_pool_map over `pool_base`, in which the cache's codes lie, with boxes of
+// `box_rows` rows, which divide the page size.  chunk, sink, gate and gate_stride (elements): `AttentionExtras`; 0 and null: none.
+extern "C" int llm_cache8_attention_prompt(const void* q, void* out, const Cache8* cache, const void* pool_map, const void* pool_base,
+                                           int box_rows, const StepLists* lists, int n_splits, int q_heads,
                                            float scale, int window, int chunk, const float* sink, const void* gate,
                                            long long gate_stride, int* error_word, cudaStream_t stream) {
   const int n_tiles = lists->n_tiles;
@@ -757,7 +851,10 @@ extern "C" int llm_cache8_attention_prompt(const void* q, void* out, const Cache
     return ERR_BAD_SIZE;
   const uintptr_t all = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(c.k) |
                         reinterpret_cast<uintptr_t>(c.v) | (uintptr_t)c.page_stride;
-  if (all & 15) return ERR_BAD_ALIGN;
+  const long long k_off = reinterpret_cast<const char*>(c.k) - reinterpret_cast<const char*>(pool_base);
+  const long long v_off = reinterpret_cast<const char*>(c.v) - reinterpret_cast<const char*>(pool_base);
+  if ((all & 15) || k_off < 0 || v_off < 0 || k_off % D || v_off % D || c.page_stride % D) return ERR_BAD_ALIGN;
+  if (box_rows < SCALE_TOKENS || BN % box_rows || box_rows % SCALE_TOKENS || c.page_tokens % box_rows) return ERR_BAD_SIZE;
   static bool configured = false;
   if (!configured) {
     if (cudaFuncSetAttribute(cache8_prompt_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES) != cudaSuccess ||
@@ -765,8 +862,11 @@ extern "C" int llm_cache8_attention_prompt(const void* q, void* out, const Cache
       return launch_status();
     configured = true;
   }
-  const AttnArgs a{reinterpret_cast<const __nv_bfloat16*>(q), reinterpret_cast<__nv_bfloat16*>(out), c, *lists, q_heads,
+  const AttnArgs a{reinterpret_cast<const __nv_bfloat16*>(q), reinterpret_cast<__nv_bfloat16*>(out), c, c.page_stride / D, k_off / D, v_off / D,
+                   box_rows, *lists, q_heads,
                    scale * 1.4426950408889634f, window, AttentionExtras{chunk, sink, gate, gate_stride}, error_word};
+  CUtensorMap map;   // the caller's buffer need not be 64-byte aligned
+  memcpy(&map, pool_map, sizeof(CUtensorMap));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(c.kv_heads, n_tiles, n_splits);
   cfg.blockDim = dim3(NUM_THREADS);
@@ -788,6 +888,6 @@ extern "C" int llm_cache8_attention_prompt(const void* q, void* out, const Cache
   }
   cfg.attrs = attr;
   cfg.numAttrs = n_attr;
-  cudaLaunchKernelEx(&cfg, window > 0 || chunk > 0 || sink || gate ? cache8_prompt_kernel<true> : cache8_prompt_kernel<false>, a);
+  cudaLaunchKernelEx(&cfg, window > 0 || chunk > 0 || sink || gate ? cache8_prompt_kernel<true> : cache8_prompt_kernel<false>, map, a);
   return launch_status();
 }

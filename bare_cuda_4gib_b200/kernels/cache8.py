@@ -6,6 +6,7 @@ Both go by the step's `StepMaps`.  Head sizes 64 and 128, bfloat16 queries and o
 from __future__ import annotations
 
 import ctypes
+import math
 from ctypes import c_float, c_int, c_longlong, c_void_p
 from typing import Dict, Optional
 
@@ -65,9 +66,11 @@ def _prompt(head_dim: int):
     if l is None:
         l = build.load_library("cache8_attention_tcgen05.cu", (f"-DHEAD_DIM={head_dim}",))
         P, I, L, F = c_void_p, c_int, c_longlong, c_float
-        l.llm_cache8_attention_prompt.argtypes = [P, P, P, P, I, I, F, I, I, P, P, L, P, P]
+        l.llm_cache8_attention_prompt.argtypes = [P, P, P, P, P, I, P, I, I, F, I, I, P, P, L, P, P]
         l.llm_cache8_attention_prompt.restype = c_int
         l.llm_cache8_attention_prompt_rows.restype = c_int
+        l.llm_cache8_prompt_pool_map.argtypes = [P, P, L, I]
+        l.llm_cache8_prompt_pool_map.restype = c_int
         l.tile_rows = int(l.llm_cache8_attention_prompt_rows())
         _prompt_libs[head_dim] = l
     return l
@@ -118,6 +121,17 @@ def _struct(cache: CacheView) -> int:
         cache.struct = _Cache8(cache.k_ptr, cache.v_ptr, cache.k_scale_ptr, cache.v_scale_ptr, cache.block_table.data_ptr(),
                                cache.page_stride, cache.scale_stride, cache.table_stride, cache.page_tokens, cache.kv_heads, cache.head_dim)
     return ctypes.addressof(cache.struct)
+
+
+def _pool_map(cache: CacheView):
+    """The prompt kernel's tensor map over the pool that the cache lies in, kept with the view: (its address, box rows)."""
+    if cache.pool_map is None:
+        box_rows = math.gcd(KEY_BLOCK, cache.page_tokens)
+        m = (ctypes.c_ubyte * 128)()
+        _check(_prompt(cache.head_dim).llm_cache8_prompt_pool_map(ctypes.addressof(m), cache.pool_ptr, cache.pool_elems // cache.head_dim, box_rows),
+               "cache8 pool map")
+        cache.pool_map = (m, ctypes.addressof(m), box_rows)
+    return cache.pool_map[1:]
 
 
 def _check_step(what: str, cache: CacheView, maps: StepMaps, q_heads: int, a: torch.Tensor, b: torch.Tensor) -> None:
@@ -209,7 +223,8 @@ def attention(q: torch.Tensor, out: torch.Tensor, cache: CacheView, maps: StepMa
             q.data_ptr(), out.data_ptr(), at, maps.lists, splits, rows, q_heads, scale, window, chunk, sink, gate, gate_stride, stream), "cache8_attention_decode")
     if maps.longest * group > FEW_ROWS:
         from . import gemm
+        pool_map, box_rows = _pool_map(cache)
         _check(_prompt(cache.head_dim).llm_cache8_attention_prompt(
-            q.data_ptr(), out.data_ptr(), at, maps.lists, prompt_splits(maps.n_tiles, cache.kv_heads, cache.table_stride * cache.page_tokens),
+            q.data_ptr(), out.data_ptr(), at, pool_map, cache.pool_ptr, box_rows, maps.lists, prompt_splits(maps.n_tiles, cache.kv_heads, cache.table_stride * cache.page_tokens),
             q_heads, scale, window, chunk, sink, gate, gate_stride, gemm.error_word(q.device).data_ptr(), stream),
             "cache8_attention_prompt")
