@@ -13,7 +13,7 @@
 //   converters (4) write a tile's codes as halves, times what is left of their scale (exact down to 2^-15), into 128-byte-swizzled shared
 //                  memory.  Halves hold e4m3 exactly and one instruction converts two codes.  Key tiles and value tiles go through ONE ring
 //                  of slots in the order K(0) V(0) K(1) ...;
-//   MMA issuer (1) S_g = Q_g K^T (M 128, N 128, K head size) into tile g's S columns of tensor memory, and
+//   MMA issuers (2) S_g = Q_g K^T (M 128, N 128, K head size) into tile g's S columns of tensor memory, and
 //                  O_g (+)= P_g V with P_g as the operand in tensor memory and V as it lies ([key][channel], MN-major), in two halves of 64
 //                  keys, each as soon as its half of P is there: P never goes through shared memory, whose bandwidth
 //                  is what a block with P there is bound by (K and V tiles, two Q tiles and two P tiles a key block);
@@ -23,16 +23,16 @@
 // A weight goes into P together with the scale of its block's values: P = 2^(s + e_V - m) with m the running maximum of s + e_V, while the sum
 // takes P 2^-e_V.  So a half of P is relative to what the row's keys can add to its output, and O needs no factor of its own.
 // m follows the true maximum only when that has grown by more than 2^8 (a half reaches 2^15), so O is rescaled rarely.
-// At head size 128 a tile's P takes the columns of its S (S 2 x 128, O 2 x 128 columns of the 512): its next S is issued when P has been
-// read, and the other tile's softmax fills that time; at head size 64 P has columns of its own.
+// A half of P takes the columns of the scores it was made of (S 2 x 128, O 2 x head size columns of the 512), and the next key block's half of S is
+// issued when P has been read, while the softmax is at the other half: it waits for no product.
 // Few tiles (a question behind a long text): the key blocks are split among the blocks of a cluster, each with a softmax of its own; their
 // states are merged in index order through distributed shared memory.
 // A NaN scale (a block that was given a NaN) makes keys NaN, hence the scores of the rows that see them; hidden scores are replaced, not
 // multiplied, and values are finite always.  Values behind the request's last key are written as zeros.
 // Every mbarrier wait is bounded: on a timeout the thread sets the error word, all roles leave their loops, tensor memory is
 // released and the block returns.
-// One B200: a prompt of 2,048 tokens (32 / 4 heads of 64) 46.8 us, 2,048 tokens behind 2,048 (32 heads of 128) 169 us, 61 tokens behind 3,001
-// (32 / 8 heads of 128) 26.2 us.
+// One B200: a prompt of 2,048 tokens (32 / 4 heads of 64) 44.2 us, 2,048 tokens behind 2,048 (32 heads of 128) 127 us, 61 tokens behind 3,001
+// (32 / 8 heads of 128) 23.5 us.
 
 #include "cache8.cuh"
 
@@ -59,12 +59,11 @@ constexpr int TILE_BYTES = KA * SUB;     // one key tile or one value tile
 constexpr int RAW_BYTES = BN * D;        // one key tile or one value tile as codes
 constexpr int SLOTS = HEAD_DIM == 64 ? 6 : 3, RAW_SLOTS = HEAD_DIM == 64 ? 6 : 4;   // tiles in flight, as halves and as codes (what shared memory allows)
 constexpr int SOFTMAX_THREADS = 128 * TILES, CONVERT_THREADS = 128;
-constexpr int CONVERT_WARP = SOFTMAX_THREADS / 32, MMA_WARP = CONVERT_WARP + CONVERT_THREADS / 32, LOADER_WARP = MMA_WARP + 1;
-constexpr int NUM_THREADS = (LOADER_WARP + 1) * 32;   // warps 0-7 softmax, 8-11 converters, 12 MMA, 13 loader
+constexpr int CONVERT_WARP = SOFTMAX_THREADS / 32, MMA_WARP = CONVERT_WARP + CONVERT_THREADS / 32, LOADER_WARP = MMA_WARP + TILES;
+constexpr int NUM_THREADS = (LOADER_WARP + 1) * 32;   // warps 0-7 softmax, 8-11 converters, 12 and 13 MMA (one a tile), 14 loader
 constexpr int GROUP_THREADS = 128;
 constexpr int S_PIECE = 64;      // columns of S a softmax thread holds in registers at a time
-constexpr bool SHARED_COLUMNS = HEAD_DIM == 128;   // whether P lies in the columns of S
-constexpr int TMEM_COLS = 512, O_COL = TILES * BN, P_COL = O_COL + TILES * D;
+constexpr int TMEM_COLS = 512, O_COL = TILES * BN;
 constexpr unsigned long long WAIT_LIMIT_NS = 1000000000ull;
 constexpr float RESCALE_STEP = 8.0f;
 constexpr int CHUNKS = D / 16;              // 16-byte chunks of a key's codes; also how many of them a converter thread takes of a tile
@@ -201,6 +200,28 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+// Two float32 numbers in one register pair, and one instruction for both.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ void unpair(uint64_t a, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // Four codes as four halves.
 __device__ __forceinline__ void halves(uint32_t codes, uint32_t& lo, uint32_t& hi) {
   asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
@@ -255,15 +276,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
   uint8_t* raw_ring = ring + SLOTS * TILE_BYTES;       // [RAW_SLOTS]: the same tiles as codes
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + TILES_BYTES);
   uint64_t* tile_full = bars;               // [SLOTS] converters -> MMA (and softmax): the slot's tile is written
-  uint64_t* tile_empty = tile_full + SLOTS; // [SLOTS] MMA (commit) -> converters
+  uint64_t* tile_empty = tile_full + SLOTS; // [SLOTS] both MMA issuers (commit) -> converters
   uint64_t* raw_full = tile_empty + SLOTS;  // [RAW_SLOTS] loader -> converters: the slot's codes have landed
   uint64_t* raw_empty = raw_full + RAW_SLOTS; // [RAW_SLOTS] converters -> loader
   uint64_t* q_full = raw_empty + RAW_SLOTS; // [2] softmax group -> MMA: Q_g staged
-  uint64_t* s_full = q_full + 2;            // [2] MMA (commit) -> softmax, per group
-  uint64_t* s_free = s_full + 2;            // [2] softmax -> MMA: the group holds its S values in registers (P in columns of its own)
-  uint64_t* p_full = s_free + 2;            // [2][2] softmax -> MMA: half h of P written, per group
-  uint64_t* pv_done = p_full + 4;           // [2][2] MMA (commit) -> softmax: the product with half h is complete, per group
-  int2* exponents = reinterpret_cast<int2*>(pv_done + 4);   // [EXPONENTS] of a key block's keys and values
+  uint64_t* s_full = q_full + 2;            // [2][2] MMA (commit) -> softmax, per group and half of 64 keys
+  uint64_t* p_full = s_full + 4;            // [2][2] softmax -> MMA: half h of P written
+  uint64_t* pv_done = p_full + 4;           // [2][2] MMA (commit) -> softmax, MMA: the product with half h is complete
+  uint64_t* known = pv_done + 4;            // [EXPONENTS] loader -> softmax: a key block's exponents
+  int2* exponents = reinterpret_cast<int2*>(known + EXPONENTS);   // [EXPONENTS] of a key block's keys and values
   uint32_t* factors = reinterpret_cast<uint32_t*>(exponents + EXPONENTS);   // [RAW_SLOTS][BLOCKS] what is left of a scale, twice as a half; 0: zeros
   uint32_t* tmem_slot = factors + RAW_SLOTS * BLOCKS;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -317,18 +338,16 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&pool_map)) : "memory");
     for (int s = 0; s < SLOTS; ++s) {
       mbar_init(&tile_full[s], CONVERT_THREADS / 32);
-      mbar_init(&tile_empty[s], 1);
+      mbar_init(&tile_empty[s], TILES);
     }
+    for (int s = 0; s < EXPONENTS; ++s) mbar_init(&known[s], 1);
     for (int s = 0; s < RAW_SLOTS; ++s) {
       mbar_init(&raw_full[s], 1);
       mbar_init(&raw_empty[s], CONVERT_THREADS / 32);
     }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(&q_full[b], GROUP_THREADS);
-      mbar_init(&s_full[b], 1);
-      mbar_init(&s_free[b], GROUP_THREADS);
-    }
+    for (int b = 0; b < 2; ++b) mbar_init(&q_full[b], GROUP_THREADS);
     for (int b = 0; b < 4; ++b) {
+      mbar_init(&s_full[b], 1);
       mbar_init(&p_full[b], GROUP_THREADS);
       mbar_init(&pv_done[b], 1);
     }
@@ -455,7 +474,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
       page = find_page(jj + 2);
       int ek, ev;
       const uint32_t fk = split_scale(now, now.k_scale, ek), fv = split_scale(now, now.v_scale, ev);
-      if (lane == 0) exponents[jj % EXPONENTS] = make_int2(ek, ev);
+      if (lane == 0) {
+        exponents[jj % EXPONENTS] = make_int2(ek, ev);
+        mbar_arrive(&known[jj % EXPONENTS]);
+      }
       const uint32_t copies = __popc(__ballot_sync(0xffffffffu, leads && now.row >= 0));
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
@@ -484,108 +506,68 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
       }
       __syncwarp();
     }
-  } else if (warp == MMA_WARP) {
-    // ------------------------------------------------------------------ MMA issuer
+  } else if (warp < LOADER_WARP && warp >= MMA_WARP) {
+    // ------------------------------------------------------------------ MMA issuers: one a tile, which waits for nothing that its tile does not
+    // need (a single one that asked for both tiles' events in turn took about 1,000 cycles from an event to its product)
     if (n_kb > 0 && elect_one()) {
-      constexpr uint32_t idesc_s = instr_desc(BM, BN, 0);
+      constexpr uint32_t idesc_s = instr_desc(BM, S_PIECE, 0);
       constexpr uint32_t idesc_o = instr_desc(BM, D, 1);
-      auto active = [&](int g, int jj) { return kb_lo + jj >= g_lo[g] && kb_lo + jj < g_hi[g]; };
-      // S_g = Q_g K(jj)^T into group g's S buffer; `last`: no product after this one reads the key tile
-      auto issue_s = [&](int g, int jj, bool last) {
-        const int slot = (2 * jj) % SLOTS;
+      const int g = warp - MMA_WARP, lo = (g ? g_lo[1] : g_lo[0]) - kb_lo, hi = (g ? g_hi[1] : g_hi[0]) - kb_lo;   // of the block's key blocks, its
+      const uint32_t s_tmem = tmem_base + g * BN, o_tmem = tmem_base + O_COL + g * D;
+      const uint64_t q_desc = smem_desc_sw128(smem_u32(q_smem) + g * Q_BYTES);
+      bool ok = true;
+      auto landed = [&](int n) { return mbar_wait(&tile_full[n % SLOTS], (uint32_t)(n / SLOTS) & 1u, abort_flag); };
+      // half h of S_g = Q_g K(jj)^T
+      auto issue_s = [&](int jj, int h) {
+        const int slot = (2 * jj) % SLOTS, i = jj - lo;
+        ok = ok && (h > 0 || landed(2 * jj)) && (i > 0 ? mbar_wait(&pv_done[g * 2 + h], (uint32_t)(i - 1) & 1u, abort_flag)   // P(i - 1) has been read
+                                                       : h > 0 || mbar_wait(&q_full[g], 0, abort_flag));
+        if (!ok) return;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t k_addr = smem_u32(ring) + slot * TILE_BYTES, q_addr = smem_u32(q_smem) + g * Q_BYTES;
+        const uint64_t k_desc = smem_desc_sw128(smem_u32(ring) + slot * TILE_BYTES + h * S_PIECE * 128);
 #pragma unroll
         for (int at = 0; at < KA; ++at)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            umma_ss(tmem_base + g * BN, smem_desc_sw128(q_addr + at * SUB) + 2 * k, smem_desc_sw128(k_addr + at * SUB) + 2 * k, idesc_s,
-                    (at > 0 || k > 0) ? 1u : 0u);
-        umma_commit(&s_full[g]);
-        if (last) umma_commit(&tile_empty[slot]);
+            umma_ss(s_tmem + h * S_PIECE, q_desc + (at * SUB >> 4) + 2 * k, k_desc + (at * SUB >> 4) + 2 * k, idesc_s, (at > 0 || k > 0) ? 1u : 0u);
+        umma_commit(&s_full[g * 2 + h]);
+        if (h == 1) umma_commit(&tile_empty[slot]);
       };
-      // O_g (+)= half h of P_g V(jj): the group's O accumulates in tensor memory over its key blocks (`first`: overwrite)
-      auto issue_pv = [&](int g, int jj, int h, bool last, bool first) {
-        const int slot = (2 * jj + 1) % SLOTS;
+      // O_g (+)= half h of P_g V(jj): the group's O accumulates in tensor memory over its key blocks
+      auto issue_pv = [&](int jj, int h) {
+        const int slot = (2 * jj + 1) % SLOTS, i = jj - lo;
+        ok = ok && (h > 0 || landed(2 * jj + 1)) && mbar_wait(&p_full[g * 2 + h], (uint32_t)i & 1u, abort_flag);
+        if (!ok) return;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t v_addr = smem_u32(ring) + slot * TILE_BYTES;
-        const uint32_t p_addr = tmem_base + (SHARED_COLUMNS ? g * BN + h * S_PIECE : P_COL + g * (BN / 2) + h * (S_PIECE / 2));
+        const uint64_t v_desc = smem_desc_sw128(smem_u32(ring) + slot * TILE_BYTES, SUB);
 #pragma unroll
         for (int kk = 0; kk < S_PIECE / 16; ++kk)
-          umma_ts(tmem_base + O_COL + g * D, p_addr + kk * 8, smem_desc_sw128(v_addr, SUB) + (uint64_t)((h * (S_PIECE / 16) + kk) * 2048 >> 4),
-                  idesc_o, (kk > 0 || !first) ? 1u : 0u);
+          umma_ts(o_tmem, s_tmem + h * S_PIECE + kk * 8, v_desc + (uint64_t)((h * (S_PIECE / 16) + kk) * 2048 >> 4), idesc_o,
+                  (kk > 0 || h > 0 || i > 0) ? 1u : 0u);
         umma_commit(&pv_done[g * 2 + h]);
-        if (last) umma_commit(&tile_empty[slot]);
+        if (h == 1) umma_commit(&tile_empty[slot]);
       };
-      // The two groups are served as they come.  Nothing is waited for while the other group could be served.
-      bool ok = true;
-      int s_next[TILES] = {}, pv_next[TILES] = {};      // per group: its next block to issue S for, its next half block to issue P V for
-      int n_g[TILES];
+      auto pass = [&](int jj) {       // a key block that only the other tile reads
 #pragma unroll
-      for (int g = 0; g < TILES; ++g) n_g[g] = g_hi[g] - g_lo[g];
-      // Whether tile n has landed.  A barrier's parity tells one filling of a slot only from the one before it.
-      // Groups that start with the same key block ask for the tiles as the slots are filled.  A group whose
-      // first key block lies behind the other's (a window, or a later block of positions) would take an
-      // earlier filling for its own: there the tiles are counted off in order.
-      const bool counted = EXTRAS && g_lo[0] != g_lo[1];
-      int arrived = 0, arrived_slot = 0;
-      uint32_t arrived_parity = 0;
-      auto landed = [&](int n) {
-        if (counted) {
-          while (arrived <= n) {
-            if (!mbar_try_wait(&tile_full[arrived_slot], arrived_parity)) return false;
-            ++arrived;
-            if (++arrived_slot == SLOTS) arrived_slot = 0, arrived_parity ^= 1u;
-          }
-          return true;
+        for (int which = 0; which < 2; ++which) {
+          ok = ok && landed(2 * jj + which);
+          if (ok) mbar_arrive(&tile_empty[(2 * jj + which) % SLOTS]);
         }
-        return mbar_try_wait(&tile_full[n % SLOTS], (n / SLOTS) & 1);
       };
-      // whether group g's S buffer may be written for its block i
-      auto s_ready = [&](int g, int i) {
-        if (i == 0) return mbar_try_wait(&q_full[g], 0);
-        if (SHARED_COLUMNS) return pv_next[g] == 2 * i && mbar_try_wait(&pv_done[g * 2 + 1], (i - 1) & 1);   // (and with it half 0)
-        return mbar_try_wait(&s_free[g], (i - 1) & 1);
-      };
-      unsigned long long idle_since = 0;
-      unsigned idle_spins = 0;
-      while (ok && (pv_next[0] < 2 * n_g[0] || pv_next[1] < 2 * n_g[1])) {
-        bool progress = false;
-#pragma unroll
-        for (int g = 0; g < TILES; ++g) {
-          const int o = 1 - g;   // the other group
-          if (pv_next[g] < 2 * s_next[g]) {
-            const int i = pv_next[g] >> 1, h = pv_next[g] & 1, jj = g_lo[g] + i - kb_lo;
-            if (mbar_try_wait(&p_full[g * 2 + h], (uint32_t)i & 1u) && landed(2 * jj + 1)) {
-              // the other group is done with V(jj) if it never reads it or has issued its product already
-              const bool last = h == 1 && (!active(o, jj) || pv_next[o] > 2 * (kb_lo + jj - g_lo[o]) + 1);
-              issue_pv(g, jj, h, last, pv_next[g] == 0);
-              ++pv_next[g];
-              progress = true;
-            }
+      for (int jj = 0; jj < (lo < hi ? lo : n_kb) && ok; ++jj) pass(jj);
+      if (lo < hi) {
+        issue_s(lo, 0);
+        issue_s(lo, 1);
+        for (int jj = lo; jj < hi && ok; ++jj)
+          for (int h = 0; h < 2; ++h) {
+            issue_pv(jj, h);
+            if (jj + 1 < hi) issue_s(jj + 1, h);
           }
-          if (s_next[g] < n_g[g]) {
-            const int i = s_next[g], jj = g_lo[g] + i - kb_lo;
-            if (s_ready(g, i) && landed(2 * jj)) {
-              const bool last = !active(o, jj) || s_next[o] > kb_lo + jj - g_lo[o];
-              issue_s(g, jj, last);
-              s_next[g] = i + 1;
-              progress = true;
-            }
-          }
-        }
-        if (progress) {
-          idle_spins = 0;
-        } else if ((++idle_spins & 63u) == 0u) {
-          if (idle_spins == 64u) idle_since = global_timer();
-          if (*abort_flag || global_timer() - idle_since > WAIT_LIMIT_NS) ok = false;
-        }
+        for (int jj = hi; jj < n_kb && ok; ++jj) pass(jj);
       }
       if (!ok) {
         *abort_flag = 1;
         atomicCAS(a.error_word, 0, ERR_MMA);
-        for (int b = 0; b < TILES; ++b) umma_commit(&s_full[b]);   // release whoever waits
-        for (int b = 0; b < 2 * TILES; ++b) umma_commit(&pv_done[b]);
       }
     }
   } else {
@@ -627,26 +609,21 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
     auto wait_pv = [&](int k, int h) { return mbar_wait(&pv_done[g * 2 + h], (uint32_t)k & 1u, abort_flag); };
     bool ok = true;
     for (int i = 0; i < my_n && ok; ++i) {
-      const int jj = my_lo + i - kb_lo, key0 = (my_lo + i) * BN, v_tile = 2 * jj + 1;
-      // the exponents were written ahead of the value tile (which stays until this group has read it)
-      ok = mbar_wait(&s_full[g], i & 1, abort_flag) && mbar_wait(&tile_full[v_tile % SLOTS], (uint32_t)(v_tile / SLOTS) & 1u, abort_flag) &&
-           !*abort_flag;
-      if (!ok) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const int jj = my_lo + i - kb_lo, key0 = (my_lo + i) * BN;
+      ok = mbar_wait(&known[jj % EXPONENTS], (uint32_t)(jj / EXPONENTS) & 1u, abort_flag);
       const int2 e = exponents[jj % EXPONENTS];
       const float c = factor * power_of_two(e.x), ev = (float)e.y;
       const bool all_visible = key0 + BN - 1 <= tile_min_pos && (!EXTRAS || key0 >= tile_max_lo);
-      float l0 = 0.0f, l1 = 0.0f, l2 = 0.0f, l3 = 0.0f;
+      uint64_t l2[2] = {0, 0};      // the block's part of the sum, four parts of it
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        ok = ok && mbar_wait(&s_full[g * 2 + h], (uint32_t)i & 1u, abort_flag) && !*abort_flag;
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         uint32_t v[S_PIECE];
 #pragma unroll
         for (int k = 0; k < S_PIECE; k += 32) tmem_load32_nowait(s_addr + h * S_PIECE + k, v + k);
         tmem_wait_loads();
-        if (!SHARED_COLUMNS && h == 1) {   // the last read of S(i): the MMA thread may overwrite the buffer with S(i + 1)
-          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-          mbar_arrive(&s_free[g]);
-        }
         if (!all_visible) {
 #pragma unroll
           for (int k = 0; k < S_PIECE; ++k) {
@@ -655,27 +632,26 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
             if (!visible) v[k] = 0xff800000u;   // -inf: probability 0
           }
         }
-        float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+        float mx0 = __uint_as_float(v[0]), mx1 = __uint_as_float(v[1]), mx2 = __uint_as_float(v[2]), mx3 = __uint_as_float(v[3]);
 #pragma unroll
-        for (int k = 0; k < S_PIECE; k += 8) {   // four independent partial maxima
-          mx0 = fmaxf(mx0, fmaxf(__uint_as_float(v[k]), __uint_as_float(v[k + 1])));
-          mx1 = fmaxf(mx1, fmaxf(__uint_as_float(v[k + 2]), __uint_as_float(v[k + 3])));
-          mx2 = fmaxf(mx2, fmaxf(__uint_as_float(v[k + 4]), __uint_as_float(v[k + 5])));
-          mx3 = fmaxf(mx3, fmaxf(__uint_as_float(v[k + 6]), __uint_as_float(v[k + 7])));
+        for (int k = 4; k < S_PIECE - 4; k += 8) {   // four independent partial maxima
+          mx0 = max3(mx0, __uint_as_float(v[k]), __uint_as_float(v[k + 1]));
+          mx1 = max3(mx1, __uint_as_float(v[k + 2]), __uint_as_float(v[k + 3]));
+          mx2 = max3(mx2, __uint_as_float(v[k + 4]), __uint_as_float(v[k + 5]));
+          mx3 = max3(mx3, __uint_as_float(v[k + 6]), __uint_as_float(v[k + 7]));
         }
-        const float m_new = fmaxf(m, fmaf(fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)), c, ev));   // c > 0: the maximum commutes with it
+        mx0 = max3(mx0, __uint_as_float(v[S_PIECE - 4]), __uint_as_float(v[S_PIECE - 3]));
+        mx1 = max3(mx1, __uint_as_float(v[S_PIECE - 2]), __uint_as_float(v[S_PIECE - 1]));
+        const float m_new = fmaxf(m, fmaf(fmaxf(max3(mx0, mx1, mx2), mx3), c, ev));   // c > 0: the maximum commutes with it
         // tensor-memory loads and stores are warp-wide: the warp moves its maxima together, as soon as one of
         // its rows has outgrown its own by the step (a row that has not may follow the true maximum just as well)
         const bool move = __any_sync(0xffffffffu, m_new > m + RESCALE_STEP);
-        if (!SHARED_COLUMNS && i > 0 && !wait_pv(i - 1, h)) {   // half h of P(i) goes where that of P(i - 1) lay
-          ok = false;
-          break;
-        }
         if (move) {
           const float corr = fast_exp2(m - (m_new == -INFINITY ? 0.0f : m_new));   // m = -inf gives 0
           m = m_new;
           l *= corr;
-          l0 *= corr, l1 *= corr, l2 *= corr, l3 *= corr;
+          l2[0] = fma2(l2[0], pair(corr, corr), 0);
+          l2[1] = fma2(l2[1], pair(corr, corr), 0);
           if (i > 0 || h > 0) {     // O = O * corr in tensor memory, when every product issued so far is complete
             if (!(h > 0 ? wait_pv(i, 0) : wait_pv(i - 1, 1))) {
               ok = false;
@@ -694,23 +670,25 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
           }
         }
         const float shift = ev - (m == -INFINITY ? 0.0f : m);
+        const uint64_t c2 = pair(c, c), shift2 = pair(shift, shift);
         uint32_t packed[S_PIECE / 2];
 #pragma unroll
         for (int k = 0; k < S_PIECE; k += 2) {
-          const float p0 = fast_exp2(fmaf(__uint_as_float(v[k]), c, shift)), p1 = fast_exp2(fmaf(__uint_as_float(v[k + 1]), c, shift));
-          if ((k & 6) == 0) l0 += p0 + p1;
-          else if ((k & 6) == 2) l1 += p0 + p1;
-          else if ((k & 6) == 4) l2 += p0 + p1;
-          else l3 += p0 + p1;
+          float x0, x1;
+          unpair(fma2(pair(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), c2, shift2), x0, x1);
+          const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+          l2[k / 2 % 2] = add2(l2[k / 2 % 2], pair(p0, p1));
           packed[k / 2] = pack_half(p0, p1);
         }
-        tmem_store32(SHARED_COLUMNS ? s_addr + h * S_PIECE : lane_addr + P_COL + g * (BN / 2) + h * (S_PIECE / 2), packed);
+        tmem_store32(s_addr + h * S_PIECE, packed);      // over the scores that it was made of
         tmem_wait_stores();
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         mbar_arrive(&p_full[g * 2 + h]);
       }
       if (!ok) break;
-      l = fmaf((l0 + l1) + (l2 + l3), power_of_two(-e.y), l);
+      float part0, part1;
+      unpair(add2(l2[0], l2[1]), part0, part1);
+      l = fmaf(part0 + part1, power_of_two(-e.y), l);
     }
     if (ok && my_n > 0) ok = wait_pv(my_n - 1, 1) && !*abort_flag;
     if (!ok) {
