@@ -7,28 +7,26 @@
 //
 // One thread block = two tiles of 128 packed rows of one request and one key/value head, which share every key and value block of 128
 // positions.  Warps:
-//   loader (1)     copies a key block's codes, as they lie in the request's pages, into a ring of their own with TMA (one tensor map over the cache's
-//                  pool, a box per piece of a page), and splits the block's scales into 2^e (the largest, which the softmax gets) and what is
-//                  left for 16 positions, at most one, which the converters get;
-//   converters (4) write a tile's codes as halves, times what is left of their scale (exact down to 2^-15), into 128-byte-swizzled shared
-//                  memory.  Halves hold e4m3 exactly and one instruction converts two codes.  Key tiles and value tiles go through ONE ring
-//                  of slots in the order K(0) V(0) K(1) ...;
-//   MMA issuers (2) S_g = Q_g K^T (M 128, N 128, K head size) into tile g's S columns of tensor memory, and
-//                  O_g (+)= P_g V with P_g as the operand in tensor memory and V as it lies ([key][channel], MN-major), in two halves of 64
-//                  keys, each as soon as its half of P is there: P never goes through shared memory, whose bandwidth
-//                  is what a block with P there is bound by (K and V tiles, two Q tiles and two P tiles a key block);
-//   softmax (8)    a group of four warps per tile, one thread per row.  First it stages Q_g as halves (times a power of two of
-//                  the row's own).  Then, per key block: read the row of S, 64 columns at a time, mask, running maximum and sum in
-//                  float32 (base 2), write P as halves back into tensor memory.
-// A weight goes into P together with the scale of its block's values: P = 2^(s + e_V - m) with m the running maximum of s + e_V, while the sum
-// takes P 2^-e_V.  So a half of P is relative to what the row's keys can add to its output, and O needs no factor of its own.
+//   loader (1)     copies a key block's codes, as they lie in the request's pages, into shared memory with TMA (one tensor map over the cache's
+//                  pool, a box per piece of a page), and hands the block's scales to the softmax;
+//   converters (4) write the value codes as halves (which hold e4m3 exactly, two a conversion) into 128-byte-swizzled tiles;
+//   MMA issuers (2, one a tile)  S_g = Q_g K^T (M 128, N 64, twice a key block) with the keys as the codes they are: an 8-bit product.  Q_g is the sum of two
+//                  e4m3 tiles, which together hold a bfloat16's eight bits exactly (but for entries 2^10 below their row's largest; those are 2^-18 of it off), times a power of
+//                  two of the row's own; two products at twice the rate of one in 16 bits, and no key is ever converted.
+//                  O_g (+)= P_g V in halves of 64 keys, each as soon as its half of P is there, with P_g as the operand in tensor memory and V as it
+//                  lies ([key][channel], MN-major): P never goes through shared memory, whose bandwidth bounds a block that has it there;
+//   softmax (8)    a group of four warps per tile, one thread per row.  First it stages Q_g.  Then, per half of 64 keys: read the row of S, mask,
+//                  running maximum and sum in float32 (base 2), write P as halves back into tensor memory.
+// The scales cost the softmax nothing but their constants: the keys' joins the factor of 16 scores, and a weight goes into P together with the
+// scale of its values: P = 2^(s + e_V - m) with m the running maximum of s + e_V, while the sum takes P 2^-e_V.  So a half of P is relative to
+// what the row's keys can add to its output, and O needs no factor of its own.
 // m follows the true maximum only when that has grown by more than 2^8 (a half reaches 2^15), so O is rescaled rarely.
 // A half of P takes the columns of the scores it was made of (S 2 x 128, O 2 x head size columns of the 512), and the next key block's half of S is
 // issued when P has been read, while the softmax is at the other half: it waits for no product.
 // Few tiles (a question behind a long text): the key blocks are split among the blocks of a cluster, each with a softmax of its own; their
 // states are merged in index order through distributed shared memory.
-// A NaN scale (a block that was given a NaN) makes keys NaN, hence the scores of the rows that see them; hidden scores are replaced, not
-// multiplied, and values are finite always.  Values behind the request's last key are written as zeros.
+// A NaN scale (a block that was given a NaN) makes NaN of its 16 scores before hidden ones are replaced, so that only rows that see
+// the block get it; values are finite always, and behind the request's last key, or where no page is held, written as zeros.
 // Every mbarrier wait is bounded: on a timeout the thread sets the error word, all roles leave their loops, tensor memory is
 // released and the block returns.
 // One B200: a prompt of 2,048 tokens (32 / 4 heads of 64) 44.2 us, 2,048 tokens behind 2,048 (32 heads of 128) 127 us, 61 tokens behind 3,001
@@ -48,16 +46,15 @@ namespace {
 
 constexpr int D = HEAD_DIM;
 static_assert(D == 64 || D == 128, "the tcgen05 attention kernel is built for head sizes 64 and 128");
-constexpr int KA = D / 64;       // 64-wide sub-tiles ("atoms") along the head dimension
 constexpr int BM = 128;          // packed rows per tile (one softmax group)
-constexpr int TILES = 2;         // tiles per block: both read every converted key and value tile
+constexpr int TILES = 2;         // tiles per block: both read every key and value tile
 constexpr int BLOCK_ROWS = TILES * BM;
 constexpr int BN = 128;          // keys per block
-constexpr int SUB = 128 * 128;   // bytes of a [128 rows x 64 halves] swizzled sub-tile
-constexpr int Q_BYTES = KA * SUB;        // one tile's queries
-constexpr int TILE_BYTES = KA * SUB;     // one key tile or one value tile
-constexpr int RAW_BYTES = BN * D;        // one key tile or one value tile as codes
-constexpr int SLOTS = HEAD_DIM == 64 ? 6 : 3, RAW_SLOTS = HEAD_DIM == 64 ? 6 : 4;   // tiles in flight, as halves and as codes (what shared memory allows)
+constexpr int CODES = BN * D;    // bytes of a key tile, of a value tile as codes, and of each part of a tile's queries
+constexpr int SUB = 128 * 128;   // bytes of a [128 keys x 64 halves] swizzled sub-tile
+constexpr int VALUES = D / 64 * SUB;     // bytes of a value tile as halves
+// what is in flight (as shared memory allows): key tiles, value tiles as codes, value tiles as halves
+constexpr int K_SLOTS = 4, C_SLOTS = HEAD_DIM == 64 ? 4 : 2, V_SLOTS = HEAD_DIM == 64 ? 4 : 2;
 constexpr int SOFTMAX_THREADS = 128 * TILES, CONVERT_THREADS = 128;
 constexpr int CONVERT_WARP = SOFTMAX_THREADS / 32, MMA_WARP = CONVERT_WARP + CONVERT_THREADS / 32, LOADER_WARP = MMA_WARP + TILES;
 constexpr int NUM_THREADS = (LOADER_WARP + 1) * 32;   // warps 0-7 softmax, 8-11 converters, 12 and 13 MMA (one a tile), 14 loader
@@ -68,11 +65,21 @@ constexpr unsigned long long WAIT_LIMIT_NS = 1000000000ull;
 constexpr float RESCALE_STEP = 8.0f;
 constexpr int CHUNKS = D / 16;              // 16-byte chunks of a key's codes; also how many of them a converter thread takes of a tile
 constexpr int BLOCKS = BN / SCALE_TOKENS;   // scale blocks of a key block
-constexpr int EXPONENTS = 16;               // key blocks whose exponents are kept (more than can be in flight)
+constexpr int KNOWN = 8;                    // key blocks whose scales are kept (a key tile's slot is free again at most five blocks on)
 constexpr int STATE = D + 4;                // floats of a row's state in a merge: D sums, the maximum, the sum
-constexpr size_t TILES_BYTES = (size_t)TILES * Q_BYTES + (size_t)SLOTS * TILE_BYTES + (size_t)RAW_SLOTS * RAW_BYTES;
+constexpr size_t TILES_BYTES = (size_t)(TILES * 2 + K_SLOTS + C_SLOTS) * CODES + (size_t)V_SLOTS * VALUES;
 static_assert((size_t)BLOCK_ROWS * STATE * 4 <= TILES_BYTES, "the states of a merge lie over the tiles");
-constexpr size_t SMEM_BYTES = TILES_BYTES + 768;
+// A key block's scales as the softmax takes them, 16 positions each.
+struct Scales {
+  float key[BLOCKS];       // 2^e_K (1 where it is lost)
+  float value[BLOCKS];     // e_V
+  float back[BLOCKS];      // 2^-e_V
+  uint32_t lost, unused[3];   // bit b: scale block b has no number as its keys' scale
+};
+
+// barriers (two to a slot, 14 of the groups, one to a block of scales), scales, rows' exponents, what is held, two words; 16 for alignment
+constexpr size_t BOOK_BYTES = 8 * (2 * (K_SLOTS + C_SLOTS + V_SLOTS) + 14 + KNOWN) + 16 + KNOWN * sizeof(Scales) + 4 * (BLOCK_ROWS + C_SLOTS + 2);
+constexpr size_t SMEM_BYTES = TILES_BYTES + BOOK_BYTES;
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -126,7 +133,7 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
 }
 // Byte offset of chunk `chunk` of row `row` in a tile of codes as TMA writes it: 128-byte swizzle for rows of 128 bytes, 64-byte swizzle
 // for rows of 64.
-__device__ __forceinline__ uint32_t raw_swizzled(int row, int chunk) {
+__device__ __forceinline__ uint32_t codes_swizzled(int row, int chunk) {
   return (uint32_t)(row * D + ((D == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) << 4));
 }
 
@@ -141,16 +148,27 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t addr, uint32_t lead
   return d;
 }
 
-// float32 accumulator, half operands, A K-major; B K-major or (b_mn = 1) MN-major.
+// The same for tiles of codes, whose rows are D bytes: 128-byte swizzle, or 64-byte swizzle with 512 bytes between 8-row groups.
+__device__ __forceinline__ uint64_t smem_desc_codes(uint32_t addr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((addr & 0x3FFFF) >> 4);
+  d |= (uint64_t)1 << 16;
+  d |= (uint64_t)(8 * D >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)(D == 128 ? 2 : 4) << 61;
+  return d;
+}
+
+// float32 accumulator, half operands (kind::f16) or e4m3 ones (kind::f8f6f4), A K-major; B K-major or (b_mn = 1) MN-major.
 __host__ __device__ constexpr uint32_t instr_desc(int m, int n, int b_mn) {
   return (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-__device__ __forceinline__ void umma_ss(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void umma_codes(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
       ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
 }
 // The A operand in tensor memory: lane = row, 32-bit column c = its elements 2 c and 2 c + 1.
@@ -227,15 +245,16 @@ __device__ __forceinline__ void halves(uint32_t codes, uint32_t& lo, uint32_t& h
   asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
       : "=r"(lo), "=r"(hi) : "r"(codes));
 }
-__device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+// Two numbers as two e4m3 codes.
+__device__ __forceinline__ uint32_t codes2(float lo, float hi) {
+  uint16_t d;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(hi), "f"(lo));
   return d;
 }
-// 2^-d twice as a half (zero where a half has no such number).
-__device__ __forceinline__ uint32_t half_power(int d) {
-  const uint32_t h = d <= 14 ? (uint32_t)(15 - d) << 10 : d <= 24 ? 1u << (24 - d) : 0u;
-  return h | (h << 16);
+__device__ __forceinline__ float2 numbers2(uint32_t codes) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)codes));
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 __device__ __forceinline__ uint32_t peer_smem(uint32_t local, uint32_t rank) {
   uint32_t remote;
@@ -271,22 +290,26 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
   const AttentionExtras extras = EXTRAS ? a.extras : AttentionExtras{0, nullptr, nullptr, 0};
   const int window = EXTRAS ? a.window : 0;
   extern __shared__ __align__(1024) uint8_t smem[];   // swizzled tiles need 1024-byte alignment (checked below)
-  uint8_t* q_smem = smem;                              // [TILES][KA sub-tiles]
-  uint8_t* ring = q_smem + TILES * Q_BYTES;            // [SLOTS][KA sub-tiles]: key and value tiles in turn
-  uint8_t* raw_ring = ring + SLOTS * TILE_BYTES;       // [RAW_SLOTS]: the same tiles as codes
+  uint8_t* q_smem = smem;                              // [TILES][2]: the queries' two parts
+  uint8_t* k_ring = q_smem + TILES * 2 * CODES;        // [K_SLOTS]
+  uint8_t* c_ring = k_ring + K_SLOTS * CODES;          // [C_SLOTS]: values as codes
+  uint8_t* v_ring = c_ring + C_SLOTS * CODES;          // [V_SLOTS]: values as halves
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + TILES_BYTES);
-  uint64_t* tile_full = bars;               // [SLOTS] converters -> MMA (and softmax): the slot's tile is written
-  uint64_t* tile_empty = tile_full + SLOTS; // [SLOTS] both MMA issuers (commit) -> converters
-  uint64_t* raw_full = tile_empty + SLOTS;  // [RAW_SLOTS] loader -> converters: the slot's codes have landed
-  uint64_t* raw_empty = raw_full + RAW_SLOTS; // [RAW_SLOTS] converters -> loader
-  uint64_t* q_full = raw_empty + RAW_SLOTS; // [2] softmax group -> MMA: Q_g staged
+  uint64_t* k_full = bars;                  // [K_SLOTS] loader -> MMA: the slot's keys have landed
+  uint64_t* k_empty = k_full + K_SLOTS;     // [K_SLOTS] both MMA issuers (commit) -> loader
+  uint64_t* c_full = k_empty + K_SLOTS;     // [C_SLOTS] loader -> converters: the slot's value codes have landed
+  uint64_t* c_empty = c_full + C_SLOTS;     // [C_SLOTS] converters -> loader
+  uint64_t* v_full = c_empty + C_SLOTS;     // [V_SLOTS] converters -> MMA: the slot's values are written
+  uint64_t* v_empty = v_full + V_SLOTS;     // [V_SLOTS] both MMA issuers (commit) -> converters
+  uint64_t* q_full = v_empty + V_SLOTS;     // [2] softmax group -> MMA: Q_g staged
   uint64_t* s_full = q_full + 2;            // [2][2] MMA (commit) -> softmax, per group and half of 64 keys
   uint64_t* p_full = s_full + 4;            // [2][2] softmax -> MMA: half h of P written
   uint64_t* pv_done = p_full + 4;           // [2][2] MMA (commit) -> softmax, MMA: the product with half h is complete
-  uint64_t* known = pv_done + 4;            // [EXPONENTS] loader -> softmax: a key block's exponents
-  int2* exponents = reinterpret_cast<int2*>(known + EXPONENTS);   // [EXPONENTS] of a key block's keys and values
-  uint32_t* factors = reinterpret_cast<uint32_t*>(exponents + EXPONENTS);   // [RAW_SLOTS][BLOCKS] what is left of a scale, twice as a half; 0: zeros
-  uint32_t* tmem_slot = factors + RAW_SLOTS * BLOCKS;
+  uint64_t* known = pv_done + 4;            // [KNOWN] loader -> softmax: a key block's scales
+  Scales* scales = reinterpret_cast<Scales*>((reinterpret_cast<uintptr_t>(known + KNOWN) + 15) & ~uintptr_t(15));   // [KNOWN]
+  int* q_exponent = reinterpret_cast<int*>(scales + KNOWN);     // [BLOCK_ROWS] of the power of two taken out of a row of Q
+  uint32_t* held = reinterpret_cast<uint32_t*>(q_exponent + BLOCK_ROWS);   // [C_SLOTS] bit b: there are values for scale block b
+  uint32_t* tmem_slot = held + C_SLOTS;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   pdl_launch_dependents();
@@ -336,15 +359,19 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
 
   if (threadIdx.x == 0) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&pool_map)) : "memory");
-    for (int s = 0; s < SLOTS; ++s) {
-      mbar_init(&tile_full[s], CONVERT_THREADS / 32);
-      mbar_init(&tile_empty[s], TILES);
+    for (int s = 0; s < K_SLOTS; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], TILES);
     }
-    for (int s = 0; s < EXPONENTS; ++s) mbar_init(&known[s], 1);
-    for (int s = 0; s < RAW_SLOTS; ++s) {
-      mbar_init(&raw_full[s], 1);
-      mbar_init(&raw_empty[s], CONVERT_THREADS / 32);
+    for (int s = 0; s < C_SLOTS; ++s) {
+      mbar_init(&c_full[s], 1);
+      mbar_init(&c_empty[s], CONVERT_THREADS / 32);
     }
+    for (int s = 0; s < V_SLOTS; ++s) {
+      mbar_init(&v_full[s], CONVERT_THREADS / 32);
+      mbar_init(&v_empty[s], TILES);
+    }
+    for (int s = 0; s < KNOWN; ++s) mbar_init(&known[s], 1);
     for (int b = 0; b < 2; ++b) mbar_init(&q_full[b], GROUP_THREADS);
     for (int b = 0; b < 4; ++b) {
       mbar_init(&s_full[b], 1);
@@ -383,51 +410,44 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
     const int row_in = D == 128 ? (cw & 1) * 8 + ((lane >> 3) ^ ((lane >> 2) & 1) * 5) : cw * 8 + (lane >> 2);
     constexpr int STEP = BN / CHUNKS;             // rows from one of a thread's chunks to the next: one or two scale blocks
     bool ok = true;
-    for (int n = 0; n < 2 * n_kb; ++n) {
-      const int raw_slot = n % RAW_SLOTS, slot = n % SLOTS, use = n / SLOTS;
-      ok = mbar_wait(&raw_full[raw_slot], (uint32_t)(n / RAW_SLOTS) & 1u, abort_flag);
+    for (int jj = 0; jj < n_kb; ++jj) {
+      const int from_slot = jj % C_SLOTS, slot = jj % V_SLOTS, use = jj / V_SLOTS;
+      ok = mbar_wait(&c_full[from_slot], (uint32_t)(jj / C_SLOTS) & 1u, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       uint4 raw[CHUNKS];
-      uint32_t factor[CHUNKS];
-      const uint32_t from = smem_u32(raw_ring) + raw_slot * RAW_BYTES;
+      const uint32_t from = smem_u32(c_ring) + from_slot * CODES, there = held[from_slot];
 #pragma unroll
-      for (int i = 0; i < CHUNKS; ++i) {
-        const int row = row_in + i * STEP;
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(raw[i].x), "=r"(raw[i].y), "=r"(raw[i].z), "=r"(raw[i].w) : "r"(from + raw_swizzled(row, chunk)) : "memory");
-        factor[i] = factors[raw_slot * BLOCKS + row / SCALE_TOKENS];      // the same for the whole warp
+      for (int i = 0; i < CHUNKS; ++i)
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(raw[i].x), "=r"(raw[i].y), "=r"(raw[i].z), "=r"(raw[i].w) : "r"(from + codes_swizzled(row_in + i * STEP, chunk)) : "memory");
+      const int behind = kv_len - (kb_lo + jj) * BN;       // rows from here on lie behind the request's last key
+      if (behind < BN || there != (1u << BLOCKS) - 1u) {   // what lies where there are no values may be anything, and zero times NaN is not zero
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i) {
+          const int row = row_in + i * STEP;
+          if (row >= behind || !((there >> (row / SCALE_TOKENS)) & 1u)) raw[i] = make_uint4(0, 0, 0, 0);
+        }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&raw_empty[raw_slot]);
-      ok = use == 0 || mbar_wait(&tile_empty[slot], (uint32_t)(use - 1) & 1u, abort_flag);
+      if (lane == 0) mbar_arrive(&c_empty[from_slot]);
+      ok = use == 0 || mbar_wait(&v_empty[slot], (uint32_t)(use - 1) & 1u, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      const uint32_t to = smem_u32(ring) + slot * TILE_BYTES + (chunk >> 2) * SUB;
-      const int behind = kv_len - (kb_lo + (n >> 1)) * BN;       // rows from here on lie behind the request's last key
+      const uint32_t to = smem_u32(v_ring) + slot * VALUES + (chunk >> 2) * SUB;
 #pragma unroll
       for (int i = 0; i < CHUNKS; ++i) {
-        const int row = row_in + i * STEP;
+        const int row = row_in + i * STEP, first = (chunk & 3) * 2;
         uint32_t w[8];
         halves(raw[i].x, w[0], w[1]);
         halves(raw[i].y, w[2], w[3]);
         halves(raw[i].z, w[4], w[5]);
         halves(raw[i].w, w[6], w[7]);
-        if (factor[i] != 0x3c003c00u) {
-          // (where no page is held, or a scale is lost beside a far larger one, zeros; whatever lay there may be NaN)
-#pragma unroll
-          for (int k = 0; k < 8; ++k) w[k] = factor[i] ? mul_half2(w[k], factor[i]) : 0u;
-        }
-        if (row >= behind) {     // masked as keys, but as values zero times whatever lies there must be zero
-#pragma unroll
-          for (int k = 0; k < 8; ++k) w[k] = 0u;
-        }
-        const int first = (chunk & 3) * 2;
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + swizzled(row, first)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + swizzled(row, first + 1)), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(&tile_full[slot]);
+      if (lane == 0) mbar_arrive(&v_full[slot]);
     }
     if (!ok && lane == 0) {
       *abort_flag = 1;
@@ -455,45 +475,47 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
       }
       return p;
     };
-    // What is left of the lane's scale once the largest exponent of the key block is taken out, and that exponent.
-    auto split_scale = [&](const Place& p, float scale, int& most) {
-      const bool lost = isnan(scale), there = p.row >= 0 && !lost;
-      const int e = there ? exponent_of(scale) : -1000;
-      most = __reduce_max_sync(0xffffffffu, e);
-      if (most == -1000) most = 0;
-      return p.row < 0 ? 0u : lost ? 0x7e007e00u : half_power(most - e);
-    };
     const int per_piece = a.box_rows / SCALE_TOKENS;
     const bool leads = lane < BLOCKS && lane % per_piece == 0;      // a piece of a page is its first scale block's lane's to copy
     bool ok = true;
-    int issued = 0;
+    int k_issued = 0, c_issued = 0;
+    auto copy = [&](uint64_t* full, uint8_t* slot, const Place& p, long long row0, uint32_t copies) {
+      if (lane == 0) mbar_expect_tx(full, copies * a.box_rows * D);   // also the one arrival
+      __syncwarp();
+      if (leads && p.row >= 0) tma_load_2d(smem_u32(slot) + lane * SCALE_TOKENS * D, &pool_map, full, 0, (int)(p.row + row0));
+    };
     Place now = place(0, find_page(0));
-    int page = find_page(1);
-    for (int jj = 0; jj < n_kb && ok; ++jj) {
+    int page = -1;
+    for (int jj = 0; jj < n_kb; ++jj) {
+      const uint32_t there = __ballot_sync(0xffffffffu, now.row >= 0), copies = __popc(__ballot_sync(0xffffffffu, leads && now.row >= 0));
+      const int ks = jj % K_SLOTS, cs = jj % C_SLOTS;
+      ok = jj < K_SLOTS || mbar_wait(&k_empty[ks], (uint32_t)(jj / K_SLOTS - 1) & 1u, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      copy(&k_full[ks], k_ring + ks * CODES, now, a.k_row0, copies);
+      k_issued = jj + 1;
+      ok = jj < C_SLOTS || mbar_wait(&c_empty[cs], (uint32_t)(jj / C_SLOTS - 1) & 1u, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (lane == 0) held[cs] = there;
+      copy(&c_full[cs], c_ring + cs * CODES, now, a.v_row0, copies);
+      c_issued = jj + 1;
+      if (jj == 0) page = find_page(1);
       const Place next = place(jj + 1, page);
       page = find_page(jj + 2);
-      int ek, ev;
-      const uint32_t fk = split_scale(now, now.k_scale, ek), fv = split_scale(now, now.v_scale, ev);
-      if (lane == 0) {
-        exponents[jj % EXPONENTS] = make_int2(ek, ev);
-        mbar_arrive(&known[jj % EXPONENTS]);
+      // the scales, while the codes are on their way
+      const bool lost = isnan(now.k_scale);
+      Scales* to = scales + jj % KNOWN;
+      if (lane < BLOCKS) {
+        const int ev = now.row >= 0 ? exponent_of(now.v_scale) : 0;
+        to->key[lane] = now.row >= 0 && !lost ? now.k_scale : 1.0f;
+        to->value[lane] = (float)ev;
+        to->back[lane] = power_of_two(-ev);
       }
-      const uint32_t copies = __popc(__ballot_sync(0xffffffffu, leads && now.row >= 0));
-#pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        const int n = 2 * jj + which, slot = n % RAW_SLOTS, use = n / RAW_SLOTS;
-        ok = ok && (use == 0 || mbar_wait(&raw_empty[slot], (uint32_t)(use - 1) & 1u, abort_flag));
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        if (lane < BLOCKS) factors[slot * BLOCKS + lane] = which ? fv : fk;
-        __syncwarp();
-        if (lane == 0) mbar_expect_tx(&raw_full[slot], copies * a.box_rows * D);   // also the one arrival
-        __syncwarp();
-        if (leads && now.row >= 0)
-          tma_load_2d(smem_u32(raw_ring) + slot * RAW_BYTES + lane * SCALE_TOKENS * D, &pool_map, &raw_full[slot], 0,
-                      (int)(now.row + (which ? a.v_row0 : a.k_row0)));
-        issued = n + 1;
-      }
+      const uint32_t all_lost = __ballot_sync(0xffffffffu, lost && now.row >= 0);
+      if (lane == 0) to->lost = all_lost;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&known[jj % KNOWN]);
       now = next;
     }
     if (!ok) {
@@ -502,7 +524,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
         atomicCAS(a.error_word, 0, ERR_LOADER);
         // this block's copies in flight land before it leaves (the waits of the others end at the flag)
         volatile int never = 0;
-        for (int n = max(0, issued - RAW_SLOTS); n < issued; ++n) mbar_wait(&raw_full[n % RAW_SLOTS], (uint32_t)(n / RAW_SLOTS) & 1u, &never);
+        for (int n = max(0, k_issued - K_SLOTS); n < k_issued; ++n) mbar_wait(&k_full[n % K_SLOTS], (uint32_t)(n / K_SLOTS) & 1u, &never);
+        for (int n = max(0, c_issued - C_SLOTS); n < c_issued; ++n) mbar_wait(&c_full[n % C_SLOTS], (uint32_t)(n / C_SLOTS) & 1u, &never);
       }
       __syncwarp();
     }
@@ -514,45 +537,45 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
       constexpr uint32_t idesc_o = instr_desc(BM, D, 1);
       const int g = warp - MMA_WARP, lo = (g ? g_lo[1] : g_lo[0]) - kb_lo, hi = (g ? g_hi[1] : g_hi[0]) - kb_lo;   // of the block's key blocks, its
       const uint32_t s_tmem = tmem_base + g * BN, o_tmem = tmem_base + O_COL + g * D;
-      const uint64_t q_desc = smem_desc_sw128(smem_u32(q_smem) + g * Q_BYTES);
+      const uint64_t q_desc = smem_desc_codes(smem_u32(q_smem) + g * 2 * CODES);
       bool ok = true;
-      auto landed = [&](int n) { return mbar_wait(&tile_full[n % SLOTS], (uint32_t)(n / SLOTS) & 1u, abort_flag); };
+      auto keys_landed = [&](int jj) { return mbar_wait(&k_full[jj % K_SLOTS], (uint32_t)(jj / K_SLOTS) & 1u, abort_flag); };
+      auto values_landed = [&](int jj) { return mbar_wait(&v_full[jj % V_SLOTS], (uint32_t)(jj / V_SLOTS) & 1u, abort_flag); };
       // half h of S_g = Q_g K(jj)^T
       auto issue_s = [&](int jj, int h) {
-        const int slot = (2 * jj) % SLOTS, i = jj - lo;
-        ok = ok && (h > 0 || landed(2 * jj)) && (i > 0 ? mbar_wait(&pv_done[g * 2 + h], (uint32_t)(i - 1) & 1u, abort_flag)   // P(i - 1) has been read
-                                                       : h > 0 || mbar_wait(&q_full[g], 0, abort_flag));
+        const int slot = jj % K_SLOTS, i = jj - lo;
+        ok = ok && (h > 0 || keys_landed(jj)) && (i > 0 ? mbar_wait(&pv_done[g * 2 + h], (uint32_t)(i - 1) & 1u, abort_flag)   // P(i - 1) has been read
+                                                        : h > 0 || mbar_wait(&q_full[g], 0, abort_flag));
         if (!ok) return;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint64_t k_desc = smem_desc_sw128(smem_u32(ring) + slot * TILE_BYTES + h * S_PIECE * 128);
+        const uint64_t k_desc = smem_desc_codes(smem_u32(k_ring) + slot * CODES + h * S_PIECE * D);
 #pragma unroll
-        for (int at = 0; at < KA; ++at)
+        for (int part = 0; part < 2; ++part)
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_ss(s_tmem + h * S_PIECE, q_desc + (at * SUB >> 4) + 2 * k, k_desc + (at * SUB >> 4) + 2 * k, idesc_s, (at > 0 || k > 0) ? 1u : 0u);
+          for (int k = 0; k < D / 32; ++k)
+            umma_codes(s_tmem + h * S_PIECE, q_desc + (part * CODES >> 4) + 2 * k, k_desc + 2 * k, idesc_s, (part > 0 || k > 0) ? 1u : 0u);
         umma_commit(&s_full[g * 2 + h]);
-        if (h == 1) umma_commit(&tile_empty[slot]);
+        if (h == 1) umma_commit(&k_empty[slot]);
       };
       // O_g (+)= half h of P_g V(jj): the group's O accumulates in tensor memory over its key blocks
       auto issue_pv = [&](int jj, int h) {
-        const int slot = (2 * jj + 1) % SLOTS, i = jj - lo;
-        ok = ok && (h > 0 || landed(2 * jj + 1)) && mbar_wait(&p_full[g * 2 + h], (uint32_t)i & 1u, abort_flag);
+        const int slot = jj % V_SLOTS, i = jj - lo;
+        ok = ok && (h > 0 || values_landed(jj)) && mbar_wait(&p_full[g * 2 + h], (uint32_t)i & 1u, abort_flag);
         if (!ok) return;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint64_t v_desc = smem_desc_sw128(smem_u32(ring) + slot * TILE_BYTES, SUB);
+        const uint64_t v_desc = smem_desc_sw128(smem_u32(v_ring) + slot * VALUES, SUB);
 #pragma unroll
         for (int kk = 0; kk < S_PIECE / 16; ++kk)
           umma_ts(o_tmem, s_tmem + h * S_PIECE + kk * 8, v_desc + (uint64_t)((h * (S_PIECE / 16) + kk) * 2048 >> 4), idesc_o,
                   (kk > 0 || h > 0 || i > 0) ? 1u : 0u);
         umma_commit(&pv_done[g * 2 + h]);
-        if (h == 1) umma_commit(&tile_empty[slot]);
+        if (h == 1) umma_commit(&v_empty[slot]);
       };
       auto pass = [&](int jj) {       // a key block that only the other tile reads
-#pragma unroll
-        for (int which = 0; which < 2; ++which) {
-          ok = ok && landed(2 * jj + which);
-          if (ok) mbar_arrive(&tile_empty[(2 * jj + which) % SLOTS]);
-        }
+        ok = ok && keys_landed(jj);
+        if (ok) mbar_arrive(&k_empty[jj % K_SLOTS]);
+        ok = ok && values_landed(jj);
+        if (ok) mbar_arrive(&v_empty[jj % V_SLOTS]);
       };
       for (int jj = 0; jj < (lo < hi ? lo : n_kb) && ok; ++jj) pass(jj);
       if (lo < hi) {
@@ -572,32 +595,47 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
     }
   } else {
     // ------------------------------------------------------------------ softmax: group g owns tile g, one thread per row
-    float factor;       // scale * log2(e), times the power of two that was taken out of the row's queries
+    // D / 8 threads to a row of Q, so that the loads are whole lines; where a row lies, and its power of two, the row's own thread knows
     {
-      uint4 raw[D / 8];
+      constexpr int LANES = D / 8, ROWS = 32 / LANES;          // of a load of the warp
+      const long long my_at = row_valid ? ((long long)(q_start + token) * a.q_heads + head) * D : -1;
+      uint4 raw[32 / ROWS];
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) raw[c] = make_uint4(0, 0, 0, 0);
-      if (row_valid) {
-        const uint4* src = reinterpret_cast<const uint4*>(a.q + ((long long)(q_start + token) * a.q_heads + head) * D);
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) raw[c] = __ldg(src + c);
+      for (int i = 0; i < 32 / ROWS; ++i) {
+        const long long at = __shfl_sync(0xffffffffu, my_at, i * ROWS + lane / LANES);
+        raw[i] = make_uint4(0, 0, 0, 0);
+        if (at >= 0) raw[i] = __ldg(reinterpret_cast<const uint4*>(a.q + at) + lane % LANES);
       }
-      const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(raw);
-      float most = 0.0f;
 #pragma unroll
-      for (int i = 0; i < D / 2; ++i) most = fmaxf(most, fmaxf(fabsf(__low2float(pairs[i])), fabsf(__high2float(pairs[i]))));
-      const int e = most > 0.0f ? min(max(exponent_of(most) - 10, -100), 116) : 0;     // the largest entry to [2^10, 2^11)
-      const float down = power_of_two(-e);
-      factor = a.scale_log2 * power_of_two(e);
+      for (int i = 0; i < 32 / ROWS; ++i) {
+        const int in_tile = (warp & 3) * 32 + i * ROWS + lane / LANES, c = lane % LANES;
+        const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(&raw[i]);
+        float most = 0.0f;
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        uint32_t w[4];
+        for (int k = 0; k < 4; ++k) most = fmaxf(most, fmaxf(fabsf(__low2float(pairs[k])), fabsf(__high2float(pairs[k]))));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = pack_half(__low2float(pairs[4 * c + i]) * down, __high2float(pairs[4 * c + i]) * down);
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(q_smem) + g * Q_BYTES + (c >> 3) * SUB + swizzled(r, c & 7)),
-                     "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+        for (int by = 1; by < LANES; by <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, by));
+        const int e = most > 0.0f ? min(max(exponent_of(most) - 7, -100), 119) : 0;     // the largest entry to [2^7, 2^8)
+        const float down = power_of_two(-e);
+        uint32_t part[2][2] = {};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float x = __low2float(pairs[k]), y = __high2float(pairs[k]);
+          x = fabsf(x) <= 3.4e38f ? x * down : __int_as_float(0x7fc00000);       // (codes have no infinity: the row becomes NaN)
+          y = fabsf(y) <= 3.4e38f ? y * down : __int_as_float(0x7fc00000);
+          const uint32_t first = codes2(x, y);
+          const float2 held_by = numbers2(first);
+          part[0][k >> 1] |= first << (k & 1) * 16;
+          part[1][k >> 1] |= codes2(x - held_by.x, y - held_by.y) << (k & 1) * 16;
+        }
+        const uint32_t to = smem_u32(q_smem) + g * 2 * CODES + codes_swizzled(in_tile, c >> 1) + (c & 1) * 8;
+        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to), "r"(part[0][0]), "r"(part[0][1]) : "memory");
+        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + CODES), "r"(part[1][0]), "r"(part[1][1]) : "memory");
+        if (c == 0) q_exponent[g * BM + in_tile] = e;
       }
     }
+    __syncwarp();
+    const float factor = a.scale_log2 * power_of_two(q_exponent[g * BM + r]);       // (this warp wrote it)
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     mbar_arrive(&q_full[g]);
     const int row_pos = row_valid ? pos0 + token : -1;
@@ -607,23 +645,32 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
     const int tile_max_lo = first_visible_key(g ? g_max_pos[1] : g_max_pos[0], window, extras.chunk);   // from here on no row's bound hides a key
     // the product with half h of this group's block k is complete
     auto wait_pv = [&](int k, int h) { return mbar_wait(&pv_done[g * 2 + h], (uint32_t)k & 1u, abort_flag); };
+    uint64_t l2 = 0;         // the row's sum, in two parts
     bool ok = true;
     for (int i = 0; i < my_n && ok; ++i) {
       const int jj = my_lo + i - kb_lo, key0 = (my_lo + i) * BN;
-      ok = mbar_wait(&known[jj % EXPONENTS], (uint32_t)(jj / EXPONENTS) & 1u, abort_flag);
-      const int2 e = exponents[jj % EXPONENTS];
-      const float c = factor * power_of_two(e.x), ev = (float)e.y;
+      ok = mbar_wait(&known[jj % KNOWN], (uint32_t)(jj / KNOWN) & 1u, abort_flag) && !*abort_flag;
+      if (!ok) break;
+      const Scales* of_block = scales + jj % KNOWN;
+      const uint32_t lost = of_block->lost;
       const bool all_visible = key0 + BN - 1 <= tile_min_pos && (!EXTRAS || key0 >= tile_max_lo);
-      uint64_t l2[2] = {0, 0};      // the block's part of the sum, four parts of it
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        ok = ok && mbar_wait(&s_full[g * 2 + h], (uint32_t)i & 1u, abort_flag) && !*abort_flag;
+        ok = ok && mbar_wait(&s_full[g * 2 + h], (uint32_t)i & 1u, abort_flag);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         uint32_t v[S_PIECE];
 #pragma unroll
         for (int k = 0; k < S_PIECE; k += 32) tmem_load32_nowait(s_addr + h * S_PIECE + k, v + k);
         tmem_wait_loads();
+        const float4 key_scale = *reinterpret_cast<const float4*>(of_block->key + h * 4), ev4 = *reinterpret_cast<const float4*>(of_block->value + h * 4);
+        const float c[4] = {factor * key_scale.x, factor * key_scale.y, factor * key_scale.z, factor * key_scale.w};
+        const float ev[4] = {ev4.x, ev4.y, ev4.z, ev4.w};
+        if ((lost >> (h * 4)) & 15u) {
+#pragma unroll
+          for (int k = 0; k < S_PIECE; ++k)
+            if ((lost >> (h * 4 + k / SCALE_TOKENS)) & 1u) v[k] = 0x7fc00000u;
+        }
         if (!all_visible) {
 #pragma unroll
           for (int k = 0; k < S_PIECE; ++k) {
@@ -632,26 +679,26 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
             if (!visible) v[k] = 0xff800000u;   // -inf: probability 0
           }
         }
-        float mx0 = __uint_as_float(v[0]), mx1 = __uint_as_float(v[1]), mx2 = __uint_as_float(v[2]), mx3 = __uint_as_float(v[3]);
+        float m_new = m;
 #pragma unroll
-        for (int k = 4; k < S_PIECE - 4; k += 8) {   // four independent partial maxima
-          mx0 = max3(mx0, __uint_as_float(v[k]), __uint_as_float(v[k + 1]));
-          mx1 = max3(mx1, __uint_as_float(v[k + 2]), __uint_as_float(v[k + 3]));
-          mx2 = max3(mx2, __uint_as_float(v[k + 4]), __uint_as_float(v[k + 5]));
-          mx3 = max3(mx3, __uint_as_float(v[k + 6]), __uint_as_float(v[k + 7]));
+        for (int j = 0; j < S_PIECE / SCALE_TOKENS; ++j) {
+          const uint32_t* w = v + j * SCALE_TOKENS;
+          float even = __uint_as_float(w[0]), odd = __uint_as_float(w[1]);
+#pragma unroll
+          for (int k = 2; k < SCALE_TOKENS - 2; k += 4) {
+            even = max3(even, __uint_as_float(w[k]), __uint_as_float(w[k + 1]));
+            odd = max3(odd, __uint_as_float(w[k + 2]), __uint_as_float(w[k + 3]));
+          }
+          const float most = max3(fmaxf(even, odd), __uint_as_float(w[SCALE_TOKENS - 2]), __uint_as_float(w[SCALE_TOKENS - 1]));
+          m_new = fmaxf(m_new, fmaf(most, c[j], ev[j]));   // c > 0: the maximum commutes with it
         }
-        mx0 = max3(mx0, __uint_as_float(v[S_PIECE - 4]), __uint_as_float(v[S_PIECE - 3]));
-        mx1 = max3(mx1, __uint_as_float(v[S_PIECE - 2]), __uint_as_float(v[S_PIECE - 1]));
-        const float m_new = fmaxf(m, fmaf(fmaxf(max3(mx0, mx1, mx2), mx3), c, ev));   // c > 0: the maximum commutes with it
         // tensor-memory loads and stores are warp-wide: the warp moves its maxima together, as soon as one of
         // its rows has outgrown its own by the step (a row that has not may follow the true maximum just as well)
         const bool move = __any_sync(0xffffffffu, m_new > m + RESCALE_STEP);
         if (move) {
           const float corr = fast_exp2(m - (m_new == -INFINITY ? 0.0f : m_new));   // m = -inf gives 0
           m = m_new;
-          l *= corr;
-          l2[0] = fma2(l2[0], pair(corr, corr), 0);
-          l2[1] = fma2(l2[1], pair(corr, corr), 0);
+          l2 = fma2(l2, pair(corr, corr), 0);
           if (i > 0 || h > 0) {     // O = O * corr in tensor memory, when every product issued so far is complete
             if (!(h > 0 ? wait_pv(i, 0) : wait_pv(i - 1, 1))) {
               ok = false;
@@ -669,16 +716,23 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
             }
           }
         }
-        const float shift = ev - (m == -INFINITY ? 0.0f : m);
-        const uint64_t c2 = pair(c, c), shift2 = pair(shift, shift);
+        const float m_use = m == -INFINITY ? 0.0f : m;
+        const float4 back4 = *reinterpret_cast<const float4*>(of_block->back + h * 4);
+        const float back[4] = {back4.x, back4.y, back4.z, back4.w};
         uint32_t packed[S_PIECE / 2];
 #pragma unroll
-        for (int k = 0; k < S_PIECE; k += 2) {
-          float x0, x1;
-          unpair(fma2(pair(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), c2, shift2), x0, x1);
-          const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
-          l2[k / 2 % 2] = add2(l2[k / 2 % 2], pair(p0, p1));
-          packed[k / 2] = pack_half(p0, p1);
+        for (int j = 0; j < S_PIECE / SCALE_TOKENS; ++j) {
+          const uint64_t c2 = pair(c[j], c[j]), shift2 = pair(ev[j] - m_use, ev[j] - m_use);
+          uint64_t sum2 = 0;
+#pragma unroll
+          for (int k = j * SCALE_TOKENS; k < (j + 1) * SCALE_TOKENS; k += 2) {
+            float x0, x1;
+            unpair(fma2(pair(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), c2, shift2), x0, x1);
+            const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+            sum2 = k == j * SCALE_TOKENS ? pair(p0, p1) : add2(sum2, pair(p0, p1));
+            packed[k / 2] = pack_half(p0, p1);
+          }
+          l2 = fma2(sum2, pair(back[j], back[j]), l2);
         }
         tmem_store32(s_addr + h * S_PIECE, packed);      // over the scores that it was made of
         tmem_wait_stores();
@@ -686,10 +740,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
         mbar_arrive(&p_full[g * 2 + h]);
       }
       if (!ok) break;
-      float part0, part1;
-      unpair(add2(l2[0], l2[1]), part0, part1);
-      l = fmaf(part0 + part1, power_of_two(-e.y), l);
     }
+    float l_odd;
+    unpair(l2, l, l_odd);
+    l += l_odd;
     if (ok && my_n > 0) ok = wait_pv(my_n - 1, 1) && !*abort_flag;
     if (!ok) {
       *abort_flag = 1;
@@ -799,7 +853,7 @@ static EncodeTiledFn encode_tiled_fn() {
 extern "C" int llm_cache8_attention_prompt_rows() { return BLOCK_ROWS; }
 
 // Writes the 128-byte tensor map of a pool of `rows` rows of D codes starting at `base` (16-byte aligned), boxes of `box_rows` whole rows
-// (the largest power of two that divides the page size, up to 128), swizzled as raw_swizzled says.
+// (the largest power of two that divides the page size, up to 128), swizzled as codes_swizzled says.
 extern "C" int llm_cache8_prompt_pool_map(void* map_out, const void* base, long long rows, int box_rows) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) return 1000 + (int)cudaErrorNotSupported;
