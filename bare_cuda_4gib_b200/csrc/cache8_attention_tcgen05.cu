@@ -193,15 +193,19 @@ __device__ __forceinline__ void tmem_load32_nowait(uint32_t taddr, uint32_t* r) 
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t* r) {
+__device__ __forceinline__ void tmem_load16_nowait(uint32_t taddr, uint32_t* r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
-        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
-        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -305,7 +309,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
   uint64_t* s_full = q_full + 2;            // [2][2] MMA (commit) -> softmax, per group and half of 64 keys
   uint64_t* p_full = s_full + 4;            // [2][2] softmax -> MMA: half h of P written
   uint64_t* pv_done = p_full + 4;           // [2][2] MMA (commit) -> softmax, MMA: the product with half h is complete
-  uint64_t* known = pv_done + 4;            // [KNOWN] loader -> softmax: a key block's scales
+  uint64_t* known = pv_done + 4;            // [KNOWN] loader -> MMA (-> softmax, with s_full): a key block's scales
   Scales* scales = reinterpret_cast<Scales*>((reinterpret_cast<uintptr_t>(known + KNOWN) + 15) & ~uintptr_t(15));   // [KNOWN]
   int* q_exponent = reinterpret_cast<int*>(scales + KNOWN);     // [BLOCK_ROWS] of the power of two taken out of a row of Q
   uint32_t* held = reinterpret_cast<uint32_t*>(q_exponent + BLOCK_ROWS);   // [C_SLOTS] bit b: there are values for scale block b
@@ -374,7 +378,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
     for (int s = 0; s < KNOWN; ++s) mbar_init(&known[s], 1);
     for (int b = 0; b < 2; ++b) mbar_init(&q_full[b], GROUP_THREADS);
     for (int b = 0; b < 4; ++b) {
-      mbar_init(&s_full[b], 1);
+      mbar_init(&s_full[b], 2);        // the product, the issuer (which has seen the scales)
       mbar_init(&p_full[b], GROUP_THREADS);
       mbar_init(&pv_done[b], 1);
     }
@@ -556,6 +560,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
             umma_codes(s_tmem + h * S_PIECE, q_desc + (part * CODES >> 4) + 2 * k, k_desc + 2 * k, idesc_s, (part > 0 || k > 0) ? 1u : 0u);
         umma_commit(&s_full[g * 2 + h]);
         if (h == 1) umma_commit(&k_empty[slot]);
+        // the group reads the block's scales behind s_full
+        ok = ok && (h > 0 || mbar_wait(&known[jj % KNOWN], (uint32_t)(jj / KNOWN) & 1u, abort_flag));
+        mbar_arrive(&s_full[g * 2 + h]);
       };
       // O_g (+)= half h of P_g V(jj): the group's O accumulates in tensor memory over its key blocks
       auto issue_pv = [&](int jj, int h) {
@@ -599,16 +606,19 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
     {
       constexpr int LANES = D / 8, ROWS = 32 / LANES;          // of a load of the warp
       const long long my_at = row_valid ? ((long long)(q_start + token) * a.q_heads + head) * D : -1;
-      uint4 raw[32 / ROWS];
+      constexpr int BATCH = 8;                                 // loads on their way at once
+#pragma unroll 1
+      for (int batch = 0; batch < 32 / ROWS / BATCH; ++batch) {
+        uint4 raw[BATCH];
 #pragma unroll
-      for (int i = 0; i < 32 / ROWS; ++i) {
-        const long long at = __shfl_sync(0xffffffffu, my_at, i * ROWS + lane / LANES);
+      for (int i = 0; i < BATCH; ++i) {
+        const long long at = __shfl_sync(0xffffffffu, my_at, (batch * BATCH + i) * ROWS + lane / LANES);
         raw[i] = make_uint4(0, 0, 0, 0);
         if (at >= 0) raw[i] = __ldg(reinterpret_cast<const uint4*>(a.q + at) + lane % LANES);
       }
 #pragma unroll
-      for (int i = 0; i < 32 / ROWS; ++i) {
-        const int in_tile = (warp & 3) * 32 + i * ROWS + lane / LANES, c = lane % LANES;
+      for (int i = 0; i < BATCH; ++i) {
+        const int in_tile = (warp & 3) * 32 + (batch * BATCH + i) * ROWS + lane / LANES, c = lane % LANES;
         const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(&raw[i]);
         float most = 0.0f;
 #pragma unroll
@@ -633,6 +643,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
         asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + CODES), "r"(part[1][0]), "r"(part[1][1]) : "memory");
         if (c == 0) q_exponent[g * BM + in_tile] = e;
       }
+      }
     }
     __syncwarp();
     const float factor = a.scale_log2 * power_of_two(q_exponent[g * BM + r]);       // (this warp wrote it)
@@ -649,23 +660,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
     bool ok = true;
     for (int i = 0; i < my_n && ok; ++i) {
       const int jj = my_lo + i - kb_lo, key0 = (my_lo + i) * BN;
-      ok = mbar_wait(&known[jj % KNOWN], (uint32_t)(jj / KNOWN) & 1u, abort_flag) && !*abort_flag;
-      if (!ok) break;
       const Scales* of_block = scales + jj % KNOWN;
-      const uint32_t lost = of_block->lost;
       const bool all_visible = key0 + BN - 1 <= tile_min_pos && (!EXTRAS || key0 >= tile_max_lo);
-#pragma unroll
+#pragma unroll 1
       for (int h = 0; h < 2; ++h) {
-        ok = ok && mbar_wait(&s_full[g * 2 + h], (uint32_t)i & 1u, abort_flag);
+        ok = ok && mbar_wait(&s_full[g * 2 + h], (uint32_t)i & 1u, abort_flag) && (h > 0 || !*abort_flag);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         uint32_t v[S_PIECE];
 #pragma unroll
         for (int k = 0; k < S_PIECE; k += 32) tmem_load32_nowait(s_addr + h * S_PIECE + k, v + k);
         tmem_wait_loads();
-        const float4 key_scale = *reinterpret_cast<const float4*>(of_block->key + h * 4), ev4 = *reinterpret_cast<const float4*>(of_block->value + h * 4);
-        const float c[4] = {factor * key_scale.x, factor * key_scale.y, factor * key_scale.z, factor * key_scale.w};
-        const float ev[4] = {ev4.x, ev4.y, ev4.z, ev4.w};
+        const uint32_t lost = of_block->lost;
         if ((lost >> (h * 4)) & 15u) {
 #pragma unroll
           for (int k = 0; k < S_PIECE; ++k)
@@ -679,62 +685,63 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
             if (!visible) v[k] = 0xff800000u;   // -inf: probability 0
           }
         }
-        float m_new = m;
+        // The exponentials are taken against the maximum so far while the scores' own is being found, which needs them only when it has
+        // outgrown the other by the step: then they are taken again (twice or so for a row of many blocks).
+        for (bool settled = false;; settled = true) {
+          const float m_use = m == -INFINITY ? 0.0f : m;
+          float m_new = m;
+          uint64_t sum = l2;
+          uint32_t packed[16];
 #pragma unroll
-        for (int j = 0; j < S_PIECE / SCALE_TOKENS; ++j) {
-          const uint32_t* w = v + j * SCALE_TOKENS;
-          float even = __uint_as_float(w[0]), odd = __uint_as_float(w[1]);
+          for (int j = 0; j < S_PIECE / SCALE_TOKENS; ++j) {
+            const uint32_t* w = v + j * SCALE_TOKENS;
+            const float c = factor * of_block->key[h * 4 + j], ev = of_block->value[h * 4 + j], back = of_block->back[h * 4 + j];
+            const uint64_t c2 = pair(c, c), shift2 = pair(ev - m_use, ev - m_use);
+            uint64_t part = 0;
 #pragma unroll
-          for (int k = 2; k < SCALE_TOKENS - 2; k += 4) {
-            even = max3(even, __uint_as_float(w[k]), __uint_as_float(w[k + 1]));
-            odd = max3(odd, __uint_as_float(w[k + 2]), __uint_as_float(w[k + 3]));
+            for (int k = 0; k < SCALE_TOKENS; k += 2) {
+              float x0, x1;
+              unpair(fma2(pair(__uint_as_float(w[k]), __uint_as_float(w[k + 1])), c2, shift2), x0, x1);
+              const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+              part = k == 0 ? pair(p0, p1) : add2(part, pair(p0, p1));
+              packed[(j & 1) * 8 + k / 2] = pack_half(p0, p1);
+            }
+            sum = fma2(part, pair(back, back), sum);
+            float even = __uint_as_float(w[0]), odd = __uint_as_float(w[1]);
+#pragma unroll
+            for (int k = 2; k < SCALE_TOKENS - 2; k += 4) {
+              even = max3(even, __uint_as_float(w[k]), __uint_as_float(w[k + 1]));
+              odd = max3(odd, __uint_as_float(w[k + 2]), __uint_as_float(w[k + 3]));
+            }
+            const float most = max3(fmaxf(even, odd), __uint_as_float(w[SCALE_TOKENS - 2]), __uint_as_float(w[SCALE_TOKENS - 1]));
+            m_new = fmaxf(m_new, fmaf(most, c, ev));   // c > 0: the maximum commutes with it
+            if (j & 1) tmem_store16(s_addr + h * S_PIECE + (j >> 1) * 16, packed);      // over the scores that they were made of
           }
-          const float most = max3(fmaxf(even, odd), __uint_as_float(w[SCALE_TOKENS - 2]), __uint_as_float(w[SCALE_TOKENS - 1]));
-          m_new = fmaxf(m_new, fmaf(most, c[j], ev[j]));   // c > 0: the maximum commutes with it
-        }
-        // tensor-memory loads and stores are warp-wide: the warp moves its maxima together, as soon as one of
-        // its rows has outgrown its own by the step (a row that has not may follow the true maximum just as well)
-        const bool move = __any_sync(0xffffffffu, m_new > m + RESCALE_STEP);
-        if (move) {
+          // tensor-memory loads and stores are warp-wide: the warp moves its maxima together, as soon as one of
+          // its rows has outgrown its own by the step (a row that has not may follow the true maximum just as well)
+          if (settled || !__any_sync(0xffffffffu, m_new > m + RESCALE_STEP)) {
+            l2 = sum;
+            break;
+          }
           const float corr = fast_exp2(m - (m_new == -INFINITY ? 0.0f : m_new));   // m = -inf gives 0
           m = m_new;
           l2 = fma2(l2, pair(corr, corr), 0);
           if (i > 0 || h > 0) {     // O = O * corr in tensor memory, when every product issued so far is complete
-            if (!(h > 0 ? wait_pv(i, 0) : wait_pv(i - 1, 1))) {
-              ok = false;
-              break;
-            }
+            ok = h > 0 ? wait_pv(i, 0) : wait_pv(i - 1, 1);
+            if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-            for (int c0 = 0; c0 < D; c0 += 32) {
-              uint32_t t[32];
-              tmem_load32_nowait(o_addr + c0, t);
+            for (int c0 = 0; c0 < D; c0 += 16) {      // (the scores are still held)
+              uint32_t t[16];
+              tmem_load16_nowait(o_addr + c0, t);
               tmem_wait_loads();
 #pragma unroll
-              for (int k = 0; k < 32; ++k) t[k] = __float_as_uint(__uint_as_float(t[k]) * corr);
-              tmem_store32(o_addr + c0, t);
+              for (int k = 0; k < 16; ++k) t[k] = __float_as_uint(__uint_as_float(t[k]) * corr);
+              tmem_store16(o_addr + c0, t);
             }
           }
         }
-        const float m_use = m == -INFINITY ? 0.0f : m;
-        const float4 back4 = *reinterpret_cast<const float4*>(of_block->back + h * 4);
-        const float back[4] = {back4.x, back4.y, back4.z, back4.w};
-        uint32_t packed[S_PIECE / 2];
-#pragma unroll
-        for (int j = 0; j < S_PIECE / SCALE_TOKENS; ++j) {
-          const uint64_t c2 = pair(c[j], c[j]), shift2 = pair(ev[j] - m_use, ev[j] - m_use);
-          uint64_t sum2 = 0;
-#pragma unroll
-          for (int k = j * SCALE_TOKENS; k < (j + 1) * SCALE_TOKENS; k += 2) {
-            float x0, x1;
-            unpair(fma2(pair(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), c2, shift2), x0, x1);
-            const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
-            sum2 = k == j * SCALE_TOKENS ? pair(p0, p1) : add2(sum2, pair(p0, p1));
-            packed[k / 2] = pack_half(p0, p1);
-          }
-          l2 = fma2(sum2, pair(back[j], back[j]), l2);
-        }
-        tmem_store32(s_addr + h * S_PIECE, packed);      // over the scores that it was made of
+        if (!ok) break;
         tmem_wait_stores();
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         mbar_arrive(&p_full[g * 2 + h]);
