@@ -29,8 +29,8 @@
 // the block get it; values are finite always, and behind the request's last key, or where no page is held, written as zeros.
 // Every mbarrier wait is bounded: on a timeout the thread sets the error word, all roles leave their loops, tensor memory is
 // released and the block returns.
-// One B200: a prompt of 2,048 tokens (32 / 4 heads of 64) 44.2 us, 2,048 tokens behind 2,048 (32 heads of 128) 127 us, 61 tokens behind 3,001
-// (32 / 8 heads of 128) 23.5 us.
+// One B200: a prompt of 2,048 tokens (32 / 4 heads of 64) 43.6 us, 2,048 tokens behind 2,048 (32 heads of 128) 117 us, 61 tokens behind 3,001
+// (32 / 8 heads of 128) 21.2 us.
 
 #include "cache8.cuh"
 
@@ -244,6 +244,27 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+// 2^x for both of a pair without the exponential unit, which takes eight cycles a warp and is what the softmax would wait for: x = n + f with
+// n the nearest whole number (found by adding 1.5 * 2^23), 2^f by a polynomial that was fitted to it on [-1/2, 1/2] for the least
+// relative error (2.6e-6), n added to its exponent.  Below 2^-126: that number.  One pair of four goes this way:
+// the 7b portion below 122 -> 117 us.
+__device__ __forceinline__ void exp2_by_products(uint64_t x, float& p0, float& p1) {
+  float a, b;
+  unpair(x, a, b);
+  a = fmaxf(a, -126.0f), b = fmaxf(b, -126.0f);
+  x = pair(a, b);
+  const uint64_t big = pair(12582912.0f, 12582912.0f), minus_big = pair(-12582912.0f, -12582912.0f), minus_one = pair(-1.0f, -1.0f);
+  const uint64_t r = add2(x, big), f = fma2(add2(r, minus_big), minus_one, x);
+  uint64_t p = fma2(f, pair(0.0095701f, 0.0095701f), pair(0.05591786f, 0.05591786f));
+  p = fma2(p, f, pair(0.24024745f, 0.24024745f));
+  p = fma2(p, f, pair(0.69312181f, 0.69312181f));
+  p = fma2(p, f, pair(0.99999926f, 0.99999926f));
+  float n0, n1;
+  unpair(r, n0, n1);
+  unpair(p, p0, p1);
+  p0 = __int_as_float(__float_as_int(p0) + (__float_as_int(n0) << 23));
+  p1 = __int_as_float(__float_as_int(p1) + (__float_as_int(n1) << 23));
+}
 // Four codes as four halves.
 __device__ __forceinline__ void halves(uint32_t codes, uint32_t& lo, uint32_t& hi) {
   asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
@@ -255,10 +276,17 @@ __device__ __forceinline__ uint32_t codes2(float lo, float hi) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(hi), "f"(lo));
   return d;
 }
-__device__ __forceinline__ float2 numbers2(uint32_t codes) {
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)codes));
-  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+// Two halves less the two numbers of `codes`, as codes.
+__device__ __forceinline__ uint32_t rest_codes2(uint32_t numbers, uint32_t codes) {
+  uint16_t d;
+  asm("{\n\t.reg .b32 h;\n\tcvt.rn.f16x2.e4m3x2 h, %2;\n\tsub.rn.f16x2 h, %1, h;\n\tcvt.rn.satfinite.e4m3x2.f16x2 %0, h;\n\t}"
+      : "=h"(d) : "r"(numbers), "h"((uint16_t)codes));
+  return d;
+}
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
 }
 __device__ __forceinline__ uint32_t peer_smem(uint32_t local, uint32_t rank) {
   uint32_t remote;
@@ -619,24 +647,27 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
 #pragma unroll
       for (int i = 0; i < BATCH; ++i) {
         const int in_tile = (warp & 3) * 32 + (batch * BATCH + i) * ROWS + lane / LANES, c = lane % LANES;
-        const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(&raw[i]);
-        float most = 0.0f;
+        const uint32_t* pairs = reinterpret_cast<const uint32_t*>(&raw[i]);
+        uint32_t most = 0;                     // of the magnitudes' bits, which are in the order of the numbers
 #pragma unroll
-        for (int k = 0; k < 4; ++k) most = fmaxf(most, fmaxf(fabsf(__low2float(pairs[k])), fabsf(__high2float(pairs[k]))));
+        for (int k = 0; k < 4; ++k) most = max_u16x2(most, pairs[k] & 0x7fff7fffu);
 #pragma unroll
-        for (int by = 1; by < LANES; by <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, by));
-        const int e = most > 0.0f ? min(max(exponent_of(most) - 7, -100), 119) : 0;     // the largest entry to [2^7, 2^8)
-        const float down = power_of_two(-e);
-        uint32_t part[2][2] = {};
+        for (int by = 1; by < LANES; by <<= 1) most = max_u16x2(most, __shfl_xor_sync(0xffffffffu, most, by));
+        most = max(most & 0xffffu, most >> 16);
+        const int e = most > 0 ? min(max((int)(most >> 7) - 127 - 7, -100), 119) : 0;     // the largest entry to [2^7, 2^8)
+        const float down = most < 0x7f80u ? power_of_two(-e) : __int_as_float(0x7fc00000);   // (codes have no infinity: such a row becomes NaN)
+        uint32_t part[2][2];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float x = __low2float(pairs[k]), y = __high2float(pairs[k]);
-          x = fabsf(x) <= 3.4e38f ? x * down : __int_as_float(0x7fc00000);       // (codes have no infinity: the row becomes NaN)
-          y = fabsf(y) <= 3.4e38f ? y * down : __int_as_float(0x7fc00000);
-          const uint32_t first = codes2(x, y);
-          const float2 held_by = numbers2(first);
-          part[0][k >> 1] |= first << (k & 1) * 16;
-          part[1][k >> 1] |= codes2(x - held_by.x, y - held_by.y) << (k & 1) * 16;
+        for (int k = 0; k < 4; k += 2) {
+          uint32_t first[2], rest[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const float x = __uint_as_float(pairs[k + u] << 16) * down, y = __uint_as_float(pairs[k + u] & 0xffff0000u) * down;
+            first[u] = codes2(x, y);
+            rest[u] = rest_codes2(pack_half(x, y), first[u]);      // (halves hold both numbers exactly)
+          }
+          part[0][k >> 1] = first[0] | first[1] << 16;
+          part[1][k >> 1] = rest[0] | rest[1] << 16;
         }
         const uint32_t to = smem_u32(q_smem) + g * 2 * CODES + codes_swizzled(in_tile, c >> 1) + (c & 1) * 8;
         asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to), "r"(part[0][0]), "r"(part[0][1]) : "memory");
@@ -700,9 +731,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
             uint64_t part = 0;
 #pragma unroll
             for (int k = 0; k < SCALE_TOKENS; k += 2) {
-              float x0, x1;
-              unpair(fma2(pair(__uint_as_float(w[k]), __uint_as_float(w[k + 1])), c2, shift2), x0, x1);
-              const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+              const uint64_t x = fma2(pair(__uint_as_float(w[k]), __uint_as_float(w[k + 1])), c2, shift2);
+              float p0, p1;
+              if (k % 8 == 4) {
+                exp2_by_products(x, p0, p1);
+              } else {
+                unpair(x, p0, p1);
+                p0 = fast_exp2(p0), p1 = fast_exp2(p1);
+              }
               part = k == 0 ? pair(p0, p1) : add2(part, pair(p0, p1));
               packed[(j & 1) * 8 + k / 2] = pack_half(p0, p1);
             }
