@@ -34,6 +34,7 @@ struct Cache8 {
 struct StepLists {
   const int32_t *seq_q_start, *seq_q_len, *seq_kv_len;   // per request: first row, new tokens, length after the step
   const int32_t *write_seq, *write_block;                // blocks of SCALE_TOKENS positions that the step writes; -1, 0 behind the last
+  const int32_t* order;                                  // the requests, longest first
   const int32_t *tile_seq, *tile_index;                  // tiles of the requests with many rows; -1, 0 behind the last
   int n_seqs, n_writes, n_tiles;
 };

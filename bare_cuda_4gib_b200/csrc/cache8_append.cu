@@ -9,9 +9,9 @@
 //   code = round(x * 2^-e), to nearest, ties to even
 //
 // One thread block per (written block of 16 positions, key/value head): it holds the head's new keys and values of those
-// positions in registers (a thread eight entries of each of one token), so they are read once, and it alone
+// positions in registers (a thread 16 entries of each of one token), so they are read once, and it alone
 // settles the two scales: no atomics, no second pass.  The query heads that share the key/value head go through the same block:
-// their angles are the ones the keys need, computed once into shared memory.
+// their angles are the ones the keys need, computed once into shared memory; their first two rows are asked for together with the keys.
 // Bound by memory for prompts (projections in, queries out), by its trips to memory for decoding steps.  One B200, a call after
 // another from Python: 8 decoding requests (32 / 8 heads of 128) 13.2 us, 64 with three partial results (32 / 4 heads of 64) 13.6, a
 // prompt's 2,048 tokens 23.6 (1.95 TB/s).
@@ -35,47 +35,58 @@ struct AppendArgs {
   int q_heads, write_cache;
 };
 
-// Four neighbouring entries of the sum of the partial results.
-template <typename T>
-__device__ __forceinline__ float4 load4(const T* p, int n_partials, long long stride);
+// Eight neighbouring entries of the sum of the partial results (ONE: there is one).
+template <typename T, bool ONE>
+__device__ __forceinline__ void load8(float (&x)[8], const T* p, int n_partials, long long stride);
 template <>
-__device__ __forceinline__ float4 load4<float>(const float* p, int n_partials, long long stride) {
-  float4 v = *reinterpret_cast<const float4*>(p);
-  for (int i = 1; i < n_partials; ++i) {
-    const float4 w = *reinterpret_cast<const float4*>(p + i * stride);
-    v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
-  }
-  return v;
+__device__ __forceinline__ void load8<float, true>(float (&x)[8], const float* p, int, long long) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
 }
 template <>
-__device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p, int n_partials, long long stride) {
-  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int i = 0; i < n_partials; ++i) {
-    const uint2 raw = *reinterpret_cast<const uint2*>(p + i * stride);
-    const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x));
-    const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
-    v.x += a.x, v.y += a.y, v.z += b.x, v.w += b.y;
+__device__ __forceinline__ void load8<__nv_bfloat16, true>(float (&x)[8], const __nv_bfloat16* p, int, long long) {
+  const uint4 raw = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+}
+template <typename T>
+__device__ __forceinline__ void load8_sum(float (&x)[8], const T* p, int n_partials, long long stride) {
+  load8<T, true>(x, p, 1, 0);
+  for (int i = 1; i < n_partials; ++i) {
+    float y[8];
+    load8<T, true>(y, p + i * stride, 1, 0);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] += y[e];
   }
-  return v;
+}
+template <>
+__device__ __forceinline__ void load8<float, false>(float (&x)[8], const float* p, int n, long long stride) { load8_sum<float>(x, p, n, stride); }
+template <>
+__device__ __forceinline__ void load8<__nv_bfloat16, false>(float (&x)[8], const __nv_bfloat16* p, int n, long long stride) {
+  load8_sum<__nv_bfloat16>(x, p, n, stride);
 }
 
-// (x, y) turned by the angles of `cs` = (cos, sin) pairs.
-__device__ __forceinline__ void turn(float4& lo, float4& hi, const float2* cs) {
-  const float4 a = lo, b = hi;
-  lo = make_float4(a.x * cs[0].x - b.x * cs[0].y, a.y * cs[1].x - b.y * cs[1].y, a.z * cs[2].x - b.z * cs[2].y, a.w * cs[3].x - b.w * cs[3].y);
-  hi = make_float4(b.x * cs[0].x + a.x * cs[0].y, b.y * cs[1].x + a.y * cs[1].y, b.z * cs[2].x + a.z * cs[2].y, b.w * cs[3].x + a.w * cs[3].y);
+// (lo, hi) turned by the angles of `cs` = (cos, sin) pairs.
+__device__ __forceinline__ void turn(float (&lo)[8], float (&hi)[8], const float2* cs) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float a = lo[i], b = hi[i];
+    const float2 t = cs[i];
+    lo[i] = a * t.x - b * t.y;
+    hi[i] = b * t.x + a * t.y;
+  }
 }
 
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
 // The largest finite entry in size; `spoilt` if one is not finite, which then counts as zero.
-__device__ __forceinline__ float largest_of(float4& x, bool& spoilt) {
+__device__ __forceinline__ float largest_of(float (&x)[8], bool& spoilt) {
   float m = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float& e = reinterpret_cast<float*>(&x)[i];
-    if (!finite(e)) spoilt = true, e = 0.0f;
-    m = fmaxf(m, fabsf(e));
+  for (int i = 0; i < 8; ++i) {
+    if (!finite(x[i])) spoilt = true, x[i] = 0.0f;
+    m = fmaxf(m, fabsf(x[i]));
   }
   return m;
 }
@@ -87,21 +98,39 @@ __device__ __forceinline__ int scale_exponent(float a) {
   return min(max(e, SCALE_LEAST), SCALE_MOST);      // zero and numbers below the normal range: the least
 }
 
-__device__ __forceinline__ uint32_t codes4(float4 x, float factor) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x.x * factor, x.y * factor), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x.z * factor, x.w * factor), __NV_SATFINITE, __NV_E4M3);
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
   return lo | (hi << 16);
 }
-__device__ __forceinline__ float4 numbers4(uint32_t codes) {
+__device__ __forceinline__ uint2 codes8(const float (&x)[8], float f) {
+  return make_uint2(codes4(x[0] * f, x[1] * f, x[2] * f, x[3] * f), codes4(x[4] * f, x[5] * f, x[6] * f, x[7] * f));
+}
+// Four codes times `factor`, rounded anew.
+__device__ __forceinline__ uint32_t rescaled(uint32_t codes, float factor) {
   const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes & 0xffff), __NV_E4M3);
   const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes >> 16), __NV_E4M3);
   const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a)), y = __half22float2(*reinterpret_cast<const __half2*>(&b));
-  return make_float4(x.x, x.y, y.x, y.y);
+  return codes4(x.x * factor, x.y * factor, y.x * factor, y.y * factor);
+}
+__device__ __forceinline__ void rescale16(uint8_t* at, float factor) {
+  uint4* p = reinterpret_cast<uint4*>(at);
+  const uint4 old = *p;
+  *p = make_uint4(rescaled(old.x, factor), rescaled(old.y, factor), rescaled(old.z, factor), rescaled(old.w, factor));
+}
+__device__ __forceinline__ uint4 bf16x8(const float (&x)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <int D, typename T>
-__global__ void __launch_bounds__(TOKENS * (D / 8)) cache8_append_kernel(const AppendArgs a) {
-  constexpr int CHUNKS = D / 8, HALF = D / 2, THREADS = TOKENS * CHUNKS;
+template <int D, typename T, bool ONE>
+__global__ void __launch_bounds__(TOKENS * (D / 16), D == 128 ? 6 : 12) cache8_append_kernel(const AppendArgs a) {
+  constexpr int CHUNKS = D / 16, HALF = D / 2, THREADS = TOKENS * CHUNKS, AHEAD = ONE ? 2 : 1;
   pdl_launch_dependents();
   __shared__ float2 angles[TOKENS][HALF];
   __shared__ float largest[2][THREADS / 32];
@@ -134,24 +163,48 @@ __global__ void __launch_bounds__(TOKENS * (D / 8)) cache8_append_kernel(const A
 
   const int group = a.q_heads / a.cache.kv_heads, n_heads = a.q_heads + 2 * a.cache.kv_heads;
   const T* qkv = reinterpret_cast<const T*>(a.qkv) + row0 * n_heads * D;
-  // ---- keys and values: token `group_of` of the new ones; pairs 4 c .. 4 c + 3 of the key, entries 8 c .. 8 c + 7 of the value
+  // ---- keys and values: token `group_of` of the new ones; pairs 8 c .. 8 c + 7 of the key, entries 16 c .. 16 c + 15 of the value
   const bool mine = write && group_of < n_new;
-  float4 k_lo, k_hi, v_lo, v_hi;
-  k_lo = k_hi = v_lo = v_hi = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  bool spoilt = false;
-  float k_most = 0.0f, v_most = 0.0f;
+  float k_lo[8] = {}, k_hi[8] = {}, v_lo[8] = {}, v_hi[8] = {};
   if (mine) {
     const T* k = qkv + ((long long)group_of * n_heads + a.q_heads + kvh) * D;
     const T* v = k + (long long)a.cache.kv_heads * D;
-    k_lo = load4<T>(k + 4 * c, a.n_partials, a.partial_stride);
-    k_hi = load4<T>(k + HALF + 4 * c, a.n_partials, a.partial_stride);
-    v_lo = load4<T>(v + 8 * c, a.n_partials, a.partial_stride);
-    v_hi = load4<T>(v + 8 * c + 4, a.n_partials, a.partial_stride);
-    if (a.inv_freq) turn(k_lo, k_hi, &angles[group_of][4 * c]);
-    k_most = fmaxf(largest_of(k_lo, spoilt), largest_of(k_hi, spoilt));
-    v_most = fmaxf(largest_of(v_lo, spoilt), largest_of(v_hi, spoilt));
+    load8<T, ONE>(k_lo, k + 8 * c, a.n_partials, a.partial_stride);
+    load8<T, ONE>(k_hi, k + HALF + 8 * c, a.n_partials, a.partial_stride);
+    load8<T, ONE>(v_lo, v + 16 * c, a.n_partials, a.partial_stride);
+    load8<T, ONE>(v_hi, v + 16 * c + 8, a.n_partials, a.partial_stride);
   }
+  // the query heads of this key/value head: (head, token) pairs dealt to the groups of threads, tokens fastest, so that
+  // a block with a single new token (a decoding request) turns up to 16 heads at once
+  const int n_units = n_new * group;
+  float q_lo[AHEAD][8], q_hi[AHEAD][8];
+  auto load_queries = [&](int from) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int u = from + i * TOKENS;
+      if (u >= n_units) break;
+      const T* q = qkv + ((long long)(u % n_new) * n_heads + kvh * group + u / n_new) * D;
+      load8<T, ONE>(q_lo[i], q + 8 * c, a.n_partials, a.partial_stride);
+      load8<T, ONE>(q_hi[i], q + HALF + 8 * c, a.n_partials, a.partial_stride);
+    }
+  };
+  auto store_queries = [&](int from) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int u = from + i * TOKENS;
+      if (u >= n_units) break;
+      const int token = u % n_new, head = kvh * group + u / n_new;
+      if (a.inv_freq) turn(q_lo[i], q_hi[i], &angles[token][8 * c]);
+      __nv_bfloat16* out = a.q_out + ((row0 + token) * a.q_heads + head) * D;
+      *reinterpret_cast<uint4*>(out + 8 * c) = bf16x8(q_lo[i]);
+      *reinterpret_cast<uint4*>(out + HALF + 8 * c) = bf16x8(q_hi[i]);
+    }
+  };
+  load_queries(group_of);
   if (write) {        // the same for every thread of the block
+    bool spoilt = false;
+    if (mine && a.inv_freq) turn(k_lo, k_hi, &angles[group_of][8 * c]);
+    float k_most = fmaxf(largest_of(k_lo, spoilt), largest_of(k_hi, spoilt)), v_most = fmaxf(largest_of(v_lo, spoilt), largest_of(v_hi, spoilt));
     k_most = warp_max(k_most), v_most = warp_max(v_most);
     if ((tid & 31) == 0) largest[0][tid >> 5] = k_most, largest[1][tid >> 5] = v_most;
     spoilt = __syncthreads_or(spoilt);
@@ -168,16 +221,8 @@ __global__ void __launch_bounds__(TOKENS * (D / 8)) cache8_append_kernel(const A
       __syncthreads();                                  // every thread has read the scales before one writes them
       ek = max(ek, fk), ev = max(ev, fv);
       if (group_of < held) {                            // the codes of those positions, should a scale have grown
-        if (ek > fk) {
-          uint2* p = reinterpret_cast<uint2*>(k_codes + group_of * D + 8 * c);
-          const uint2 old = *p;
-          *p = make_uint2(codes4(numbers4(old.x), power_of_two(max(fk - ek, -126))), codes4(numbers4(old.y), power_of_two(max(fk - ek, -126))));
-        }
-        if (ev > fv) {
-          uint2* p = reinterpret_cast<uint2*>(v_codes + group_of * D + 8 * c);
-          const uint2 old = *p;
-          *p = make_uint2(codes4(numbers4(old.x), power_of_two(max(fv - ev, -126))), codes4(numbers4(old.y), power_of_two(max(fv - ev, -126))));
-        }
+        if (ek > fk) rescale16(k_codes + group_of * D + 16 * c, power_of_two(max(fk - ek, -126)));
+        if (ev > fv) rescale16(v_codes + group_of * D + 16 * c, power_of_two(max(fv - ev, -126)));
       }
     }
     if (tid == 0) {
@@ -186,29 +231,23 @@ __global__ void __launch_bounds__(TOKENS * (D / 8)) cache8_append_kernel(const A
     }
     if (mine) {
       uint8_t *k = k_codes + (held + group_of) * D, *v = v_codes + (held + group_of) * D;
-      *reinterpret_cast<uint32_t*>(k + 4 * c) = codes4(k_lo, power_of_two(-ek));
-      *reinterpret_cast<uint32_t*>(k + HALF + 4 * c) = codes4(k_hi, power_of_two(-ek));
-      *reinterpret_cast<uint2*>(v + 8 * c) = make_uint2(codes4(v_lo, power_of_two(-ev)), codes4(v_hi, power_of_two(-ev)));
+      *reinterpret_cast<uint2*>(k + 8 * c) = codes8(k_lo, power_of_two(-ek));
+      *reinterpret_cast<uint2*>(k + HALF + 8 * c) = codes8(k_hi, power_of_two(-ek));
+      const uint2 a0 = codes8(v_lo, power_of_two(-ev)), a1 = codes8(v_hi, power_of_two(-ev));
+      *reinterpret_cast<uint4*>(v + 16 * c) = make_uint4(a0.x, a0.y, a1.x, a1.y);
     }
   }
-  // ---- the query heads of this key/value head: (head, token) pairs dealt to the groups of threads, tokens fastest, so that
-  // a block with a single new token (a decoding request) turns up to 16 heads at once
-  for (int u = group_of; u < n_new * group; u += TOKENS) {
-    const int token = u % n_new, head = kvh * group + u / n_new;
-    const T* q = qkv + ((long long)token * n_heads + head) * D;
-    float4 lo4 = load4<T>(q + 4 * c, a.n_partials, a.partial_stride), hi4 = load4<T>(q + HALF + 4 * c, a.n_partials, a.partial_stride);
-    if (a.inv_freq) turn(lo4, hi4, &angles[token][4 * c]);
-    __nv_bfloat16* out = a.q_out + ((row0 + token) * a.q_heads + head) * D;
-    const __nv_bfloat162 l0 = __floats2bfloat162_rn(lo4.x, lo4.y), l1 = __floats2bfloat162_rn(lo4.z, lo4.w);
-    const __nv_bfloat162 h0 = __floats2bfloat162_rn(hi4.x, hi4.y), h1 = __floats2bfloat162_rn(hi4.z, hi4.w);
-    *reinterpret_cast<uint2*>(out + 4 * c) = make_uint2(*reinterpret_cast<const uint32_t*>(&l0), *reinterpret_cast<const uint32_t*>(&l1));
-    *reinterpret_cast<uint2*>(out + HALF + 4 * c) = make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
+  store_queries(group_of);
+  for (int from = group_of + AHEAD * TOKENS; from < n_units; from += AHEAD * TOKENS) {
+    load_queries(from);
+    store_queries(from);
   }
 }
 
 template <int D, typename T>
 int launch(const AppendArgs& a, cudaStream_t stream) {
-  launch_kernel(cache8_append_kernel<D, T>, dim3(a.lists.n_writes, a.cache.kv_heads), TOKENS * (D / 8), 0, stream, a);
+  launch_kernel(a.n_partials == 1 ? cache8_append_kernel<D, T, true> : cache8_append_kernel<D, T, false>, dim3(a.lists.n_writes, a.cache.kv_heads),
+                TOKENS * (D / 16), 0, stream, a);
   return launch_status();
 }
 

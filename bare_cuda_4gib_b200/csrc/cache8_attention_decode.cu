@@ -6,12 +6,13 @@
 //
 // The codes are all that is worth bandwidth (2 head_dim bytes a key against a few hundred bytes for the rest), so the kernel is built
 // around their way into the tensor cores:
-//  * A warp takes 16 keys at a time: one scale block.  Keys and values go from memory straight into registers, 16 bytes a
-//    load, in the layout in which a matrix instruction wants them, so nothing passes through shared memory: the products are
-//    turned around (S^T = K Q^T and O^T = V^T P^T with the codes as the left operand, 16 keys or 16 channels, and up to 8 query
-//    rows as the right one), and the order of the inner dimension is free.  Of a key, thread t of four takes 16 neighbouring channels of every 64
-//    and uses them four at a time; of a value, the eight threads of a column take an eighth of the channels each.
-//    Two such products take 8 rows where the usual way round takes 16 with half of them empty (a group of 4 or 8 heads).
+//  * A warp takes 16 keys at a time: one scale block, whose keys are one piece of memory and whose values are another.  It asks for STAGES such
+//    blocks ahead, as TMA copies into a ring of its own (one warp's ring is nobody else's: no warp waits for another).
+//  * The products are turned around: S^T = K Q^T and O^T = V^T P^T, with the codes as the left operand (16 keys or 16 channels) and up
+//    to 8 query rows as the right one, which takes half the instructions of the usual way round for a group of 4 or 8 heads.  The order of the
+//    inner dimension is free, so a thread takes 16 neighbouring codes a load: of a key, thread t of four takes 16 channels of every 64 and uses them
+//    four at a time; of a value, the eight threads of a column take an eighth of the channels each.  Row g of the left operand is key
+//    g, or g ^ 4 for odd g: then the swizzled loads of keys and values meet every bank once (values of head size 64 twice).
 //  * A code becomes a half by one conversion for two; halves hold e4m3 exactly.  The scale of the keys joins the factor of
 //    the scores.  A weight goes into P together with its block's value scale: P = 2^(s + e_V - m) with m the running maximum of s + e_V,
 //    while the sum takes P 2^-e_V; so a half of P is relative to what the row's keys can add to its output, and O needs no factor.
@@ -26,7 +27,9 @@
 
 #include "cache8.cuh"
 
+#include <cuda.h>
 #include <cuda_fp16.h>
+#include <string.h>
 
 #ifndef HEAD_DIM
 #define HEAD_DIM 64
@@ -43,17 +46,25 @@ constexpr int TILES = D / 16;                  // 16-channel tiles of the output
 constexpr int VW = D / 32;                     // 32-bit words of a value that a thread takes (an eighth of its channels)
 constexpr int FEW_ROWS = 16;
 constexpr float RESCALE_STEP = 8.0f;           // base-2 units
+constexpr int UNIT_BYTES = UNIT * D;           // keys, or values, of one scale block
+constexpr int STAGES = D == 128 ? 3 : 6;       // scale blocks a warp has in flight: 96 KB a thread block, two of which share an SM
+constexpr int RING_BYTES = WARPS * STAGES * 2 * UNIT_BYTES;
+constexpr unsigned long long WAIT_LIMIT_NS = 1000000000ull;
+constexpr int ERR_DECODE = 46, ERR_DECODE_LAYOUT = 47;
 constexpr int STATE = D + 4;                   // floats of a row's state: D sums, the maximum, the sum
 
 struct DecodeArgs {
   const __nv_bfloat16* q;      // [rows][q_heads * D]
   __nv_bfloat16* out;
   Cache8 cache;
+  long long page_rows, k_row0, v_row0;   // the pool seen as rows of D codes
   StepLists lists;
   int q_heads;
   float scale_log2;
   int window;
+  int ordered;                 // longest requests first
   AttentionExtras extras;
+  int* error_word;
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -90,32 +101,85 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-template <int W>
-__device__ __forceinline__ void load_words(uint32_t (&w)[W], const uint8_t* p) {
-  if (W == 4) {
-    const uint4 v = __ldcg(reinterpret_cast<const uint4*>(p));
-    w[0] = v.x, w[1] = v.y, w[W > 2 ? 2 : 0] = v.z, w[W > 3 ? 3 : 0] = v.w;
-  } else {
-    const uint2 v = __ldcg(reinterpret_cast<const uint2*>(p));
-    w[0] = v.x, w[1] = v.y;
+__device__ __forceinline__ unsigned long long global_timer() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
+__device__ __forceinline__ void mbar_init(uint64_t* bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
+}
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return ok != 0;
+}
+// Waits for a copy (about a second; then the error word is set and the warp goes on with what is there, to its barriers and its end).
+__device__ __forceinline__ void mbar_wait(uint64_t* bar, uint32_t parity, int* error_word) {
+  if (mbar_try_wait(bar, parity)) return;
+  const unsigned long long start = global_timer();
+  for (unsigned spins = 0;; ++spins) {
+    if (mbar_try_wait(bar, parity)) return;
+    if ((spins & 63u) == 63u && global_timer() - start > WAIT_LIMIT_NS) {
+      atomicCAS(error_word, 0, ERR_DECODE);
+      return;
+    }
   }
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y) : "memory");
+}
+// Byte offset of chunk `chunk` (16 codes) of row `row` in a block as TMA writes it: 128-byte swizzle for rows of 128 bytes, 64-byte swizzle
+// for rows of 64.
+__device__ __forceinline__ uint32_t codes_swizzled(int row, int chunk) {
+  return (uint32_t)(row * D + ((D == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) << 4));
+}
+// Which of 16 keys is row (or inner index) i of the products.
+__device__ __forceinline__ int key_of(int i) { return (i & 1) ? i ^ 4 : i; }
+
+__device__ __forceinline__ void load_shared4(uint32_t* w, uint32_t at) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void load_shared2(uint32_t* w, uint32_t at) {
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
 }
 
 // NT: groups of 8 query rows.  EXTRAS: whether blocks of positions, a sink or a gate may be asked for.
 template <int NT, bool EXTRAS>
-__global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel(const DecodeArgs a) {
+__global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel(const __grid_constant__ CUtensorMap pool_map, const DecodeArgs a) {
   constexpr int ROWS = 8 * NT;
   const AttentionExtras extras = EXTRAS ? a.extras : AttentionExtras{0, nullptr, nullptr, 0};
-  extern __shared__ __align__(16) float smem[];
+  extern __shared__ __align__(1024) uint8_t ring[];         // [WARPS][STAGES][keys, values][UNIT_BYTES]
   const int n_splits = gridDim.z, split = blockIdx.z, owned_rows = (ROWS + n_splits - 1) / n_splits;
-  float* st = smem;                                       // [WARPS][ROWS][STATE]: this block's warps
-  float* recv = smem + WARPS * ROWS * STATE;              // [n_splits][owned_rows][STATE]: written by the cluster
+  float* st = reinterpret_cast<float*>(ring);             // [WARPS][ROWS][STATE]: this block's warps, when they are done with the ring
+  float* recv = reinterpret_cast<float*>(ring + RING_BYTES);   // [n_splits][owned_rows][STATE]: written by the cluster
+  uint64_t* full = reinterpret_cast<uint64_t*>(recv + n_splits * owned_rows * STATE);   // [WARPS][STAGES]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   pdl_launch_dependents();
-  const int seq = blockIdx.x, kvh = blockIdx.y;
+  if (lane == 0) {
+    for (int i = 0; i < STAGES; ++i) mbar_init(&full[warp * STAGES + i], 1);      // (its own warp's alone)
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&pool_map)) : "memory");
+  }
+  __syncwarp();
+  const int seq = a.ordered ? a.lists.order[blockIdx.x] : blockIdx.x, kvh = blockIdx.y;
   const int group = a.q_heads / a.cache.kv_heads;
   const int q_start = a.lists.seq_q_start[seq], q_len = a.lists.seq_q_len[seq], kv_len = a.lists.seq_kv_len[seq], n_rows = q_len * group;
   if (n_rows <= 0 || n_rows > FEW_ROWS) {                 // nothing, or the prompt kernel's: the same for the whole cluster
+    pdl_wait();
+    return;
+  }
+  if (smem_u32(ring) & 1023) {      // never seen; the swizzled blocks need it
+    if (threadIdx.x == 0) atomicCAS(a.error_word, 0, ERR_DECODE_LAYOUT);
     pdl_wait();
     return;
   }
@@ -128,47 +192,54 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
   const int n_units = first > u_hi ? 0 : (u_hi - first) / stride + 1;         // this warp's: first, first + stride, ...
   const int closed = pos0 / UNIT;                                             // units from here on this step's append may write
 
-  // Where the warp's units lie, looked up 32 at a time: lane i knows unit i of the stretch.
-  long long where = -1;
-  float k_scale = 0.0f;
-  int v_exponent = 0;
+  // Where the warp's units lie, looked up 32 at a time and 32 ahead: lane i knows unit i of the stretch at hand and of the next.
+  struct Places {
+    int row;                 // of the pool, without the cache's own offset, or -1
+    float k_scale;
+    int v_exponent;
+  };
   auto look_up = [&](int from) {
-    const int unit = first + (from + lane) * stride;
-    where = -1;
+    Places p{-1, 0.0f, 0};
     if (from + lane < n_units) {
-      const int page = page_of(a.cache, seq, unit * UNIT);
+      const int unit = first + (from + lane) * stride, page = page_of(a.cache, seq, unit * UNIT);
       if (page >= 0) {
         const int in_page = unit * UNIT % a.cache.page_tokens;
-        where = (long long)page * a.cache.page_stride + ((long long)kvh * a.cache.page_tokens + in_page) * D;
+        p.row = (int)((long long)page * a.page_rows + (long long)kvh * a.cache.page_tokens + in_page);
         const long long at = (long long)page * a.cache.scale_stride + (long long)kvh * (a.cache.page_tokens / UNIT) + in_page / UNIT;
-        k_scale = __ldcg(a.cache.k_scale + at);
-        v_exponent = exponent_of(__ldcg(a.cache.v_scale + at));
+        p.k_scale = __ldcg(a.cache.k_scale + at);
+        p.v_exponent = exponent_of(__ldcg(a.cache.v_scale + at));
+      }
+    }
+    return p;
+  };
+  Places here{-1, 0.0f, 0}, ahead{-1, 0.0f, 0};
+  const uint32_t my_ring = smem_u32(ring) + warp * STAGES * 2 * UNIT_BYTES;
+  uint64_t* my_full = full + warp * STAGES;
+  // asks for unit j, whose row the caller knows, into its stage (a unit without a page: nothing comes, and nothing is waited for long)
+  auto request = [&](int j, int row) {
+    if (lane == 0) {
+      const uint32_t to = my_ring + (j % STAGES) * 2 * UNIT_BYTES;
+      mbar_expect_tx(&my_full[j % STAGES], row >= 0 ? 2 * UNIT_BYTES : 0);
+      if (row >= 0) {
+        tma_load_2d(to, &pool_map, &my_full[j % STAGES], 0, (int)(row + a.k_row0));
+        tma_load_2d(to + UNIT_BYTES, &pool_map, &my_full[j % STAGES], 0, (int)(row + a.v_row0));
       }
     }
   };
-  uint32_t kc[2][KG][4], vc[4][VW];
-  auto load_keys = [&](long long at) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < KG; ++i) load_words<4>(kc[h][i], a.cache.k + at + (g + 8 * h) * D + i * 64 + 16 * t);
-  };
-  auto load_values = [&](long long at) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) load_words<VW>(vc[i], a.cache.v + at + (2 * t + (i & 1) + 8 * (i >> 1)) * D + g * (D / 8));
-  };
   bool waited = false;
-  auto wait_once = [&]() {
-    if (!waited) pdl_wait(), waited = true;
-  };
   if (n_units > 0) {
-    // the scale of an open block is the append's to write: only stretches below it may be looked up ahead of the wait
-    if (first + (min(n_units, 32) - 1) * stride >= closed) wait_once();
-    look_up(0);
-    const long long at = __shfl_sync(0xffffffffu, where, 0);
-    if (at >= 0) load_keys(at), load_values(at);
+    // the append ahead of this kernel may still write the open blocks, codes and scales: only stretches below them may be read ahead
+    // of the wait
+    if (first + (min(n_units, 32) - 1) * stride >= closed) pdl_wait(), waited = true;
+    here = look_up(0);
+#pragma unroll
+    for (int j = 0; j < STAGES; ++j) {
+      const int row = __shfl_sync(0xffffffffu, here.row, j);
+      if (j < n_units) request(j, row);
+    }
   }
-  wait_once();
+  if (!waited) pdl_wait();
+  ahead = look_up(32);
 
   // ---- the query rows as halves, times a power of two that brings a row's largest entry to [2^10, 2^11)
   uint32_t qf[NT][KG * 4][2];
@@ -218,19 +289,30 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
   }
 
   for (int j = 0; j < n_units; ++j) {
-    const long long at = __shfl_sync(0xffffffffu, where, j & 31);
-    const float ks = __shfl_sync(0xffffffffu, k_scale, j & 31);
-    const int ev = __shfl_sync(0xffffffffu, v_exponent, j & 31);
-    if ((j & 31) == 31) look_up(j + 1);
-    const long long next = j + 1 < n_units ? __shfl_sync(0xffffffffu, where, (j + 1) & 31) : -1;
-    if (at < 0) {                   // a page that a window has given back: no row sees it
-      if (next >= 0) load_keys(next), load_values(next);
+    if (j > 0 && (j & 31) == 0) here = ahead, ahead = look_up(j + 32);
+    const int row = __shfl_sync(0xffffffffu, here.row, j & 31);
+    const float ks = __shfl_sync(0xffffffffu, here.k_scale, j & 31);
+    const int ev = __shfl_sync(0xffffffffu, here.v_exponent, j & 31);
+    const int later = j + STAGES;                          // the unit that takes this one's stage
+    const int later_row = (later ^ j) & 32 ? __shfl_sync(0xffffffffu, ahead.row, later & 31) : __shfl_sync(0xffffffffu, here.row, later & 31);
+    mbar_wait(&my_full[j % STAGES], (uint32_t)(j / STAGES) & 1u, a.error_word);
+    if (row < 0) {                  // a page that a window has given back: no row sees it
+      __syncwarp();                 // (every lane has seen this phase)
+      if (later < n_units) request(later, later_row);
       continue;
     }
-    const int key0 = (first + j * stride) * UNIT;
-    float s[NT][4];
+    const uint32_t k_at = my_ring + (j % STAGES) * 2 * UNIT_BYTES, v_at = k_at + UNIT_BYTES;
+    uint32_t kc[2][KG][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < KG; ++i) load_shared4(kc[h][i], k_at + codes_swizzled(key_of(g) + 8 * h, i * 4 + t));
+    const int key0 = (first + j * stride) * UNIT;
+    float s[NT][4], s_odd[NT][4];      // two chains of products instead of one
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[n][e] = s_odd[n][e] = 0.0f;
 #pragma unroll
     for (int i = 0; i < KG; ++i)
 #pragma unroll
@@ -239,9 +321,8 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
         halves(kc[0][i][w], a0, a2);
         halves(kc[1][i][w], a1, a3);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma_f16(s[n], a0, a1, a2, a3, qf[n][i * 4 + w][0], qf[n][i * 4 + w][1]);
+        for (int n = 0; n < NT; ++n) mma_f16(w & 1 ? s_odd[n] : s[n], a0, a1, a2, a3, qf[n][i * 4 + w][0], qf[n][i * 4 + w][1]);
       }
-    if (next >= 0) load_keys(next);
     const bool all_visible = key0 + UNIT - 1 <= pos0 && key0 >= max_lo;
     bool grown = false;
 #pragma unroll
@@ -249,9 +330,9 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int h = e & 1;
-        float v = fmaf(s[n][e], factor[n][h] * ks, (float)ev);
+        float v = fmaf(s[n][e] + s_odd[n][e], factor[n][h] * ks, (float)ev);
         if (!all_visible) {
-          const int key = key0 + g + 8 * (e >> 1);
+          const int key = key0 + key_of(g) + 8 * (e >> 1);
           if (key > row_pos[n][h] || key < row_lo[n][h]) v = -INFINITY;
         }
         s[n][e] = v;
@@ -283,10 +364,17 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
       pf[n][0] = transposed(pack_half(p0, p1));
       pf[n][1] = transposed(pack_half(p2, p3));
     }
+    uint32_t vc[4][VW];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int key = key_of(2 * t + (i & 1)) + 8 * (i >> 1);
+      if (D == 128) load_shared4(vc[i], v_at + codes_swizzled(key, g));
+      else load_shared2(vc[i], v_at + codes_swizzled(key, g >> 1) + (g & 1) * 8);
+    }
     if (key0 + UNIT > kv_len) {     // behind the last key a page may hold anything, and zero times NaN is not zero
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (key0 + 2 * t + (i & 1) + 8 * (i >> 1) >= kv_len)
+        if (key0 + key_of(2 * t + (i & 1)) + 8 * (i >> 1) >= kv_len)
 #pragma unroll
           for (int w = 0; w < VW; ++w) vc[i][w] = 0;
     }
@@ -302,9 +390,13 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
 #pragma unroll
         for (int n = 0; n < NT; ++n) mma_f16(o[n][2 * w + half], a0, a1, a2, a3, pf[n][0], pf[n][1]);
       }
-    if (next >= 0) load_values(next);
+    // behind the products: what every lane read of the stage has arrived in its registers (a load that is merely on its way when the
+    // copy is asked for may be overtaken by it)
+    __syncwarp();
+    if (later < n_units) request(later, later_row);
   }
 
+  __syncthreads();      // every warp is done with its ring
   // ---- the warps' states into shared memory: row C of the tile, channels g * D / 8 + 2 i (+ 1)
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -353,10 +445,12 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
     const int token = r / group, head = kvh * group + r % group;
     const float sink = sink_log2(extras, head);            // joins the row's sum here, once
     float M = sink;
+#pragma unroll 8
     for (int z = 0; z < n_splits; ++z) M = fmaxf(M, recv[((size_t)z * owned_rows + slot) * STATE + D]);
     const float M_use = M == -INFINITY ? 0.0f : M;
     float L = exp2f(sink - M_use);
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
     for (int z = 0; z < n_splits; ++z) {
       const float* from = recv + ((size_t)z * owned_rows + slot) * STATE;
       const float f = from[D] == -INFINITY ? 1.0f : exp2f(from[D] - M_use);
@@ -370,15 +464,16 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
   }
 }
 
+static_assert(WARPS * FEW_ROWS * STATE * 4 <= RING_BYTES, "the warps' states lie over the ring");
 size_t smem_bytes(int rows, int n_splits) {
-  return (size_t)(WARPS * rows + n_splits * ((rows + n_splits - 1) / n_splits)) * STATE * 4;
+  return RING_BYTES + (size_t)n_splits * ((rows + n_splits - 1) / n_splits) * STATE * 4 + WARPS * STAGES * 8;
 }
 
 template <int NT>
-int launch(const DecodeArgs& a, int n_splits, cudaStream_t stream) {
+int launch(const CUtensorMap& map, const DecodeArgs& a, int n_splits, cudaStream_t stream) {
   static bool raised = false;
   if (!raised) {
-    const int most = (int)((WARPS * 8 * NT + 8 * NT + 8) * STATE * 4);
+    const int most = (int)(RING_BYTES + (8 * NT + 8) * STATE * 4 + WARPS * STAGES * 8);
     if (cudaFuncSetAttribute(cache8_decode_kernel<NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess ||
         cudaFuncSetAttribute(cache8_decode_kernel<NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess)
       return launch_status();
@@ -406,18 +501,52 @@ int launch(const DecodeArgs& a, int n_splits, cudaStream_t stream) {
   cfg.attrs = attr;
   cfg.numAttrs = n_attr;
   const AttentionExtras& x = a.extras;
-  cudaLaunchKernelEx(&cfg, x.chunk > 0 || x.sink || x.gate ? cache8_decode_kernel<NT, true> : cache8_decode_kernel<NT, false>, a);
+  cudaLaunchKernelEx(&cfg, x.chunk > 0 || x.sink || x.gate ? cache8_decode_kernel<NT, true> : cache8_decode_kernel<NT, false>, map, a);
   return launch_status();
 }
 
 }  // namespace
 
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiledFn encode_tiled_fn() {
+  static EncodeTiledFn fn = nullptr;
+  if (!fn) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(p);
+  }
+  return fn;
+}
+
+// Writes the 128-byte tensor map of a pool of `rows` rows of D codes starting at `base` (16-byte aligned), boxes of one scale block, swizzled as
+// codes_swizzled says.
+extern "C" int llm_cache8_decode_pool_map(void* map_out, const void* base, long long rows) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return 1000 + (int)cudaErrorNotSupported;
+  if ((reinterpret_cast<uintptr_t>(base) & 15) || rows <= 0 || rows > 0x7fffffffLL) return ERR_BAD_SIZE;
+  cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)D};
+  cuuint32_t box[2] = {(cuuint32_t)D, (cuuint32_t)UNIT};
+  cuuint32_t elem[2] = {1, 1};
+  CUresult r = fn(reinterpret_cast<CUtensorMap*>(map_out), CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : 2000 + (int)r;
+}
+
 // Every request with 1 .. 16 packed rows (q_len * q_heads / kv_heads); the others' blocks return at once.  `rows`: the most packed rows
 // that such a request of the step brings (more than 8 take the kernel for 16).  n_splits (1, 2, 4 or 8) blocks share a
-// request's keys.  chunk, sink, gate and gate_stride: `AttentionExtras`; 0 and null: none.
-extern "C" int llm_cache8_attention_decode(const void* q, void* out, const Cache8* cache, const StepLists* lists, int n_splits, int rows,
-                                           int q_heads, float scale, int window, int chunk, const float* sink, const void* gate,
-                                           long long gate_stride, cudaStream_t stream) {
+// request's keys.  `ordered`: the longest requests' blocks start first
+// (worth its look-up where not all blocks run at once).  `pool_map`: llm_cache8_decode_pool_map over `pool_base`, in which the cache's codes lie.  chunk, sink, gate and gate_stride: `AttentionExtras`; 0 and null: none.
+extern "C" int llm_cache8_attention_decode(const void* q, void* out, const Cache8* cache, const void* pool_map, const void* pool_base,
+                                           const StepLists* lists, int n_splits, int ordered, int rows, int q_heads, float scale, int window, int chunk,
+                                           const float* sink, const void* gate, long long gate_stride, int* error_word,
+                                           cudaStream_t stream) {
   if (lists->n_seqs <= 0) return 0;
   const Cache8& c = *cache;
   if (c.head_dim != D || c.kv_heads <= 0 || q_heads <= 0 || q_heads % c.kv_heads || c.kv_heads > 65535 || c.page_tokens <= 0 ||
@@ -425,7 +554,12 @@ extern "C" int llm_cache8_attention_decode(const void* q, void* out, const Cache
     return ERR_BAD_SIZE;
   const uintptr_t all = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(c.k) |
                         reinterpret_cast<uintptr_t>(c.v) | (uintptr_t)c.page_stride;
-  if (all & 15) return ERR_BAD_ALIGN;
-  DecodeArgs a{reinterpret_cast<const __nv_bfloat16*>(q), reinterpret_cast<__nv_bfloat16*>(out), c, *lists, q_heads, scale * 1.4426950408889634f, window, AttentionExtras{chunk, sink, gate, gate_stride}};
-  return rows <= 8 ? launch<1>(a, n_splits, stream) : launch<2>(a, n_splits, stream);
+  const long long k_off = reinterpret_cast<const char*>(c.k) - reinterpret_cast<const char*>(pool_base);
+  const long long v_off = reinterpret_cast<const char*>(c.v) - reinterpret_cast<const char*>(pool_base);
+  if ((all & 15) || k_off < 0 || v_off < 0 || k_off % D || v_off % D || c.page_stride % D) return ERR_BAD_ALIGN;
+  DecodeArgs a{reinterpret_cast<const __nv_bfloat16*>(q), reinterpret_cast<__nv_bfloat16*>(out), c, c.page_stride / D, k_off / D,
+               v_off / D, *lists, q_heads, scale * 1.4426950408889634f, window, ordered, AttentionExtras{chunk, sink, gate, gate_stride}, error_word};
+  CUtensorMap map;   // the caller's buffer need not be 64-byte aligned
+  memcpy(&map, pool_map, sizeof(CUtensorMap));
+  return rows <= 8 ? launch<1>(map, a, n_splits, stream) : launch<2>(map, a, n_splits, stream);
 }

@@ -65,6 +65,7 @@ constexpr unsigned long long WAIT_LIMIT_NS = 1000000000ull;
 constexpr float RESCALE_STEP = 8.0f;
 constexpr int CHUNKS = D / 16;              // 16-byte chunks of a key's codes; also how many of them a converter thread takes of a tile
 constexpr int BLOCKS = BN / SCALE_TOKENS;   // scale blocks of a key block
+constexpr int MAX_SPLITS = 8;               // blocks that may share a tile's keys
 constexpr int KNOWN = 8;                    // key blocks whose scales are kept (a key tile's slot is free again at most five blocks on)
 constexpr int STATE = D + 4;                // floats of a row's state in a merge: D sums, the maximum, the sum
 constexpr size_t TILES_BYTES = (size_t)(TILES * 2 + K_SLOTS + C_SLOTS) * CODES + (size_t)V_SLOTS * VALUES;
@@ -460,8 +461,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
           if (row >= behind || !((there >> (row / SCALE_TOKENS)) & 1u)) raw[i] = make_uint4(0, 0, 0, 0);
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&c_empty[from_slot]);
       ok = use == 0 || mbar_wait(&v_empty[slot], (uint32_t)(use - 1) & 1u, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -479,7 +478,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(&v_full[slot]);
+      if (lane == 0) {
+        mbar_arrive(&c_empty[from_slot]);      // (here, where every lane's loads of the codes have arrived, not where they were asked for)
+        mbar_arrive(&v_full[slot]);
+      }
     }
     if (!ok && lane == 0) {
       *abort_flag = 1;
@@ -849,18 +851,28 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
       const int tok = packed / group, hd = kvh * group + packed % group;
       const uint32_t local = smem_u32(states + (size_t)row * STATE);
       const float sink = sink_log2(extras, hd);
+      // (all blocks' numbers are asked for at once: a trip to another block's memory takes as long as to L2)
+      float4 ml[MAX_SPLITS], v[MAX_SPLITS];
+#pragma unroll
+      for (int z = 0; z < MAX_SPLITS; ++z)
+        if (z < n_splits) {
+          const uint32_t from = peer_smem(local, z);
+          ml[z] = load_peer4(from + D * 4), v[z] = load_peer4(from + c4 * 16);
+        }
       float M = sink;
-      for (int z = 0; z < n_splits; ++z) M = fmaxf(M, load_peer4(peer_smem(local, z) + D * 4).x);
+#pragma unroll
+      for (int z = 0; z < MAX_SPLITS; ++z)
+        if (z < n_splits) M = fmaxf(M, ml[z].x);
       const float M_use = M == -INFINITY ? 0.0f : M;
       float L = exp2f(sink - M_use);
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      for (int z = 0; z < n_splits; ++z) {
-        const uint32_t from = peer_smem(local, z);
-        const float4 ml = load_peer4(from + D * 4), v = load_peer4(from + c4 * 16);
-        const float f = ml.x == -INFINITY ? 1.0f : exp2f(ml.x - M_use);      // without a maximum: zeros, or NaN to be handed on
-        L += ml.y * f;
-        acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
-      }
+#pragma unroll
+      for (int z = 0; z < MAX_SPLITS; ++z)
+        if (z < n_splits) {
+          const float f = ml[z].x == -INFINITY ? 1.0f : exp2f(ml[z].x - M_use);      // without a maximum: zeros, or NaN to be handed on
+          L += ml[z].y * f;
+          acc.x += v[z].x * f, acc.y += v[z].y * f, acc.z += v[z].z * f, acc.w += v[z].w * f;
+        }
       const float inv = L == 0.0f ? 0.0f : head_gate<__nv_bfloat16>(extras, q_start + tok, hd) / L;
       *reinterpret_cast<uint2*>(a.out + ((long long)(q_start + tok) * a.q_heads + hd) * D + c4 * 4) =
           make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));

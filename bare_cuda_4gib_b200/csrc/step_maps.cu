@@ -34,7 +34,7 @@ struct MapsArgs {
   const int32_t* pages;
   int n_pages;
   int n_rows, page_tokens, group, tile_rows, few_rows, max_blocks, n_writes, n_tiles;
-  int32_t *seq_q_start, *seq_q_len, *seq_kv_len, *positions, *row_seq;
+  int32_t *seq_q_start, *seq_q_len, *seq_kv_len, *order, *positions, *row_seq;
   long long* slots;
   int32_t *block_table, *write_seq, *write_block, *tile_seq, *tile_index;
 };
@@ -66,10 +66,10 @@ __device__ __forceinline__ int whose(const int* starts, int n, int i) {
 }
 
 __global__ void __launch_bounds__(THREADS) step_maps_kernel(const MapsArgs a) {
-  extern __shared__ int sums[];      // [4][n_seqs + 1]: exclusive sums of rows, pages, written blocks, tiles
+  extern __shared__ int sums[];      // [5][n_seqs + 1]: exclusive sums of rows, pages, written blocks, tiles; lengths after the step
   __shared__ int4 warp_total[THREADS / 32];
   const int S = a.n_seqs, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int *rows = sums, *first_page = rows + S + 1, *writes = first_page + S + 1, *tiles = writes + S + 1;
+  int *rows = sums, *first_page = rows + S + 1, *writes = first_page + S + 1, *tiles = writes + S + 1, *kv_len = tiles + S + 1;
   // each thread sums a stretch of requests, the block sums the stretches
   const int per = (S + THREADS - 1) / THREADS, s0 = min(S, tid * per), s1 = min(S, s0 + per);
   int4 mine = make_int4(0, 0, 0, 0);
@@ -88,6 +88,7 @@ __global__ void __launch_bounds__(THREADS) step_maps_kernel(const MapsArgs a) {
   for (int s = s0; s < s1; ++s) {
     rows[s] = at.x, first_page[s] = at.y, writes[s] = at.z, tiles[s] = at.w;
     const int4 c = counts_of(a, s, cached, q);
+    kv_len[s] = cached < 0 ? 0 : cached + q;
     if (blockIdx.x == 0) {
       a.seq_q_start[s] = at.x;
       a.seq_q_len[s] = cached < 0 ? 0 : q;
@@ -123,6 +124,14 @@ __global__ void __launch_bounds__(THREADS) step_maps_kernel(const MapsArgs a) {
     a.tile_seq[i] = s < S ? s : -1;
     a.tile_index[i] = s < S ? i - tiles[s] : 0;
   }
+  // a request's place by length: how many are longer, or as long and come before it (a warp counts for one request)
+  for (int s = first >> 5; s < S; s += step >> 5) {
+    const int mine_len = kv_len[s];
+    int before = 0;
+    for (int o = lane; o < S; o += 32) before += kv_len[o] > mine_len || (kv_len[o] == mine_len && o < s);
+    before = __reduce_add_sync(0xffffffffu, before);
+    if (lane == 0) a.order[before] = s;
+  }
   // the tables: a warp takes a stretch of TABLE_CHUNK entries of a row at a time, all of its loads on their way at once
   const int chunks = (a.max_blocks + TABLE_CHUNK - 1) / TABLE_CHUNK;
   for (int c = first >> 5; c < S * chunks; c += step >> 5) {
@@ -141,27 +150,27 @@ __global__ void __launch_bounds__(THREADS) step_maps_kernel(const MapsArgs a) {
 
 extern "C" int llm_step_maps_max_seqs() { return MAX_SEQS; }
 
-// Every output is a dense device array: per request (seq_q_start, seq_q_len, seq_kv_len), per row of the step (positions, row_seq,
+// Every output is a dense device array: per request (seq_q_start, seq_q_len, seq_kv_len, order), per row of the step (positions, row_seq,
 // slots), [n_seqs][max_blocks] (block_table), and lists of n_writes and n_tiles entries, whose entries behind the last
 // are -1 and 0.  `pages`: the held pages of request 0, then of request 1, ..., ceil(kv_len / page_tokens) each (-1: given back).
 extern "C" int llm_step_maps(const int32_t* cached, const int32_t* q_len, int n_seqs, const int32_t* pages, int n_pages, int n_rows,
                              int page_tokens, int group, int tile_rows, int few_rows, int max_blocks, int n_writes, int n_tiles,
-                             int32_t* seq_q_start, int32_t* seq_q_len, int32_t* seq_kv_len, int32_t* positions, int32_t* row_seq,
+                             int32_t* seq_q_start, int32_t* seq_q_len, int32_t* seq_kv_len, int32_t* order, int32_t* positions, int32_t* row_seq,
                              long long* slots, int32_t* block_table, int32_t* write_seq, int32_t* write_block, int32_t* tile_seq,
                              int32_t* tile_index, cudaStream_t stream) {
   if (n_seqs <= 0) return 0;
   if (n_seqs > MAX_SEQS || page_tokens <= 0 || page_tokens % SCALE_TOKENS || group <= 0 || tile_rows <= 0 || max_blocks <= 0 ||
       n_rows < 0 || n_writes < 0 || n_tiles < 0 || n_pages < 0)
     return ERR_BAD_SIZE;
-  const size_t smem = (size_t)4 * (n_seqs + 1) * 4;
+  const size_t smem = (size_t)5 * (n_seqs + 1) * 4;
   static bool raised = false;
   if (!raised) {
-    if (cudaFuncSetAttribute(step_maps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * (MAX_SEQS + 1) * 4) != cudaSuccess)
+    if (cudaFuncSetAttribute(step_maps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 5 * (MAX_SEQS + 1) * 4) != cudaSuccess)
       return launch_status();
     raised = true;
   }
   MapsArgs a{cached, q_len, n_seqs, pages, n_pages, n_rows, page_tokens, group, tile_rows, few_rows, max_blocks, n_writes, n_tiles,
-             seq_q_start, seq_q_len, seq_kv_len, positions, row_seq, slots, block_table, write_seq, write_block, tile_seq, tile_index};
+             seq_q_start, seq_q_len, seq_kv_len, order, positions, row_seq, slots, block_table, write_seq, write_block, tile_seq, tile_index};
   // four numbers a thread, one block an SM at most
   const long long numbers = (long long)n_rows + n_writes + n_tiles + (long long)n_seqs * max_blocks;
   const long long blocks = (numbers + 4 * THREADS - 1) / (4 * THREADS);

@@ -12,7 +12,7 @@ from typing import Dict, Optional
 
 import torch
 
-from . import build
+from . import build, gemm
 from ..errors import KernelLaunchError
 from .lib import AttentionExtras, CacheView, Partials, _check, _ptr, dtype_code, sm_count, stream_handle
 from .step_maps import SCALE_TOKENS, StepMaps
@@ -55,8 +55,10 @@ def _decode(head_dim: int):
     if l is None:
         l = build.load_library("cache8_attention_decode.cu", (f"-DHEAD_DIM={head_dim}",))
         P, I, L, F = c_void_p, c_int, c_longlong, c_float
-        l.llm_cache8_attention_decode.argtypes = [P, P, P, P, I, I, I, F, I, I, P, P, L, P]
+        l.llm_cache8_attention_decode.argtypes = [P, P, P, P, P, P, I, I, I, I, F, I, I, P, P, L, P, P]
         l.llm_cache8_attention_decode.restype = c_int
+        l.llm_cache8_decode_pool_map.argtypes = [P, P, L]
+        l.llm_cache8_decode_pool_map.restype = c_int
         _decode_libs[head_dim] = l
     return l
 
@@ -123,14 +125,14 @@ def _struct(cache: CacheView) -> int:
     return ctypes.addressof(cache.struct)
 
 
-def _pool_map(cache: CacheView):
-    """The prompt kernel's tensor map over the pool that the cache lies in, kept with the view: (its address, box rows)."""
+def _pool_maps(cache: CacheView):
+    """The kernels' tensor maps over the pool that the cache lies in, kept with the view: (decode map, prompt map, the prompt map's box rows)."""
     if cache.pool_map is None:
-        box_rows = math.gcd(KEY_BLOCK, cache.page_tokens)
-        m = (ctypes.c_ubyte * 128)()
-        _check(_prompt(cache.head_dim).llm_cache8_prompt_pool_map(ctypes.addressof(m), cache.pool_ptr, cache.pool_elems // cache.head_dim, box_rows),
-               "cache8 pool map")
-        cache.pool_map = (m, ctypes.addressof(m), box_rows)
+        box_rows, rows = math.gcd(KEY_BLOCK, cache.page_tokens), cache.pool_elems // cache.head_dim
+        maps = (ctypes.c_ubyte * 128)(), (ctypes.c_ubyte * 128)()
+        _check(_decode(cache.head_dim).llm_cache8_decode_pool_map(ctypes.addressof(maps[0]), cache.pool_ptr, rows), "cache8 pool map")
+        _check(_prompt(cache.head_dim).llm_cache8_prompt_pool_map(ctypes.addressof(maps[1]), cache.pool_ptr, rows, box_rows), "cache8 pool map")
+        cache.pool_map = (maps, ctypes.addressof(maps[0]), ctypes.addressof(maps[1]), box_rows)
     return cache.pool_map[1:]
 
 
@@ -181,9 +183,12 @@ def append(qkv: Partials, q_out: torch.Tensor, cache: CacheView, maps: StepMaps,
 
 def decode_splits(n_seqs: int, kv_heads: int, max_keys: int) -> int:
     """How many blocks of the decode kernel share a request's keys: a power of two up to 8, about two blocks an SM in all, and no more
-    than have a scale block for every warp."""
+    than have a scale block for every warp.  With long caches twice that: requests of different lengths then leave fewer SMs idle at the
+    end than a block's start and merge cost (one / two blocks: 64 requests of 2,000 to 8,191 positions, 8 heads of 128, 128 / 118 us; of 500 to
+    2,047 positions 37 / 44).  The number goes by what the cache holds, not by the lengths at hand, so a captured graph stays valid."""
     splits = 1
-    while splits < 8 and n_seqs * kv_heads * splits * 2 <= 2 * sm_count() and max_keys > splits * DECODE_WARPS * SCALE_TOKENS:
+    while splits < 8 and max_keys > splits * DECODE_WARPS * SCALE_TOKENS and (
+            n_seqs * kv_heads * splits * 2 <= 2 * sm_count() or (max_keys >= splits * 2 * 2560 and n_seqs * kv_heads * splits <= 4 * sm_count())):
         splits *= 2
     return splits
 
@@ -215,16 +220,17 @@ def attention(q: torch.Tensor, out: torch.Tensor, cache: CacheView, maps: StepMa
                                 f"{tile_rows(cache.head_dim)}")
     chunk, sink, gate, gate_stride = extras.arguments(q_heads, q.dtype) if extras is not None else (0, 0, 0, 0)
     stream = stream if stream is not None else stream_handle()
-    group = maps.group
+    group, keys = maps.group, cache.table_stride * cache.page_tokens
+    decode_map, prompt_map, box_rows = _pool_maps(cache)
+    error_word = gemm.error_word(q.device).data_ptr()
     if maps.shortest * group <= FEW_ROWS:
-        rows = min(maps.longest * group, FEW_ROWS)
-        splits = decode_splits(maps.n_seqs, cache.kv_heads, cache.table_stride * cache.page_tokens)
+        splits = decode_splits(maps.n_seqs, cache.kv_heads, keys)
         _check(_decode(cache.head_dim).llm_cache8_attention_decode(
-            q.data_ptr(), out.data_ptr(), at, maps.lists, splits, rows, q_heads, scale, window, chunk, sink, gate, gate_stride, stream), "cache8_attention_decode")
+            q.data_ptr(), out.data_ptr(), at, decode_map, cache.pool_ptr, maps.lists, splits,
+            1 if maps.n_seqs * cache.kv_heads * splits > 2 * sm_count() else 0, min(maps.longest * group, FEW_ROWS), q_heads, scale, window, chunk, sink, gate, gate_stride, error_word, stream),
+            "cache8_attention_decode")
     if maps.longest * group > FEW_ROWS:
-        from . import gemm
-        pool_map, box_rows = _pool_map(cache)
         _check(_prompt(cache.head_dim).llm_cache8_attention_prompt(
-            q.data_ptr(), out.data_ptr(), at, pool_map, cache.pool_ptr, box_rows, maps.lists, prompt_splits(maps.n_tiles, cache.kv_heads, cache.table_stride * cache.page_tokens),
-            q_heads, scale, window, chunk, sink, gate, gate_stride, gemm.error_word(q.device).data_ptr(), stream),
+            q.data_ptr(), out.data_ptr(), at, prompt_map, cache.pool_ptr, box_rows, maps.lists,
+            prompt_splits(maps.n_tiles, cache.kv_heads, keys), q_heads, scale, window, chunk, sink, gate, gate_stride, error_word, stream),
             "cache8_attention_prompt")

@@ -62,7 +62,8 @@ def check_errors() -> None:
                     14: "attention (shared memory not 1024-byte aligned)", 21: "few-token product, producer",
                     22: "few-token product, consumer", 4: "gemm cluster exchange", 31: "decode attention",
                     41: "attention over 8-bit codes, converters", 42: "attention over 8-bit codes, MMA issuer",
-                    43: "attention over 8-bit codes, softmax", 44: "attention over 8-bit codes (shared memory not 1024-byte aligned)", 45: "attention over 8-bit codes, loader"}.get(code, f"code {code}")
+                    43: "attention over 8-bit codes, softmax", 44: "attention over 8-bit codes (shared memory not 1024-byte aligned)", 45: "attention over 8-bit codes, loader", 46: "decode attention over 8-bit codes",
+                    47: "decode attention over 8-bit codes (shared memory not 1024-byte aligned)"}.get(code, f"code {code}")
             raise KernelLaunchError(f"a kernel gave up ({role}): a bounded wait ran out; the result is invalid")
 
 

@@ -24,7 +24,7 @@ def lib():
     if _lib is None:
         l = build.load_library("step_maps.cu")
         P, I = c_void_p, c_int
-        l.llm_step_maps.argtypes = [P, P, I, P, I, I, I, I, I, I, I, I, I] + [P] * 12
+        l.llm_step_maps.argtypes = [P, P, I, P, I, I, I, I, I, I, I, I, I] + [P] * 13
         l.llm_step_maps.restype = c_int
         l.llm_step_maps_max_seqs.restype = c_int
         _lib = l
@@ -34,8 +34,8 @@ def lib():
 class StepLists(ctypes.Structure):
     """struct StepLists of csrc/cache8.cuh."""
 
-    _fields_ = [(name, c_void_p) for name in ("seq_q_start", "seq_q_len", "seq_kv_len", "write_seq", "write_block", "tile_seq",
-                                              "tile_index")] + [(name, c_int) for name in ("n_seqs", "n_writes", "n_tiles")]
+    _fields_ = [(name, c_void_p) for name in ("seq_q_start", "seq_q_len", "seq_kv_len", "write_seq", "write_block", "order",
+                                              "tile_seq", "tile_index")] + [(name, c_int) for name in ("n_seqs", "n_writes", "n_tiles")]
 
 
 class StepMaps:
@@ -47,7 +47,7 @@ class StepMaps:
 
     After `build`, for that step (S requests, T rows):
 
-    * seq_q_start, seq_q_len, seq_kv_len  int32 [S]: first row, new tokens, length after the step
+    * seq_q_start, seq_q_len, seq_kv_len, order  int32 [S]: first row, new tokens, length after the step; the requests, longest first
     * positions, row_seq  int32 [T]; slots int64 [T] = page * page_tokens + place in the page, -1 where no page is held
     * block_table  int32 [S, max_blocks], -1 behind a request's last page
     * write_seq, write_block  int32: the blocks of 16 positions that the step writes (request, number of the block in it)
@@ -71,7 +71,7 @@ class StepMaps:
         self.device = torch.device(device)
         i32 = dict(dtype=torch.int32, device=self.device)
         writes, tiles = self._list_lengths(max_rows, max_seqs)
-        self._seqs = torch.zeros(3, max_seqs, **i32)
+        self._seqs = torch.zeros(4, max_seqs, **i32)
         self._rows = torch.zeros(2, max_rows, **i32)
         self._slots = torch.full((max_rows,), -1, dtype=torch.int64, device=self.device)
         self._table = torch.full((max_seqs, max_blocks), -1, **i32)
@@ -90,14 +90,15 @@ class StepMaps:
     def _arrays(self, seqs: int, rows: int) -> None:
         self.n_seqs, self.n_rows = seqs, rows
         self.n_writes, self.n_tiles = self._list_lengths(rows, seqs)
-        self.seq_q_start, self.seq_q_len, self.seq_kv_len = (t[:seqs] for t in self._seqs)
+        self.seq_q_start, self.seq_q_len, self.seq_kv_len, self.order = (t[:seqs] for t in self._seqs)
         self.positions, self.row_seq = (t[:rows] for t in self._rows)
         self.slots, self.block_table = self._slots[:rows], self._table[:seqs]
         self.write_seq, self.write_block = (t[:self.n_writes] for t in self._writes)
         self.tile_seq, self.tile_index = (t[:self.n_tiles] for t in self._tiles)
         self._shape = (seqs, rows)
         self._lists = StepLists(*(t.data_ptr() for t in (self.seq_q_start, self.seq_q_len, self.seq_kv_len, self.write_seq,
-                                                         self.write_block, self.tile_seq, self.tile_index)),
+                                                         self.write_block, self.order, self.tile_seq,
+                                                         self.tile_index)),
                                 seqs, self.n_writes, self.n_tiles)
         self.lists = ctypes.addressof(self._lists)      # what the launchers of the step's kernels hand on
 
