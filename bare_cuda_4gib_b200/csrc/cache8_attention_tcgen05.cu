@@ -636,7 +636,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
     {
       constexpr int LANES = D / 8, ROWS = 32 / LANES;          // of a load of the warp
       const long long my_at = row_valid ? ((long long)(q_start + token) * a.q_heads + head) * D : -1;
-      constexpr int BATCH = 8;                                 // loads on their way at once
+      constexpr int BATCH = 4;                                 // loads on their way at once
 #pragma unroll 1
       for (int batch = 0; batch < 32 / ROWS / BATCH; ++batch) {
         uint4 raw[BATCH];
@@ -845,37 +845,39 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
       *reinterpret_cast<float4*>(row + D) = make_float4(m, l, 0.0f, 0.0f);
     }
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    for (int i = threadIdx.x; i < BLOCK_ROWS / n_splits * (D / 4); i += NUM_THREADS) {
-      const int row = i / (D / 4) * n_splits + split, c4 = i % (D / 4), packed = row0 + row;
-      if (packed >= n_rows) continue;
-      const int tok = packed / group, hd = kvh * group + packed % group;
-      const uint32_t local = smem_u32(states + (size_t)row * STATE);
+    // A warp takes 128 columns at a time: a row, or two rows at head size 64.  All blocks' numbers are asked for at once (a trip to another
+    // block's memory takes as long as to L2), a row's maxima and sums by one lane a block.
+    constexpr int LANES = D / 4, ROWS = 32 / LANES;
+    const int c4 = lane % LANES, owned = BLOCK_ROWS / n_splits;
+#pragma unroll 1
+    for (int i = warp * ROWS; i < owned; i += NUM_THREADS / 32 * ROWS) {
+      const int row = (i + lane / LANES) * n_splits + split, packed = row0 + row;
+      const bool there = i + lane / LANES < owned && packed < n_rows;
+      const uint32_t local = smem_u32(states + (size_t)(there ? row : 0) * STATE);
+      float4 v[MAX_SPLITS];
+      const float4 ml = c4 < n_splits ? load_peer4(peer_smem(local, c4) + D * 4) : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int z = 0; z < MAX_SPLITS; ++z) v[z] = z < n_splits ? load_peer4(peer_smem(local, z) + c4 * 16) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      const int tok = there ? packed / group : 0, hd = there ? kvh * group + packed % group : 0;
       const float sink = sink_log2(extras, hd);
-      // (all blocks' numbers are asked for at once: a trip to another block's memory takes as long as to L2)
-      float4 ml[MAX_SPLITS], v[MAX_SPLITS];
+      float M = ml.x;
 #pragma unroll
-      for (int z = 0; z < MAX_SPLITS; ++z)
-        if (z < n_splits) {
-          const uint32_t from = peer_smem(local, z);
-          ml[z] = load_peer4(from + D * 4), v[z] = load_peer4(from + c4 * 16);
-        }
-      float M = sink;
-#pragma unroll
-      for (int z = 0; z < MAX_SPLITS; ++z)
-        if (z < n_splits) M = fmaxf(M, ml[z].x);
+      for (int by = 1; by < MAX_SPLITS; by <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, by));      // (of the first eight lanes of a row)
+      M = fmaxf(__shfl_sync(0xffffffffu, M, lane & ~(LANES - 1)), sink);
       const float M_use = M == -INFINITY ? 0.0f : M;
+      const float f_mine = ml.x == -INFINITY ? 1.0f : exp2f(ml.x - M_use);      // without a maximum: zeros, or NaN to be handed on
       float L = exp2f(sink - M_use);
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-      for (int z = 0; z < MAX_SPLITS; ++z)
-        if (z < n_splits) {
-          const float f = ml[z].x == -INFINITY ? 1.0f : exp2f(ml[z].x - M_use);      // without a maximum: zeros, or NaN to be handed on
-          L += ml[z].y * f;
-          acc.x += v[z].x * f, acc.y += v[z].y * f, acc.z += v[z].z * f, acc.w += v[z].w * f;
-        }
+      for (int z = 0; z < MAX_SPLITS; ++z) {
+        const float f = __shfl_sync(0xffffffffu, f_mine, (lane & ~(LANES - 1)) + z), part = __shfl_sync(0xffffffffu, ml.y, (lane & ~(LANES - 1)) + z);
+        L += part * f;
+        acc.x += v[z].x * f, acc.y += v[z].y * f, acc.z += v[z].z * f, acc.w += v[z].w * f;
+      }
       const float inv = L == 0.0f ? 0.0f : head_gate<__nv_bfloat16>(extras, q_start + tok, hd) / L;
-      *reinterpret_cast<uint2*>(a.out + ((long long)(q_start + tok) * a.q_heads + hd) * D + c4 * 4) =
-          make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+      if (there)
+        *reinterpret_cast<uint2*>(a.out + ((long long)(q_start + tok) * a.q_heads + hd) * D + c4 * 4) =
+            make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
     }
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");   // others may still read this block's states
   }
