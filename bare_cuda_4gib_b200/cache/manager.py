@@ -21,6 +21,9 @@ with the same needs, and slots of fixed-size per-request state beside them.
 * A run of a layer may state several demands (a block with two mixers, say): `demands[run]` is one
   `CacheDemand` or a list of them, and caches and states are addressed by (run, index in that list).
 
+* Storage of e4m3 codes (`dtype` torch.float8_e4m3fn): one byte an entry, and beside the pages a float32 scale for every 16
+  positions, key/value head and keys or values each: [page][cache][keys | values][kv head][block of 16 positions].
+
 All bookkeeping is host-side and runs without a GPU (`device="cpu"` or storage disabled).
 """
 
@@ -36,6 +39,10 @@ from ..errors import CacheError, OutOfPages
 from ..kernels.lib import CacheView
 from ..parts.base import KVCacheRequest, StateRequest
 from .page_pool import PagePool
+
+
+CODES = torch.float8_e4m3fn      # the element type that asks for storage of codes with scales
+CODES_HEAD_DIMS, SCALE_TOKENS = (64, 128), 16
 
 
 @dataclass
@@ -60,13 +67,20 @@ class CacheGroup:
         self.key_elems = request.kv_heads * page_tokens * request.head_dim      # values follow the keys
         self.cache_elems = self.key_elems + request.kv_heads * page_tokens * request.value_dim
         self.page_stride = len(members) * self.cache_elems
-        self.storage = None
+        self.codes = dtype == CODES
+        if self.codes and (request.head_dim not in CODES_HEAD_DIMS or request.value_dim != request.head_dim or page_tokens % SCALE_TOKENS):
+            raise CacheError(f"a cache of e4m3 codes takes heads of {CODES_HEAD_DIMS} entries, values of the same size and pages of a multiple "
+                             f"of {SCALE_TOKENS} positions, not heads of {request.head_dim}, values of {request.value_dim} and pages of {page_tokens}")
+        self.cache_scales = 2 * request.kv_heads * (page_tokens // SCALE_TOKENS) if self.codes else 0
+        self.storage = self.scales = None
         if allocate:
-            self.storage = torch.zeros((num_pages, self.page_stride), dtype=dtype, device=device)
+            self.storage = torch.zeros((num_pages, self.page_stride), dtype=torch.uint8 if self.codes else dtype, device=device)
+            if self.codes:
+                self.scales = torch.zeros((num_pages, len(members) * self.cache_scales), dtype=torch.float32, device=device)
 
     @property
     def bytes(self) -> int:
-        return self.num_pages * self.page_stride * torch.empty((), dtype=self.dtype).element_size()
+        return self.num_pages * (self.page_stride * torch.empty((), dtype=self.dtype).element_size() + len(self.members) * self.cache_scales * 4)
 
     def first_needed_block(self, length_before: int) -> int:
         """Blocks below this hold only positions that no query at >= length_before can see."""
@@ -241,6 +255,11 @@ class CacheManager:
         self.lengths[slot] = self.length(slot) + n
 
     # ------------------------------------------------------------------ views for a step
+    def pages_of(self, group: int, slot: int, length: int) -> List[int]:
+        """The pages of the blocks that `length` positions of a slot take, -1 for one that was given back."""
+        g = self.groups[group]
+        return g.tables[slot][: -(-length // g.page_tokens)]
+
     def block_table_rows(self, group: int, slots: Sequence[int], out: np.ndarray) -> None:
         """Fills out[i, :] with slot i's block table of `group` (-1 beyond what is held)."""
         g = self.groups[group]
@@ -261,9 +280,13 @@ class CacheManager:
         esize = g.storage.element_size()
         k_ptr = g.storage.data_ptr() + j * g.cache_elems * esize
         v_ptr = k_ptr + g.key_elems * esize
+        scales = {}
+        if g.codes:
+            k_scale = g.scales.data_ptr() + 4 * j * g.cache_scales
+            scales = dict(k_scale_ptr=k_scale, v_scale_ptr=k_scale + 4 * (g.cache_scales // 2), scale_stride=g.scales.stride(0))
         return CacheView(k_ptr, v_ptr, block_table, g.page_stride, block_table.stride(0), g.page_tokens,
                          g.request.kv_heads, g.request.head_dim, g.dtype, g.storage.data_ptr(), g.storage.numel(),
-                         v_dim=g.request.value_dim)
+                         v_dim=g.request.value_dim, **scales)
 
     # ------------------------------------------------------------------ accounting
     def pages_in_use(self) -> List[int]:

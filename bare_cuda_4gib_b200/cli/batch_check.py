@@ -11,7 +11,7 @@ with `--batch` sequences decoding at once.  Alone and batched steps run differen
 sum in different orders, so a near-tie between the two best logits may break the other way: a
 divergence is scored from one fresh pass over the shared prefix (a third, neutral path) and
 only a gap between the two candidates' logits above `--tol` fails.  Exit status 1 on failure.
-Added here: `--dtype`, `--page-tokens`, `--random NAME` (write random weights of that preset
+Added here: `--dtype`, `--cache-dtype`, `--page-tokens`, `--random NAME` (write random weights of that preset
 into `--model` first) and `--spacing` (the reference's 1,000; smaller for short id files).
 """
 
@@ -35,6 +35,8 @@ def main(argv=None) -> int:
                     help="largest logit gap a divergence may have and still pass (default 0.01)")
     ap.add_argument("--spacing", type=int, default=1000, help="ids between the starts of two prompts' slices")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32", "bf16", "fp32"])
+    ap.add_argument("--cache-dtype", default=None, choices=["bfloat16", "float32", "float8_e4m3"],
+                    help="how keys and values are held (default: as --dtype); float8_e4m3: 8 bits, scales by 16 positions")
     ap.add_argument("--page-tokens", type=int, default=64)
     ap.add_argument("--random", default=None, help="write random weights of this preset into --model first")
     args = ap.parse_args(argv)
@@ -61,7 +63,7 @@ def main(argv=None) -> int:
         write_random_model(args.model, preset_config(args.random), 0)
     try:
         engine = LLMEngine(args.model, max_tokens=longest + args.tokens, max_seqs=args.batch, dtype=args.dtype,
-                           page_tokens=args.page_tokens)
+                           cache_dtype=args.cache_dtype, page_tokens=args.page_tokens)
     except EngineError as e:
         print(f"[llm] {e}", file=sys.stderr)
         return 1

@@ -13,7 +13,7 @@ batch the whole batch's rates; mean, nearest-rank p50 / p90 / p99, min, max.  `-
 breakdown of one request by kernel: launches, device time and its share (that request runs
 without CUDA graphs and with an event pair around every launch, so its own wall time says
 nothing).  Added here: `--random NAME` (write random weights of that preset into --model
-first), `--dtype`, `--page-tokens`.  What it reports is the engine as a user meets it; the
+first), `--dtype`, `--cache-dtype`, `--page-tokens`.  What it reports is the engine as a user meets it; the
 fractions of roofline come from `bench.py` and `llm-kernel-bench`.
 """
 
@@ -116,6 +116,8 @@ def main(argv=None) -> int:
     ap.add_argument("--kernels", action="store_true", help="add a per-kernel breakdown of one profiled request")
     ap.add_argument("--random", default=None, help="write random weights of this preset into --model first")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32", "bf16", "fp32"])
+    ap.add_argument("--cache-dtype", default=None, choices=["bfloat16", "float32", "float8_e4m3"],
+                    help="how keys and values are held (default: as --dtype); float8_e4m3: 8 bits, scales by 16 positions")
     ap.add_argument("--page-tokens", type=int, default=64)
     args = ap.parse_args(argv)
     if (not args.prompt) == (args.prompt_len <= 0) or args.tokens < 2 or args.runs < 1 or args.warmup < 0 or args.batch < 0:
@@ -140,7 +142,7 @@ def main(argv=None) -> int:
 
     def make_engine(graphs=True):
         return LLMEngine(args.model, max_tokens=prompt_tokens + args.tokens, max_seqs=max(args.batch, 1),
-                         dtype=args.dtype, page_tokens=args.page_tokens, use_cuda_graphs=graphs)
+                         dtype=args.dtype, cache_dtype=args.cache_dtype, page_tokens=args.page_tokens, use_cuda_graphs=graphs)
 
     load_start = time.perf_counter()
     engine = make_engine()

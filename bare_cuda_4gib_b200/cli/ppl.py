@@ -8,7 +8,7 @@ windows of `--ctx` tokens, a BOS id (1) and then ctx - 1 text ids; each window i
 request whose logits at every position score the id that follows, so a window yields ctx - 1
 predictions; `--windows N` evaluates only the first N (0: all full windows).  The negative
 log-likelihood is taken in double from the float32 logits (ppl_main.cc:53-58) and the
-perplexity is exp(mean).  Added here: `--dtype`, `--page-tokens`, and `--random NAME`, which
+perplexity is exp(mean).  Added here: `--dtype`, `--cache-dtype`, `--page-tokens`, and `--random NAME`, which
 first writes random weights of that preset into `--model` (the perplexity of random weights is
 about the vocabulary size: a smoke check, not a quality figure).
 """
@@ -46,6 +46,8 @@ def main(argv=None) -> int:
     ap.add_argument("--ctx", type=int, default=512, help="window length in tokens, BOS included (default 512)")
     ap.add_argument("--windows", type=int, default=0, help="evaluate only the first N windows (default: all full windows)")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32", "bf16", "fp32"])
+    ap.add_argument("--cache-dtype", default=None, choices=["bfloat16", "float32", "float8_e4m3"],
+                    help="how keys and values are held (default: as --dtype); float8_e4m3: 8 bits, scales by 16 positions")
     ap.add_argument("--page-tokens", type=int, default=64)
     ap.add_argument("--random", default=None, help="write random weights of this preset into --model first")
     args = ap.parse_args(argv)
@@ -69,7 +71,8 @@ def main(argv=None) -> int:
         from ..weights.random_init import write_random_model
         write_random_model(args.model, preset_config(args.random), 0)
     try:
-        engine = LLMEngine(args.model, max_tokens=args.ctx, max_seqs=1, dtype=args.dtype, page_tokens=args.page_tokens)
+        engine = LLMEngine(args.model, max_tokens=args.ctx, max_seqs=1, dtype=args.dtype, cache_dtype=args.cache_dtype,
+                           page_tokens=args.page_tokens)
     except EngineError as e:
         print(f"[llm] {e}", file=sys.stderr)
         return 1

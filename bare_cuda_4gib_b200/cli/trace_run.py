@@ -28,6 +28,8 @@ def main(argv=None) -> int:
                                  formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument("--model", required=True, help="folder with config.json and model.safetensors")
     ap.add_argument("--dtype", required=True, choices=["bfloat16", "float32"])
+    ap.add_argument("--cache-dtype", default=None, choices=["bfloat16", "float32", "float8_e4m3"],
+                    help="how keys and values are held (default: as --dtype)")
     ap.add_argument("--out", required=True, help="folder the logits files are written to")
     ap.add_argument("--max-tokens", type=int, required=True,
                     help="most tokens that live requests hold at any time (rounded up per request to a page)")
@@ -38,7 +40,7 @@ def main(argv=None) -> int:
     import torch
 
     from ..cache.manager import CacheManager
-    from ..engine.model import load_model
+    from ..engine.model import cache_type, load_model
     from ..engine.step import StepEntry, StepRunner
 
     if not torch.cuda.is_available():
@@ -49,8 +51,9 @@ def main(argv=None) -> int:
     page = args.page_tokens
     capacity = -(-args.max_tokens // page) * page
     model, _config = load_model(args.model, args.dtype, "cuda")
+    kept = cache_type(args.cache_dtype, model)
     cache = CacheManager(model.cache_demands(), page_tokens=page, max_seqs=args.max_live,
-                         max_tokens=capacity, num_pages=capacity // page, dtype=model.dtype, device="cuda")
+                         max_tokens=capacity, num_pages=capacity // page, dtype=kept, device="cuda")
     runner = StepRunner(model, cache, max_step_tokens=capacity, max_batch_seqs=args.max_live)
     slots = {}
     for line in sys.stdin:

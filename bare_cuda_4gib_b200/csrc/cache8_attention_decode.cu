@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
         p.row = (int)((long long)page * a.page_rows + (long long)kvh * a.cache.page_tokens + in_page);
         const long long at = (long long)page * a.cache.scale_stride + (long long)kvh * (a.cache.page_tokens / UNIT) + in_page / UNIT;
         p.k_scale = __ldcg(a.cache.k_scale + at);
-        p.v_exponent = exponent_of(__ldcg(a.cache.v_scale + at));
+        p.v_exponent = max(exponent_of(__ldcg(a.cache.v_scale + at)), SCALE_LEAST);      // (a scale that nothing has written is zero)
       }
     }
     return p;
@@ -526,9 +526,9 @@ static EncodeTiledFn encode_tiled_fn() {
 // Writes the 128-byte tensor map of a pool of `rows` rows of D codes starting at `base` (16-byte aligned), boxes of one scale block, swizzled as
 // codes_swizzled says.
 extern "C" int llm_cache8_decode_pool_map(void* map_out, const void* base, long long rows) {
+  if ((reinterpret_cast<uintptr_t>(base) & 15) || rows <= 0 || rows > 0x7fffffffLL) return ERR_BAD_SIZE;
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) return 1000 + (int)cudaErrorNotSupported;
-  if ((reinterpret_cast<uintptr_t>(base) & 15) || rows <= 0 || rows > 0x7fffffffLL) return ERR_BAD_SIZE;
   cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)D};
   cuuint32_t box[2] = {(cuuint32_t)D, (cuuint32_t)UNIT};

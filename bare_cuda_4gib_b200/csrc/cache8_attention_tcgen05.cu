@@ -541,8 +541,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
       const bool lost = isnan(now.k_scale);
       Scales* to = scales + jj % KNOWN;
       if (lane < BLOCKS) {
-        const int ev = now.row >= 0 ? exponent_of(now.v_scale) : 0;
-        to->key[lane] = now.row >= 0 && !lost ? now.k_scale : 1.0f;
+        const int ev = now.row >= 0 ? max(exponent_of(now.v_scale), SCALE_LEAST) : 0;      // (a scale that nothing has written is zero)
+        to->key[lane] = now.row >= 0 && !lost ? fmaxf(now.k_scale, power_of_two(SCALE_LEAST)) : 1.0f;
         to->value[lane] = (float)ev;
         to->back[lane] = power_of_two(-ev);
       }
@@ -912,9 +912,9 @@ extern "C" int llm_cache8_attention_prompt_rows() { return BLOCK_ROWS; }
 // Writes the 128-byte tensor map of a pool of `rows` rows of D codes starting at `base` (16-byte aligned), boxes of `box_rows` whole rows
 // (the largest power of two that divides the page size, up to 128), swizzled as codes_swizzled says.
 extern "C" int llm_cache8_prompt_pool_map(void* map_out, const void* base, long long rows, int box_rows) {
+  if ((reinterpret_cast<uintptr_t>(base) & 15) || rows <= 0 || rows > 0x7fffffffLL || box_rows < SCALE_TOKENS || BN % box_rows) return ERR_BAD_SIZE;
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) return 1000 + (int)cudaErrorNotSupported;
-  if ((reinterpret_cast<uintptr_t>(base) & 15) || rows <= 0 || rows > 0x7fffffffLL || box_rows < SCALE_TOKENS || BN % box_rows) return ERR_BAD_SIZE;
   cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)D};
   cuuint32_t box[2] = {(cuuint32_t)D, (cuuint32_t)box_rows};

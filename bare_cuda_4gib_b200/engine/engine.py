@@ -25,7 +25,7 @@ from ..cache.manager import CacheManager
 from ..errors import EngineError
 from ..sampling.params import SamplingParams
 from ..sampling.sampler import DeviceSampler
-from .model import load_model, random_model
+from .model import cache_type, load_model, random_model
 from .scheduler import (FINISH_CANCELLED, FINISH_ERROR, Request, Scheduler, SchedulerStats, TokenEvent)
 from .step import StepEntry, StepRunner
 
@@ -76,8 +76,12 @@ class LLMEngine:
     def __init__(self, model_path, max_tokens: int = 1024, max_seqs: int = 8, kv_pages: int = 0,
                  dtype: str = "bfloat16", page_tokens: int = 64, max_step_tokens: Optional[int] = None,
                  policy: str = "reserve", device: str = "cuda", use_fast_gemm: bool = True,
-                 use_fast_attention: bool = True, use_cuda_graphs: bool = True, random=None):
-        """`random=(config, seed)`: no folder is read; the model of that typed configuration gets
+                 use_fast_attention: bool = True, use_cuda_graphs: bool = True, random=None, cache_dtype: Optional[str] = None):
+        """`cache_dtype` "float8_e4m3": keys and values are held in 8 bits, e4m3 codes with a scale for every 16 positions and head
+        (bfloat16 runs of models whose every mixer with a cache is "attention", heads of 64 or 128, pages of a multiple of 16
+        positions); None or `dtype`'s name: in the step's type.
+
+        `random=(config, seed)`: no folder is read; the model of that typed configuration gets
         seeded random weights generated on the device (the values `write_random_model` would have
         written with that seed from this device), and `model_path` may be None."""
         if not torch.cuda.is_available():
@@ -91,12 +95,13 @@ class LLMEngine:
             raise EngineError(f"max_tokens {max_tokens} exceeds the model's {self.model.spec.max_positions} positions")
         if max_seqs <= 0:
             raise EngineError("max_seqs must be positive")
+        kept = cache_type(cache_dtype, self.model)
         demands = self.model.cache_demands()
         blocks = -(-max_tokens // page_tokens)
         wanted = max_seqs * blocks
         if kv_pages <= 0:
             probe = CacheManager(demands, page_tokens=page_tokens, max_seqs=1, max_tokens=page_tokens,
-                                 num_pages=1, dtype=self.model.dtype, allocate=False)
+                                 num_pages=1, dtype=kept, allocate=False)
             page_bytes = max(sum(g.bytes for g in probe.groups), 1)
             free, _total = torch.cuda.mem_get_info()
             kv_pages = int(min(wanted, max(0, free - VRAM_HEADROOM) // page_bytes))
@@ -104,7 +109,7 @@ class LLMEngine:
                 raise EngineError(f"too little GPU memory for one sequence of {max_tokens} tokens "
                                   f"({kv_pages} pages fit, {blocks} are needed)")
         self.cache = CacheManager(demands, page_tokens=page_tokens, max_seqs=max_seqs, max_tokens=max_tokens,
-                                  num_pages=kv_pages, dtype=self.model.dtype, device=device)
+                                  num_pages=kv_pages, dtype=kept, device=device)
         self.max_step_tokens = int(max_step_tokens or min(max_tokens, 2048) + max_seqs)
         self.runner = StepRunner(self.model, self.cache, max_step_tokens=self.max_step_tokens,
                                  max_batch_seqs=max_seqs, use_fast_gemm=use_fast_gemm,

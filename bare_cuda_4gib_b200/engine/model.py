@@ -25,6 +25,9 @@ from ..weights.loader import load_weights, random_weights
 RUN_DTYPES = {"float32": torch.float32, "fp32": torch.float32, "bfloat16": torch.bfloat16, "bf16": torch.bfloat16}
 
 
+CACHE_DTYPES = {"float8_e4m3": torch.float8_e4m3fn, "e4m3": torch.float8_e4m3fn}
+
+
 def run_dtype(name) -> torch.dtype:
     if isinstance(name, torch.dtype):
         if name not in (torch.float32, torch.bfloat16):
@@ -33,6 +36,24 @@ def run_dtype(name) -> torch.dtype:
     if name not in RUN_DTYPES:
         raise ConfigError(f"dtype '{name}' is not supported (float32 or bfloat16)")
     return RUN_DTYPES[name]
+
+
+def cache_type(name, model: "Model") -> torch.dtype:
+    """The element type that a model's caches are held in: None or the run's own type, or "float8_e4m3" (e4m3 codes with scales)
+    where every mixer that keeps a cache can read them."""
+    if name is None or CACHE_DTYPES.get(name, RUN_DTYPES.get(name, name)) == model.dtype:
+        return model.dtype
+    if CACHE_DTYPES.get(name, name) != torch.float8_e4m3fn:
+        raise ConfigError(f"cache dtype '{name}' is not supported (the run's own type or float8_e4m3)")
+    if model.dtype != torch.bfloat16:
+        raise ConfigError("a cache of e4m3 codes goes with bfloat16 runs; a float32 run keeps its cache in 32 bits")
+    for block in model.blocks:
+        # every cache that the block asks for has to belong to one of its own parts that reads codes
+        able = [part for part in block.parts() if getattr(part, "takes_codes", False)]
+        if sum(kv is not None for kv, _state in block.cache_demands()) > len(able):
+            kinds = [part.spec.kind for part in block.parts() if hasattr(part, "cache_request") and part not in able]
+            raise ConfigError(f"a cache of e4m3 codes is not supported by the mixer {' and '.join(repr(k) for k in kinds)}")
+    return torch.float8_e4m3fn
 
 
 def _walk(part) -> List[Part]:

@@ -10,6 +10,9 @@ Per step the host builds one block of int32 metadata in pinned memory - token id
 the batch sequence of every row, wanted rows, per-sequence lengths, and every cache group's
 block-table rows - and sends it with one asynchronous copy.  Kernels read all variable data
 from that block, so a step of the same padded shape can be replayed as a CUDA graph.
+
+With caches of e4m3 codes the host sends less: lengths, the requests' pages as they are, token ids and wanted rows.  Positions,
+the rows' requests, the padded block tables and the kernels' work lists are then built on the device (`kernels.step_maps`).
 """
 
 from __future__ import annotations
@@ -107,6 +110,7 @@ class StepContext:
         self.host_kv_len: List[int] = []
         self.max_q_len = 0
         self.max_kv_len = 0
+        self.codes = False         # the caches are held as e4m3 codes
         self.extras: Dict[object, object] = {}
         self.residual = None       # the float32 residual stream while a layer runs
         self.following_norm = None # the norm part that reads the stream after the part that runs now
@@ -188,8 +192,71 @@ class StepRunner:
                 views.append(cache.cache_view(i, self._tables[where[0]][1], j) if where is not None else None)
                 states.append(cache.state_of(i, j))
             c.calls.append(CallContext(i, views, call.cache_from is None, states))
+        c.codes = any(g.codes for g in cache.groups)
+        if c.codes:
+            self._prepare_codes()
         for part in model.all_parts():
             getattr(part, "reserve", lambda ctx: None)(c)
+
+    def _prepare_codes(self) -> None:
+        """The step's maps, one per cache group, and the places in the metadata block of what they are built from."""
+        from ..kernels import cache8
+        from ..kernels.step_maps import StepMaps
+        T, S, P, G = self._sizes
+        heads: List[Optional[int]] = [None] * G
+        for i, call in enumerate(self.model.order):
+            parts = [p for p in self.model.blocks[call.layer].parts() if hasattr(p, "cache_request")]
+            for j, part in enumerate(parts):
+                where = self.cache.group_of(i, j)
+                if where is None:
+                    continue
+                if not getattr(part, "takes_codes", False):
+                    raise EngineError(f"the cache of run {i} cannot be held as e4m3 codes: its mixer '{part.spec.kind}' reads it in 16 or 32 bits")
+                group = part.heads // part.kv_heads
+                if heads[where[0]] not in (None, group):
+                    raise EngineError("layers that share a cache group must share its query heads' grouping for a cache of e4m3 codes")
+                heads[where[0]] = group
+        self._maps = [StepMaps(T, S, P, self.cache.page_tokens, group=heads[gi] or 1, tile_rows=cache8.tile_rows(g.request.head_dim),
+                               few_rows=cache8.FEW_ROWS, device=self.device) for gi, g in enumerate(self.cache.groups)]
+        for g in self.cache.groups:
+            cache8.prepare(g.request.head_dim)
+        for i, call in enumerate(self.model.order):
+            for j in range(len(self.cache.demands[i])):
+                where = self.cache.group_of(i, j)
+                if where is not None:
+                    view = self.cache.cache_view(i, self._maps[where[0]].table, j)
+                    view.maps = self._maps[where[0]]
+                    self.ctx.calls[i].caches[j] = view
+
+    def _send_codes(self, entries, rows: int, seqs: int) -> int:
+        """Puts token ids and wanted rows (which graphs of this shape hold by their place) and then what the maps are built from behind the
+        per-sequence slots; returns the words used."""
+        n, lengths = len(entries), [self.cache.lengths[e.slot] for e in entries]
+        h, d, c = self._host_np, self._dev, self.ctx
+        at = self._seq_slot[0].size
+        ids, wanted = self._rows_h[:rows].copy(), self._rows_h[3 * rows: 4 * rows].copy()      # (put together further on in the same block)
+        h[at: at + rows], h[at + rows: at + 2 * rows] = ids, wanted
+        c.token_ids, c.want_rows = d[at: at + rows], d[at + rows: at + 2 * rows]
+        at += 2 * rows
+        self._codes_at = [at, at + seqs, []]
+        h[at: at + n], h[at + n: at + seqs] = lengths, -1
+        at += seqs
+        h[at: at + n], h[at + n: at + seqs] = [len(e.tokens) for e in entries], 1
+        at += seqs
+        for gi in range(len(self.cache.groups)):
+            pages = [p for e, length in zip(entries, lengths) for p in self.cache.pages_of(gi, e.slot, length + len(e.tokens))]
+            h[at: at + len(pages)] = pages
+            self._codes_at[2].append((at, len(pages)))
+            at += len(pages)
+        return at
+
+    def _build_maps(self, rows: int, seqs: int, longest: int, shortest: int) -> None:
+        d, (cached, q_len, pages) = self._dev, self._codes_at
+        for maps, (at, n) in zip(self._maps, pages):
+            maps.build(d[cached: cached + seqs], d[q_len: q_len + seqs], d[at: at + n], rows, longest, shortest)
+        c, maps = self.ctx, self._maps[0]
+        c.positions, c.row_seq = maps.positions, maps.row_seq
+        c.seq_q_start, c.seq_q_len, c.seq_kv_len = maps.seq_q_start, maps.seq_q_len, maps.seq_kv_len
 
     def _row_views(self, rows: int):
         """token ids, positions, batch sequence of a row, wanted rows: four arrays of `rows` entries at
@@ -198,7 +265,9 @@ class StepRunner:
         return [(h[i * rows: (i + 1) * rows], d[i * rows: (i + 1) * rows]) for i in range(4)]
 
     def metadata_bytes(self, n_tokens: int, n_seqs: int) -> int:
-        """Bytes of step metadata sent to the device for a batch of this shape."""
+        """Bytes of step metadata sent to the device for a batch of this shape (with caches of codes: at most)."""
+        if self.ctx.codes:
+            return (self._sizes[1] + 2 * n_tokens + (2 + len(self.cache.groups) * self.cache.max_blocks) * n_seqs) * 4
         return (self._rows_offset + 4 * n_tokens) * 4
 
     # ------------------------------------------------------------------
@@ -299,7 +368,8 @@ class StepRunner:
                 c.host_kv_len.append(length + n)
                 row += n
         slots = [e.slot for e in entries]
-        for gi in range(len(self.cache.groups)):
+        groups = [] if c.codes else range(len(self.cache.groups))
+        for gi in groups:
             self.cache.block_table_rows(gi, slots, self._tables[gi][0])
         # idle rows: token 0 at position 0 of a sequence that holds no page and whose state row is
         # the spare one that no request owns
@@ -308,11 +378,11 @@ class StepRunner:
             tok_h[row], pos_h[row], rs_h[row], want_h[w] = 0, 0, s, row
             self._seq_slot[0][s], self._seq_q_start[0][s] = self.cache.idle_slot, row
             self._seq_q_len[0][s], self._seq_kv_len[0][s] = 0, 0
-            for gi in range(len(self.cache.groups)):
+            for gi in groups:
                 self._tables[gi][0][s].fill(-1)
             row += 1
             w += 1
-        used = self._rows_offset + 4 * rows
+        used = self._send_codes(entries, rows, seqs) if c.codes else self._rows_offset + 4 * rows
         turn, self._turn = self._turn, (self._turn + 1) % len(self._send)
         if self._sent[turn] is not None:
             self._sent[turn].synchronize()       # the copy that last read this buffer has run (almost always long ago)
@@ -321,10 +391,12 @@ class StepRunner:
         if self._sent[turn] is None:
             self._sent[turn] = torch.cuda.Event()
         self._sent[turn].record()
+        if c.codes:
+            self._build_maps(rows, seqs, max(c.host_q_len), min(c.host_q_len))
         if device_fed:
             if any(len(e.tokens) != 1 for e in entries):
                 raise EngineError("step: device-fed token ids need one token per request")
-            tok_d[:n_seqs].copy_(self.argmax[:n_seqs], non_blocking=True)
+            c.token_ids[:n_seqs].copy_(self.argmax[:n_seqs], non_blocking=True)
         c.n_tokens, c.n_seqs, c.n_want, c.pad_seqs = rows, seqs, wanted, pad
         c.max_q_len, c.max_kv_len = max(c.host_q_len), max(c.host_kv_len)
         c.host_slots = slots

@@ -49,6 +49,8 @@ class Attention(Part):
     def adjacent_weights(self):
         return [("q", "k", "v")]
 
+    takes_codes = True      # whether this mixer's cache may be held as e4m3 codes (kernels.cache8); its `heads` and `kv_heads` then go into the step's maps
+
     def cache_request(self):
         return KVCacheRequest(self.kv_heads, self.head_dim, self.window)
 
@@ -69,7 +71,7 @@ class Attention(Part):
             self.fast = None
 
     def plan_step(self, ctx) -> None:
-        if self.fast is not None and ctx.use_fast_attention:
+        if self.fast is not None and ctx.use_fast_attention and not ctx.codes:
             from ..kernels import attention as fast
             fast.step_tiles(ctx, self.fast, int(self.window or 0))
 
@@ -86,7 +88,10 @@ class Attention(Part):
         q = ctx.ws.get("q", (n, qd), ctx.dtype)
         inv_freq = self.position.fused_rotation()
         apply = getattr(self.position, "apply", None)
-        if apply is not None:
+        codes = call.cache.maps is not None      # a cache of e4m3 codes: kernels of its own, behind the plain projection
+        if codes and apply is None:
+            qkv = self.qkv.forward(ctx, h, n, qkv_dtype, "qkv", allow_partials=True)
+        elif apply is not None:
             # a position encoding with kernels of its own: it changes q and k in place, as [tokens, heads,
             # head_dim] views of the finished projection, before k and v go into the cache
             qkv = self.qkv.forward(ctx, h, n, ctx.dtype, "qkv")
@@ -97,12 +102,17 @@ class Attention(Part):
             rotate = K.RotateAndCache(q, call.cache, ctx.positions, ctx.row_seq, inv_freq, self.heads, call.writes_cache,
                                       getattr(self.position, "angles", None))
             qkv = self.qkv.forward(ctx, h, n, qkv_dtype, "qkv", allow_partials=True, epilogue=rotate)
-        if qkv is not None:
+        if codes:
+            from ..kernels import cache8
+            cache8.append(qkv, q, call.cache, call.cache.maps, None if apply is not None else inv_freq, self.heads, call.writes_cache, ctx.stream)
+        elif qkv is not None:
             K.rope_cache_write(qkv, q, call.cache, ctx.positions, ctx.row_seq, inv_freq, self.heads,
                                call.writes_cache, n, ctx.stream)
         out = ctx.ws.get("attn_out", (n, qd), ctx.dtype)
         window = int(self.window) if self.window else 0
-        if self.fast is not None and ctx.use_fast_attention:
+        if codes:
+            cache8.attention(q, out, call.cache, call.cache.maps, self.heads, self.scale, window, None, ctx.stream)
+        elif self.fast is not None and ctx.use_fast_attention:
             from ..kernels import attention as fast
             fast.run(ctx, self.fast, q, out, call.cache, self.scale, window)
         else:
