@@ -21,9 +21,10 @@ struct Cache8 {
   uint8_t* v;
   float* k_scale;              // this cache's scales of page 0
   float* v_scale;
-  const int32_t* block_table;  // [batch sequences][table_stride]: page of a request's n-th block, -1 if none
+  const int32_t* block_table;  // [batch sequences][table_stride]: page of a request's n-th block, below zero if none
   long long page_stride;       // codes from one page to the next
   long long scale_stride;      // scales from one page to the next
+  int n_pages;                 // of the pool: the table's entries outside 0 .. n_pages - 1 count as no page
   int table_stride;
   int page_tokens;             // a multiple of SCALE_TOKENS
   int kv_heads;
@@ -44,8 +45,19 @@ __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e 
 // The exponent of a normal positive power of two.
 __device__ __forceinline__ int exponent_of(float s) { return (__float_as_int(s) >> 23) - 127; }
 
-// The page that holds `position` of batch sequence `seq`, -1 if none does.
+// Whether the current device is met for the first time (a kernel's attributes hold for one device); `met`: a bit a device.
+static inline bool first_on_device(unsigned long long& met) {
+  int device = 0;
+  cudaGetDevice(&device);
+  const unsigned long long bit = 1ull << (device & 63);
+  const bool first = !(met & bit);
+  met |= bit;
+  return first;
+}
+
+// The page that holds `position` (zero or more) of batch sequence `seq`, -1 if none does.
 __device__ __forceinline__ int page_of(const Cache8& c, int seq, int position) {
   const int block = position / c.page_tokens;
-  return block < c.table_stride ? __ldg(c.block_table + (long long)seq * c.table_stride + block) : -1;
+  const int page = block < c.table_stride ? __ldg(c.block_table + (long long)seq * c.table_stride + block) : -1;
+  return page < c.n_pages ? page : -1;
 }

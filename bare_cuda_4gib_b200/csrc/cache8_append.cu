@@ -144,6 +144,10 @@ __global__ void __launch_bounds__(TOKENS * (D / 16), D == 128 ? 6 : 12) cache8_a
   const int q_start = a.lists.seq_q_start[seq], kv_len = a.lists.seq_kv_len[seq], cached = kv_len - a.lists.seq_q_len[seq];
   const int lo = max(first, cached), n_new = min(first + TOKENS, kv_len) - lo;      // the block's new positions: lo ..
   const long long row0 = (long long)q_start + lo - cached;                            // their first row
+  if (n_new <= 0) {        // (rows that the step does not have)
+    pdl_wait();
+    return;
+  }
   const int page = page_of(a.cache, seq, first);
   const bool write = a.write_cache && page >= 0;
   const int in_page = first % a.cache.page_tokens;

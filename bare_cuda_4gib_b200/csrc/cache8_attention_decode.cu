@@ -16,6 +16,10 @@
 //  * A code becomes a half by one conversion for two; halves hold e4m3 exactly.  The scale of the keys joins the factor of
 //    the scores.  A weight goes into P together with its block's value scale: P = 2^(s + e_V - m) with m the running maximum of s + e_V,
 //    while the sum takes P 2^-e_V; so a half of P is relative to what the row's keys can add to its output, and O needs no factor.
+//    Float32 drops a P below 2^-126, and with it a share of that times 2^(largest e_V - e_V) of the sum: nothing where e_V is of the size of the
+//    others', all of it for a block of zeros (e_V = -100) beside values in the millions.  Blocks with e_V below FAR_VALUES take 2^(s - m) itself, so
+//    that no share above 2^-26 is lost while the largest value is below 448 * 2^60.  (A test a block, which costs nothing here.)  For the same reason a
+//    sum goes from one maximum to a larger one by way of half their distance, twice: m of a row that has seen only zeros may lie 2^200 below.
 //    Queries become halves times a power of two of their row's own (exact but for entries 2^24 below the row's largest).
 //  * The maximum that the exponentials are taken against moves only when a score has outgrown it by 2^8: until then 16 keys need no
 //    exchange between threads but one vote.
@@ -46,6 +50,7 @@ constexpr int TILES = D / 16;                  // 16-channel tiles of the output
 constexpr int VW = D / 32;                     // 32-bit words of a value that a thread takes (an eighth of its channels)
 constexpr int FEW_ROWS = 16;
 constexpr float RESCALE_STEP = 8.0f;           // base-2 units
+constexpr int FAR_VALUES = -40;
 constexpr int UNIT_BYTES = UNIT * D;           // keys, or values, of one scale block
 constexpr int STAGES = D == 128 ? 3 : 6;       // scale blocks a warp has in flight: 96 KB a thread block, two of which share an SM
 constexpr int RING_BYTES = WARPS * STAGES * 2 * UNIT_BYTES;
@@ -347,9 +352,9 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
 #pragma unroll
           for (int by = 4; by < 32; by <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, by));
           const float m_new = fmaxf(m[n][h], top);
-          const float corr = m_new == -INFINITY ? 1.0f : fast_exp2(m[n][h] - m_new);
+          const float down = m_new == -INFINITY ? 0.0f : m[n][h] - m_new, half_way = fast_exp2(0.5f * down), corr = fast_exp2(down);
           m[n][h] = m_new;
-          l[n][h] *= corr;
+          l[n][h] = l[n][h] * half_way * half_way;
 #pragma unroll
           for (int i = 0; i < TILES; ++i) o[n][i][h] *= corr, o[n][i][h + 2] *= corr;
         }
@@ -359,8 +364,14 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
     for (int n = 0; n < NT; ++n) {
       const float m0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
       const float p0 = fast_exp2(s[n][0] - m0), p1 = fast_exp2(s[n][1] - m1), p2 = fast_exp2(s[n][2] - m0), p3 = fast_exp2(s[n][3] - m1);
-      l[n][0] = fmaf(p0 + p2, power_of_two(-ev), l[n][0]);
-      l[n][1] = fmaf(p1 + p3, power_of_two(-ev), l[n][1]);
+      if (ev >= FAR_VALUES) {       // the same for the whole warp
+        l[n][0] = fmaf(p0 + p2, power_of_two(-ev), l[n][0]);
+        l[n][1] = fmaf(p1 + p3, power_of_two(-ev), l[n][1]);
+      } else {
+        const float e = (float)ev;
+        l[n][0] += fast_exp2(s[n][0] - e - m0) + fast_exp2(s[n][2] - e - m0);
+        l[n][1] += fast_exp2(s[n][1] - e - m1) + fast_exp2(s[n][3] - e - m1);
+      }
       pf[n][0] = transposed(pack_half(p0, p1));
       pf[n][1] = transposed(pack_half(p2, p3));
     }
@@ -425,9 +436,9 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
       const float* from = st + ((size_t)w * ROWS + r) * STATE;
-      const float f = from[D] == -INFINITY ? 1.0f : exp2f(from[D] - M_use);   // without a maximum: zeros, or NaN to be handed on
+      const float half_way = from[D] == -INFINITY ? 1.0f : exp2f(0.5f * (from[D] - M_use)), f = half_way * half_way;   // without a maximum: zeros, or NaN to be handed on
       const float4 v = *reinterpret_cast<const float4*>(from + c4 * 4);
-      L += from[D + 1] * f;
+      L += from[D + 1] * half_way * half_way;
       acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
     }
     const uint32_t local = smem_u32(recv + ((size_t)split * owned_rows + r / n_splits) * STATE);
@@ -453,9 +464,9 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
 #pragma unroll 8
     for (int z = 0; z < n_splits; ++z) {
       const float* from = recv + ((size_t)z * owned_rows + slot) * STATE;
-      const float f = from[D] == -INFINITY ? 1.0f : exp2f(from[D] - M_use);
+      const float half_way = from[D] == -INFINITY ? 1.0f : exp2f(0.5f * (from[D] - M_use)), f = half_way * half_way;
       const float4 v = *reinterpret_cast<const float4*>(from + c4 * 4);
-      L += from[D + 1] * f;
+      L += from[D + 1] * half_way * half_way;
       acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
     }
     const float inv = L == 0.0f ? 0.0f : head_gate<__nv_bfloat16>(extras, q_start + token, head) / L;
@@ -471,13 +482,12 @@ size_t smem_bytes(int rows, int n_splits) {
 
 template <int NT>
 int launch(const CUtensorMap& map, const DecodeArgs& a, int n_splits, cudaStream_t stream) {
-  static bool raised = false;
-  if (!raised) {
+  static unsigned long long met = 0;
+  if (first_on_device(met)) {
     const int most = (int)(RING_BYTES + (8 * NT + 8) * STATE * 4 + WARPS * STAGES * 8);
     if (cudaFuncSetAttribute(cache8_decode_kernel<NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess ||
         cudaFuncSetAttribute(cache8_decode_kernel<NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess)
-      return launch_status();
-    raised = true;
+      return met = 0, launch_status();
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.lists.n_seqs, a.cache.kv_heads, n_splits);

@@ -19,7 +19,9 @@
 //                  running maximum and sum in float32 (base 2), write P as halves back into tensor memory.
 // The scales cost the softmax nothing but their constants: the keys' joins the factor of 16 scores, and a weight goes into P together with the
 // scale of its values: P = 2^(s + e_V - m) with m the running maximum of s + e_V, while the sum takes P 2^-e_V.  So a half of P is relative to
-// what the row's keys can add to its output, and O needs no factor of its own.
+// what the row's keys can add to its output, and O needs no factor of its own.  A block whose values are all below 2^-60 of the
+// largest so far (one of zeros, say, whose scale is the least one) would leave of such a P nothing to take a sum from; its values count as zeros and
+// its e_V as the largest so far.
 // m follows the true maximum only when that has grown by more than 2^8 (a half reaches 2^15), so O is rescaled rarely.
 // A half of P takes the columns of the scores it was made of (S 2 x 128, O 2 x head size columns of the 512), and the next key block's half of S is
 // issued when P has been read, while the softmax is at the other half: it waits for no product.
@@ -67,6 +69,7 @@ constexpr int CHUNKS = D / 16;              // 16-byte chunks of a key's codes; 
 constexpr int BLOCKS = BN / SCALE_TOKENS;   // scale blocks of a key block
 constexpr int MAX_SPLITS = 8;               // blocks that may share a tile's keys
 constexpr int KNOWN = 8;                    // key blocks whose scales are kept (a key tile's slot is free again at most five blocks on)
+constexpr int VALUE_RANGE = 60;             // how far below the largest exponent of a value scale another one counts (base 2)
 constexpr int STATE = D + 4;                // floats of a row's state in a merge: D sums, the maximum, the sum
 constexpr size_t TILES_BYTES = (size_t)(TILES * 2 + K_SLOTS + C_SLOTS) * CODES + (size_t)V_SLOTS * VALUES;
 static_assert((size_t)BLOCK_ROWS * STATE * 4 <= TILES_BYTES, "the states of a merge lie over the tiles");
@@ -75,7 +78,7 @@ struct Scales {
   float key[BLOCKS];       // 2^e_K (1 where it is lost)
   float value[BLOCKS];     // e_V
   float back[BLOCKS];      // 2^-e_V
-  uint32_t lost, unused[3];   // bit b: scale block b has no number as its keys' scale
+  uint32_t special, unused[3];   // bits b, 8 + b: scale block b has no number as its keys' scale, has no page
 };
 
 // barriers (two to a slot, 14 of the groups, one to a block of scales), scales, rows' exponents, what is held, two words; 16 for alignment
@@ -247,19 +250,19 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 // 2^x for both of a pair without the exponential unit, which takes eight cycles a warp and is what the softmax would wait for: x = n + f with
 // n the nearest whole number (found by adding 1.5 * 2^23), 2^f by a polynomial that was fitted to it on [-1/2, 1/2] for the least
-// relative error (2.6e-6), n added to its exponent.  Below 2^-126: that number.  One pair of four goes this way:
-// the 7b portion below 122 -> 117 us.
+// relative error (2.9e-6) with 1 at 0, n added to its exponent.  Up to x = -127: zero, as that exponent says of a one.  One pair of four goes
+// this way: the 7b portion below 122 -> 117 us.
 __device__ __forceinline__ void exp2_by_products(uint64_t x, float& p0, float& p1) {
   float a, b;
   unpair(x, a, b);
-  a = fmaxf(a, -126.0f), b = fmaxf(b, -126.0f);
+  a = fmaxf(a, -127.0f), b = fmaxf(b, -127.0f);
   x = pair(a, b);
   const uint64_t big = pair(12582912.0f, 12582912.0f), minus_big = pair(-12582912.0f, -12582912.0f), minus_one = pair(-1.0f, -1.0f);
   const uint64_t r = add2(x, big), f = fma2(add2(r, minus_big), minus_one, x);
-  uint64_t p = fma2(f, pair(0.0095701f, 0.0095701f), pair(0.05591786f, 0.05591786f));
-  p = fma2(p, f, pair(0.24024745f, 0.24024745f));
-  p = fma2(p, f, pair(0.69312181f, 0.69312181f));
-  p = fma2(p, f, pair(0.99999926f, 0.99999926f));
+  uint64_t p = fma2(f, pair(0.009582576f, 0.009582576f), pair(0.05590683f, 0.05590683f));
+  p = fma2(p, f, pair(0.24024107f, 0.24024107f));
+  p = fma2(p, f, pair(0.6931241f, 0.6931241f));
+  p = fma2(p, f, pair(1.0f, 1.0f));
   float n0, n1;
   unpair(r, n0, n1);
   unpair(p, p0, p1);
@@ -363,6 +366,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
   const int group = a.q_heads / a.cache.kv_heads;
   const int q_start = a.lists.seq_q_start[seq], q_len = a.lists.seq_q_len[seq], kv_len = a.lists.seq_kv_len[seq];
   const int row0 = a.lists.tile_index[tile] * BLOCK_ROWS, n_rows = q_len * group, pos0 = kv_len - q_len;
+  if (row0 >= n_rows) {      // (rows that the step does not have)
+    pdl_wait();
+    return;
+  }
   // per group (tile of 128 rows): its key blocks [g_lo, g_hi) and the positions of its first and last row
   int g_lo[TILES] = {}, g_hi[TILES] = {}, g_min_pos[TILES] = {}, g_max_pos[TILES] = {};
   int kb_lo = 1 << 30, kb_hi = 0;   // the union of the two ranges, then this block's share of it
@@ -519,9 +526,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
       if (leads && p.row >= 0) tma_load_2d(smem_u32(slot) + lane * SCALE_TOKENS * D, &pool_map, full, 0, (int)(p.row + row0));
     };
     Place now = place(0, find_page(0));
-    int page = -1;
+    int page = -1, most = SCALE_LEAST;        // the largest exponent of a value scale so far
     for (int jj = 0; jj < n_kb; ++jj) {
-      const uint32_t there = __ballot_sync(0xffffffffu, now.row >= 0), copies = __popc(__ballot_sync(0xffffffffu, leads && now.row >= 0));
+      int ev = now.row >= 0 ? max(exponent_of(now.v_scale), SCALE_LEAST) : SCALE_LEAST;      // (a scale that nothing has written is zero)
+      most = max(most, __reduce_max_sync(0xffffffffu, ev));
+      const bool small = ev < most - VALUE_RANGE;
+      if (small) ev = most;
+      const uint32_t there = __ballot_sync(0xffffffffu, now.row >= 0 && !small), copies = __popc(__ballot_sync(0xffffffffu, leads && now.row >= 0));
       const int ks = jj % K_SLOTS, cs = jj % C_SLOTS;
       ok = jj < K_SLOTS || mbar_wait(&k_empty[ks], (uint32_t)(jj / K_SLOTS - 1) & 1u, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
@@ -541,13 +552,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
       const bool lost = isnan(now.k_scale);
       Scales* to = scales + jj % KNOWN;
       if (lane < BLOCKS) {
-        const int ev = now.row >= 0 ? max(exponent_of(now.v_scale), SCALE_LEAST) : 0;      // (a scale that nothing has written is zero)
         to->key[lane] = now.row >= 0 && !lost ? fmaxf(now.k_scale, power_of_two(SCALE_LEAST)) : 1.0f;
         to->value[lane] = (float)ev;
         to->back[lane] = power_of_two(-ev);
       }
       const uint32_t all_lost = __ballot_sync(0xffffffffu, lost && now.row >= 0);
-      if (lane == 0) to->lost = all_lost;
+      const uint32_t all_absent = __ballot_sync(0xffffffffu, lane < BLOCKS && now.row < 0 && (kb_lo + jj) * BN + lane * SCALE_TOKENS < kv_len);
+      if (lane == 0) to->special = all_lost | all_absent << 8;
       __syncwarp();
       if (lane == 0) mbar_arrive(&known[jj % KNOWN]);
       now = next;
@@ -633,13 +644,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
   } else {
     // ------------------------------------------------------------------ softmax: group g owns tile g, one thread per row
     // D / 8 threads to a row of Q, so that the loads are whole lines; where a row lies, and its power of two, the row's own thread knows
-    {
-      constexpr int LANES = D / 8, ROWS = 32 / LANES;          // of a load of the warp
-      const long long my_at = row_valid ? ((long long)(q_start + token) * a.q_heads + head) * D : -1;
-      constexpr int BATCH = 4;                                 // loads on their way at once
+    constexpr int LANES = D / 8, ROWS = 32 / LANES;          // of a load of the warp
+    constexpr int BATCH = 4;                                 // loads on their way at once
+    const long long my_at = row_valid ? ((long long)(q_start + token) * a.q_heads + head) * D : -1;
 #pragma unroll 1
-      for (int batch = 0; batch < 32 / ROWS / BATCH; ++batch) {
-        uint4 raw[BATCH];
+    for (int batch = 0; batch < 32 / ROWS / BATCH; ++batch) {
+      uint4 raw[BATCH];
 #pragma unroll
       for (int i = 0; i < BATCH; ++i) {
         const long long at = __shfl_sync(0xffffffffu, my_at, (batch * BATCH + i) * ROWS + lane / LANES);
@@ -676,7 +686,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
         asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + CODES), "r"(part[1][0]), "r"(part[1][1]) : "memory");
         if (c == 0) q_exponent[g * BM + in_tile] = e;
       }
-      }
     }
     __syncwarp();
     const float factor = a.scale_log2 * power_of_two(q_exponent[g * BM + r]);       // (this warp wrote it)
@@ -704,11 +713,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
 #pragma unroll
         for (int k = 0; k < S_PIECE; k += 32) tmem_load32_nowait(s_addr + h * S_PIECE + k, v + k);
         tmem_wait_loads();
-        const uint32_t lost = of_block->lost;
-        if ((lost >> (h * 4)) & 15u) {
+        const uint32_t special = of_block->special >> (h * 4);
+        if (special & 0x0f0fu) {
 #pragma unroll
-          for (int k = 0; k < S_PIECE; ++k)
-            if ((lost >> (h * 4 + k / SCALE_TOKENS)) & 1u) v[k] = 0x7fc00000u;
+          for (int k = 0; k < S_PIECE; ++k) {
+            if ((special >> (k / SCALE_TOKENS)) & 1u) v[k] = 0x7fc00000u;
+            if ((special >> (8 + k / SCALE_TOKENS)) & 1u) v[k] = 0xff800000u;
+          }
         }
         if (!all_visible) {
 #pragma unroll
@@ -761,9 +772,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
             l2 = sum;
             break;
           }
-          const float corr = fast_exp2(m - (m_new == -INFINITY ? 0.0f : m_new));   // m = -inf gives 0
+          const float down = m - (m_new == -INFINITY ? 0.0f : m_new), half_way = fast_exp2(0.5f * down), corr = fast_exp2(down);   // m = -inf gives 0
           m = m_new;
-          l2 = fma2(l2, pair(corr, corr), 0);
+          l2 = fma2(fma2(l2, pair(half_way, half_way), 0), pair(half_way, half_way), 0);
           if (i > 0 || h > 0) {     // O = O * corr in tensor memory, when every product issued so far is complete
             ok = h > 0 ? wait_pv(i, 0) : wait_pv(i - 1, 1);
             if (!ok) break;
@@ -865,13 +876,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
       for (int by = 1; by < MAX_SPLITS; by <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, by));      // (of the first eight lanes of a row)
       M = fmaxf(__shfl_sync(0xffffffffu, M, lane & ~(LANES - 1)), sink);
       const float M_use = M == -INFINITY ? 0.0f : M;
-      const float f_mine = ml.x == -INFINITY ? 1.0f : exp2f(ml.x - M_use);      // without a maximum: zeros, or NaN to be handed on
+      const float h_mine = ml.x == -INFINITY ? 1.0f : exp2f(0.5f * (ml.x - M_use));      // without a maximum: zeros, or NaN to be handed on
+      const float part_mine = ml.y * h_mine * h_mine, f_mine = h_mine * h_mine;
       float L = exp2f(sink - M_use);
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int z = 0; z < MAX_SPLITS; ++z) {
-        const float f = __shfl_sync(0xffffffffu, f_mine, (lane & ~(LANES - 1)) + z), part = __shfl_sync(0xffffffffu, ml.y, (lane & ~(LANES - 1)) + z);
-        L += part * f;
+        const float f = __shfl_sync(0xffffffffu, f_mine, (lane & ~(LANES - 1)) + z), part = __shfl_sync(0xffffffffu, part_mine, (lane & ~(LANES - 1)) + z);
+        L += part;
         acc.x += v[z].x * f, acc.y += v[z].y * f, acc.z += v[z].z * f, acc.w += v[z].w * f;
       }
       const float inv = L == 0.0f ? 0.0f : head_gate<__nv_bfloat16>(extras, q_start + tok, hd) / L;
@@ -944,12 +956,11 @@ extern "C" int llm_cache8_attention_prompt(const void* q, void* out, const Cache
   const long long v_off = reinterpret_cast<const char*>(c.v) - reinterpret_cast<const char*>(pool_base);
   if ((all & 15) || k_off < 0 || v_off < 0 || k_off % D || v_off % D || c.page_stride % D) return ERR_BAD_ALIGN;
   if (box_rows < SCALE_TOKENS || BN % box_rows || box_rows % SCALE_TOKENS || c.page_tokens % box_rows) return ERR_BAD_SIZE;
-  static bool configured = false;
-  if (!configured) {
+  static unsigned long long met = 0;
+  if (first_on_device(met)) {
     if (cudaFuncSetAttribute(cache8_prompt_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES) != cudaSuccess ||
         cudaFuncSetAttribute(cache8_prompt_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES) != cudaSuccess)
-      return launch_status();
-    configured = true;
+      return met = 0, launch_status();
   }
   const AttnArgs a{reinterpret_cast<const __nv_bfloat16*>(q), reinterpret_cast<__nv_bfloat16*>(out), c, c.page_stride / D, k_off / D, v_off / D,
                    box_rows, *lists, q_heads,

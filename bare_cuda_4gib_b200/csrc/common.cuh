@@ -32,10 +32,10 @@
 //  - shared memory and tensor memory;
 //  - weights and tables that were made with the model;
 //  - the step's metadata (positions, lengths, block tables): it is copied to the device ahead of the
-//    step's first kernel, and no kernel writes it;
+//    step's first kernel, or made there by llm_step_maps, which is an ordinary launch; no other kernel writes it;
 //  - cache positions below the step's first new one (read so by the two attentions of decoding requests): kernels of
 //    earlier steps wrote them.
-// The last two are safe because every step begins with that copy, an ordinary operation of the stream:
+// The last two are safe because every step begins with that copy (and that launch), ordinary operations of the stream:
 // no kernel of the step starts before it, and it waits for all kernels of the step before.  A caller that
 // appends to a request's cache and attends over it, or writes metadata by a kernel, with nothing but
 // such kernels in between would race: it has to put a copy or a synchronisation there.

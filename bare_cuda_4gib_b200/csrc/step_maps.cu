@@ -9,7 +9,8 @@
 //   position = cached + place in the request  slot = page * page_tokens + position % page_tokens
 //   table[s][b] = pages[first page of s + b]  for the ceil(kv_len / page_tokens) blocks of s, -1 behind them
 //
-// A request with cached < 0 is an idle row that pads a decode step: its rows count, it holds nothing.
+// A request with cached < 0 is an idle row that pads a decode step: its rows count, it holds nothing.  Positions behind the table's
+// last page are not held, and rows behind the step's last belong to no request: what is listed here is in bounds, whatever the lengths say.
 //
 // Nothing here is worth bandwidth (3 MB at most); what it costs is its chain of dependent trips to memory: lengths, then pages, then
 // the stores.  So every block sums the lengths of all requests for itself (no block waits for another, no second launch), and
@@ -21,12 +22,7 @@
 
 #include "cache8.cuh"
 
-namespace {
-
-constexpr int THREADS = 256;
-constexpr int TABLE_CHUNK = 256;     // entries of a table row that a warp fills at a time
-constexpr int MAX_SEQS = 4096;       // the four sums of every request lie in shared memory
-
+// What a call is made of (all arrays on the device; what they hold, see llm_step_maps).
 struct MapsArgs {
   const int32_t* cached;
   const int32_t* q_len;
@@ -39,13 +35,20 @@ struct MapsArgs {
   int32_t *block_table, *write_seq, *write_block, *tile_seq, *tile_index;
 };
 
+namespace {
+
+constexpr int THREADS = 256;
+constexpr int TABLE_CHUNK = 256;     // entries of a table row that a warp fills at a time
+constexpr int MAX_SEQS = 4096;       // the four sums of every request lie in shared memory
+
 // What request s brings: rows, pages, written blocks, tiles.
 __device__ __forceinline__ int4 counts_of(const MapsArgs& a, int s, int& cached, int& q) {
   cached = a.cached[s];
-  q = max(a.q_len[s], 0);
-  if (cached < 0 || q == 0) return make_int4(q, cached > 0 ? (cached + a.page_tokens - 1) / a.page_tokens : 0, 0, 0);
+  q = min(max(a.q_len[s], 0), a.n_rows);
+  const int blocks = cached < 0 ? 0 : (int)(((long long)cached + q + a.page_tokens - 1) / a.page_tokens);
+  if (cached < 0 || q == 0) return make_int4(q, blocks, 0, 0);
   const int kv = cached + q, packed = q * a.group;
-  return make_int4(q, (kv + a.page_tokens - 1) / a.page_tokens, (kv - 1) / SCALE_TOKENS - cached / SCALE_TOKENS + 1,
+  return make_int4(q, blocks, (kv - 1) / SCALE_TOKENS - cached / SCALE_TOKENS + 1,
                    packed > a.few_rows ? (packed + a.tile_rows - 1) / a.tile_rows : 0);
 }
 __device__ __forceinline__ int4 add(int4 x, int4 y) { return make_int4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w); }
@@ -88,10 +91,11 @@ __global__ void __launch_bounds__(THREADS) step_maps_kernel(const MapsArgs a) {
   for (int s = s0; s < s1; ++s) {
     rows[s] = at.x, first_page[s] = at.y, writes[s] = at.z, tiles[s] = at.w;
     const int4 c = counts_of(a, s, cached, q);
+    q = cached < 0 ? 0 : min(q, max(a.n_rows - at.x, 0));
     kv_len[s] = cached < 0 ? 0 : cached + q;
     if (blockIdx.x == 0) {
       a.seq_q_start[s] = at.x;
-      a.seq_q_len[s] = cached < 0 ? 0 : q;
+      a.seq_q_len[s] = q;
       a.seq_kv_len[s] = cached < 0 ? 0 : cached + q;
     }
     at = add(at, c);
@@ -107,7 +111,7 @@ __global__ void __launch_bounds__(THREADS) step_maps_kernel(const MapsArgs a) {
     if (s < S && a.cached[s] >= 0) {
       position = a.cached[s] + i - rows[s];
       const int b = position / a.page_tokens, at_page = first_page[s] + b;
-      const int page = b < a.max_blocks && at_page < a.n_pages ? a.pages[at_page] : -1;
+      const int page = b < a.max_blocks && (unsigned)at_page < (unsigned)a.n_pages ? a.pages[at_page] : -1;
       if (page >= 0) slot = (long long)page * a.page_tokens + position % a.page_tokens;
     }
     a.positions[i] = position;
@@ -135,7 +139,7 @@ __global__ void __launch_bounds__(THREADS) step_maps_kernel(const MapsArgs a) {
   // the tables: a warp takes a stretch of TABLE_CHUNK entries of a row at a time, all of its loads on their way at once
   const int chunks = (a.max_blocks + TABLE_CHUNK - 1) / TABLE_CHUNK;
   for (int c = first >> 5; c < S * chunks; c += step >> 5) {
-    const int s = c / chunks, b0 = (c - s * chunks) * TABLE_CHUNK + lane, from = first_page[s], held = min(first_page[s + 1], a.n_pages) - from;
+    const int s = c / chunks, b0 = (c - s * chunks) * TABLE_CHUNK + lane, from = first_page[s], held = from < 0 ? 0 : min(first_page[s + 1], a.n_pages) - from;
     int32_t* row = a.block_table + (long long)s * a.max_blocks;
     int page[TABLE_CHUNK / 32];
 #pragma unroll
@@ -144,6 +148,7 @@ __global__ void __launch_bounds__(THREADS) step_maps_kernel(const MapsArgs a) {
     for (int i = 0; i < TABLE_CHUNK / 32; ++i)
       if (b0 + 32 * i < a.max_blocks) row[b0 + 32 * i] = page[i];
   }
+  __threadfence();      // what this thread wrote is there for all before its block has ended, and with it any kernel behind it can start
 }
 
 }  // namespace
@@ -153,26 +158,20 @@ extern "C" int llm_step_maps_max_seqs() { return MAX_SEQS; }
 // Every output is a dense device array: per request (seq_q_start, seq_q_len, seq_kv_len, order), per row of the step (positions, row_seq,
 // slots), [n_seqs][max_blocks] (block_table), and lists of n_writes and n_tiles entries, whose entries behind the last
 // are -1 and 0.  `pages`: the held pages of request 0, then of request 1, ..., ceil(kv_len / page_tokens) each (-1: given back).
-extern "C" int llm_step_maps(const int32_t* cached, const int32_t* q_len, int n_seqs, const int32_t* pages, int n_pages, int n_rows,
-                             int page_tokens, int group, int tile_rows, int few_rows, int max_blocks, int n_writes, int n_tiles,
-                             int32_t* seq_q_start, int32_t* seq_q_len, int32_t* seq_kv_len, int32_t* order, int32_t* positions, int32_t* row_seq,
-                             long long* slots, int32_t* block_table, int32_t* write_seq, int32_t* write_block, int32_t* tile_seq,
-                             int32_t* tile_index, cudaStream_t stream) {
-  if (n_seqs <= 0) return 0;
-  if (n_seqs > MAX_SEQS || page_tokens <= 0 || page_tokens % SCALE_TOKENS || group <= 0 || tile_rows <= 0 || max_blocks <= 0 ||
-      n_rows < 0 || n_writes < 0 || n_tiles < 0 || n_pages < 0)
+extern "C" int llm_step_maps(const MapsArgs* args, cudaStream_t stream) {
+  const MapsArgs& a = *args;
+  if (a.n_seqs <= 0) return 0;
+  if (a.n_seqs > MAX_SEQS || a.page_tokens <= 0 || a.page_tokens % SCALE_TOKENS || a.group <= 0 || a.tile_rows <= 0 || a.max_blocks <= 0 ||
+      a.few_rows < 0 || a.n_rows < 0 || a.n_writes < 0 || a.n_tiles < 0 || a.n_pages < 0)
     return ERR_BAD_SIZE;
-  const size_t smem = (size_t)5 * (n_seqs + 1) * 4;
-  static bool raised = false;
-  if (!raised) {
+  const size_t smem = (size_t)5 * (a.n_seqs + 1) * 4;
+  static unsigned long long met = 0;
+  if (first_on_device(met)) {
     if (cudaFuncSetAttribute(step_maps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 5 * (MAX_SEQS + 1) * 4) != cudaSuccess)
-      return launch_status();
-    raised = true;
+      return met = 0, launch_status();
   }
-  MapsArgs a{cached, q_len, n_seqs, pages, n_pages, n_rows, page_tokens, group, tile_rows, few_rows, max_blocks, n_writes, n_tiles,
-             seq_q_start, seq_q_len, seq_kv_len, order, positions, row_seq, slots, block_table, write_seq, write_block, tile_seq, tile_index};
   // four numbers a thread, one block an SM at most
-  const long long numbers = (long long)n_rows + n_writes + n_tiles + (long long)n_seqs * max_blocks;
+  const long long numbers = (long long)a.n_rows + a.n_writes + a.n_tiles + (long long)a.n_seqs * a.max_blocks;
   const long long blocks = (numbers + 4 * THREADS - 1) / (4 * THREADS);
   step_maps_kernel<<<(int)(blocks < 1 ? 1 : blocks > 148 ? 148 : blocks), THREADS, smem, stream>>>(a);
   return launch_status();

@@ -6,6 +6,7 @@ Both go by the step's `StepMaps`.  Head sizes 64 and 128, bfloat16 queries and o
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from ctypes import c_float, c_int, c_longlong, c_void_p
 from typing import Dict, Optional
@@ -31,8 +32,8 @@ class _Cache8(ctypes.Structure):
     """struct Cache8 of csrc/cache8.cuh."""
 
     _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p), ("block_table", c_void_p),
-                ("page_stride", c_longlong), ("scale_stride", c_longlong), ("table_stride", c_int), ("page_tokens", c_int),
-                ("kv_heads", c_int), ("head_dim", c_int)]
+                ("page_stride", c_longlong), ("scale_stride", c_longlong), ("n_pages", c_int), ("table_stride", c_int),
+                ("page_tokens", c_int), ("kv_heads", c_int), ("head_dim", c_int)]
 
 
 def supports(head_dim: int, v_dim: Optional[int] = None, page_tokens: int = SCALE_TOKENS) -> bool:
@@ -111,45 +112,54 @@ def view(codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, i
     per_cache, per_cache_scales = 2 * kv_heads * page_tokens * head_dim, 2 * kv_heads * (page_tokens // SCALE_TOKENS)
     k = codes.data_ptr() + index * per_cache
     s = scales.data_ptr() + index * per_cache_scales * 4
-    return CacheView(k, k + per_cache // 2, block_table, caches * per_cache, block_table.stride(0), page_tokens, kv_heads, head_dim,
-                     DTYPE, codes.data_ptr(), codes.numel(), k_scale_ptr=s, v_scale_ptr=s + per_cache_scales // 2 * 4,
-                     scale_stride=caches * per_cache_scales)
+    out = CacheView(k, k + per_cache // 2, block_table, caches * per_cache, block_table.stride(0), page_tokens, kv_heads, head_dim,
+                    DTYPE, codes.data_ptr(), codes.numel(), k_scale_ptr=s, v_scale_ptr=s + per_cache_scales // 2 * 4,
+                    scale_stride=caches * per_cache_scales)
+    out.keeps = (codes, scales)
+    return out
 
 
-def _struct(cache: CacheView) -> int:
-    if cache.dtype != DTYPE:
-        raise KernelLaunchError(f"cache8: a cache of {cache.dtype} is not one of e4m3 codes")
-    if cache.struct is None:
-        cache.struct = _Cache8(cache.k_ptr, cache.v_ptr, cache.k_scale_ptr, cache.v_scale_ptr, cache.block_table.data_ptr(),
-                               cache.page_stride, cache.scale_stride, cache.table_stride, cache.page_tokens, cache.kv_heads, cache.head_dim)
-    return ctypes.addressof(cache.struct)
+class _Launch:
+    """What the launchers hand on of a cache, made at its first use and kept with its view: the struct's address, the kernels' tensor maps
+    over the pool, and the kernels' entries."""
+
+    def __init__(self, cache: CacheView):
+        if cache.dtype != DTYPE:
+            raise KernelLaunchError(f"cache8: a cache of {cache.dtype} is not one of e4m3 codes")
+        d = cache.head_dim
+        self._struct = _Cache8(cache.k_ptr, cache.v_ptr, cache.k_scale_ptr, cache.v_scale_ptr, cache.block_table.data_ptr(),
+                               cache.page_stride, cache.scale_stride, cache.pool_elems // cache.page_stride, cache.table_stride, cache.page_tokens,
+                               cache.kv_heads, d)
+        self.cache = ctypes.addressof(self._struct)
+        self.box_rows, rows = math.gcd(KEY_BLOCK, cache.page_tokens), cache.pool_elems // d
+        self._maps = (ctypes.c_ubyte * 128)(), (ctypes.c_ubyte * 128)()
+        self.decode_map, self.prompt_map = (ctypes.addressof(m) for m in self._maps)
+        _check(_decode(d).llm_cache8_decode_pool_map(self.decode_map, cache.pool_ptr, rows), "cache8 pool map")
+        _check(_prompt(d).llm_cache8_prompt_pool_map(self.prompt_map, cache.pool_ptr, rows, self.box_rows), "cache8 pool map")
+        self.append, self.decode, self.prompt = (_append().llm_cache8_append, _decode(d).llm_cache8_attention_decode,
+                                                 _prompt(d).llm_cache8_attention_prompt)
+        self.tile_rows, self.keys = tile_rows(d), cache.table_stride * cache.page_tokens
+        self.device, self.table_rows = cache.block_table.get_device(), cache.block_table.shape[0]
 
 
-def _pool_maps(cache: CacheView):
-    """The kernels' tensor maps over the pool that the cache lies in, kept with the view: (decode map, prompt map, the prompt map's box rows)."""
-    if cache.pool_map is None:
-        box_rows, rows = math.gcd(KEY_BLOCK, cache.page_tokens), cache.pool_elems // cache.head_dim
-        maps = (ctypes.c_ubyte * 128)(), (ctypes.c_ubyte * 128)()
-        _check(_decode(cache.head_dim).llm_cache8_decode_pool_map(ctypes.addressof(maps[0]), cache.pool_ptr, rows), "cache8 pool map")
-        _check(_prompt(cache.head_dim).llm_cache8_prompt_pool_map(ctypes.addressof(maps[1]), cache.pool_ptr, rows, box_rows), "cache8 pool map")
-        cache.pool_map = (maps, ctypes.addressof(maps[0]), ctypes.addressof(maps[1]), box_rows)
-    return cache.pool_map[1:]
-
-
-def _check_step(what: str, cache: CacheView, maps: StepMaps, q_heads: int, a: torch.Tensor, b: torch.Tensor) -> None:
+def _check_step(what: str, cache: CacheView, maps: StepMaps, q_heads: int, a: torch.Tensor, b: torch.Tensor) -> _Launch:
     """Whether cache, maps and the two tensors belong together (this and what follows runs for every layer of a step)."""
+    launch = cache.launch
+    if launch is None:
+        launch = cache.launch = _Launch(cache)
     if q_heads <= 0 or maps.group * cache.kv_heads != q_heads or maps.page_tokens != cache.page_tokens:
         raise KernelLaunchError(f"{what}: the step's maps are for pages of {maps.page_tokens} positions and {maps.group} heads a key/value "
                                 f"head, the cache has pages of {cache.page_tokens} and {cache.kv_heads} key/value heads for {q_heads} heads")
     if maps.longest == 0:
         raise KernelLaunchError(f"{what}: the step's maps have not been built")
-    if cache.block_table.shape[0] < maps.n_seqs:
-        raise KernelLaunchError(f"{what}: {maps.n_seqs} requests, and a block table of {cache.block_table.shape[0]} rows")
+    if launch.table_rows < maps.n_seqs:
+        raise KernelLaunchError(f"{what}: {maps.n_seqs} requests, and a block table of {launch.table_rows} rows")
     index = maps.index
-    if cache.block_table.get_device() != index or a.get_device() != index or b.get_device() != index:
+    if launch.device != index or a.get_device() != index or b.get_device() != index:
         raise KernelLaunchError(f"{what}: maps, cache and tensors must lie on one CUDA device")
     if index != torch.cuda.current_device():
         raise KernelLaunchError(f"{what}: the tensors lie on {maps.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return launch
 
 
 def _bf16_rows(t: torch.Tensor, rows: int, width: int) -> bool:
@@ -166,8 +176,7 @@ def append(qkv: Partials, q_out: torch.Tensor, cache: CacheView, maps: StepMaps,
     left as they were in `q_out`."""
     t = qkv.tensor
     width, d = (q_heads + 2 * cache.kv_heads) * cache.head_dim, cache.head_dim
-    at = _struct(cache)
-    _check_step("cache8_append", cache, maps, q_heads, t, q_out)
+    launch = _check_step("cache8_append", cache, maps, q_heads, t, q_out)
     shape = t.shape
     if shape[-1] != width or shape[-2] < maps.n_rows or t.stride(-1) != 1 or t.stride(-2) != width or (qkv.n > 1 and shape[0] < qkv.n):
         raise KernelLaunchError(f"cache8_append: projections of {tuple(shape)} for {maps.n_rows} dense rows of {width}")
@@ -176,11 +185,12 @@ def append(qkv: Partials, q_out: torch.Tensor, cache: CacheView, maps: StepMaps,
     if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.numel() != d // 2 or not inv_freq.is_contiguous()
                                  or inv_freq.get_device() != maps.index):
         raise KernelLaunchError(f"cache8_append: the inverse frequencies must be {d // 2} contiguous float32 numbers")
-    _check(_append().llm_cache8_append(
-        t.data_ptr(), dtype_code(t.dtype), qkv.n, qkv.stride, q_out.data_ptr(), at, maps.lists, _ptr(inv_freq), q_heads,
+    _check(launch.append(
+        t.data_ptr(), dtype_code(t.dtype), qkv.n, qkv.stride, q_out.data_ptr(), launch.cache, maps.lists, _ptr(inv_freq), q_heads,
         1 if write_cache else 0, stream if stream is not None else stream_handle()), "cache8_append")
 
 
+@functools.lru_cache(maxsize=256)
 def decode_splits(n_seqs: int, kv_heads: int, max_keys: int) -> int:
     """How many blocks of the decode kernel share a request's keys: a power of two up to 8, about two blocks an SM in all, and no more
     than have a scale block for every warp.  With long caches twice that: requests of different lengths then leave fewer SMs idle at the
@@ -193,6 +203,7 @@ def decode_splits(n_seqs: int, kv_heads: int, max_keys: int) -> int:
     return splits
 
 
+@functools.lru_cache(maxsize=256)
 def prompt_splits(n_tiles: int, kv_heads: int, max_keys: int) -> int:
     """How many blocks of the prompt kernel share a tile's keys: a power of two up to 8, as many as the SMs take at once."""
     splits = 1
@@ -206,31 +217,26 @@ def attention(q: torch.Tensor, out: torch.Tensor, cache: CacheView, maps: StepMa
     """out = softmax(scale * q k^T) v over each request's cached positions up to the query's own (with `window` > 0 the newest
     `window` of them), q and out contiguous bfloat16 [rows, q_heads * head size].  `extras`: blocks of positions, sink, gate.
     Requests of few packed rows go to the decode kernel, the others to the prompt kernel, which a step may launch both of; rows
-    of no request and idle ones are left as they were in `out`, a row that sees no key is zero."""
-    at = _struct(cache)
-    _check_step("cache8_attention", cache, maps, q_heads, q, out)
+    of no request and idle ones are left as they were in `out`, a row that sees no key is zero.  A position whose page is not held (an entry of the
+    block table outside the pool) is seen by no query."""
+    launch = _check_step("cache8_attention", cache, maps, q_heads, q, out)
     width = q_heads * cache.head_dim
     if not _bf16_rows(q, maps.n_rows, width) or not _bf16_rows(out, maps.n_rows, width):
         raise KernelLaunchError(f"cache8_attention: queries and outputs must be contiguous bfloat16 [{maps.n_rows} rows, {width}], not "
                                 f"{tuple(q.shape)} of {q.dtype} and {tuple(out.shape)} of {out.dtype}")
     if not scale > 0.0 or window < 0:
         raise KernelLaunchError(f"cache8_attention: scale {scale} and window {window} are not supported (above zero; zero or more)")
-    if maps.few_rows != FEW_ROWS or maps.tile_rows != tile_rows(cache.head_dim):
-        raise KernelLaunchError(f"cache8_attention: the step's maps must be made with few_rows {FEW_ROWS} and tile_rows "
-                                f"{tile_rows(cache.head_dim)}")
-    chunk, sink, gate, gate_stride = extras.arguments(q_heads, q.dtype) if extras is not None else (0, 0, 0, 0)
+    if maps.few_rows != FEW_ROWS or maps.tile_rows != launch.tile_rows:
+        raise KernelLaunchError(f"cache8_attention: the step's maps must be made with few_rows {FEW_ROWS} and tile_rows {launch.tile_rows}")
+    more = extras.arguments(q_heads, q.dtype) if extras is not None else (0, 0, 0, 0)
     stream = stream if stream is not None else stream_handle()
-    group, keys = maps.group, cache.table_stride * cache.page_tokens
-    decode_map, prompt_map, box_rows = _pool_maps(cache)
-    error_word = gemm.error_word(q.device).data_ptr()
+    q_at, out_at, error_word, group = q.data_ptr(), out.data_ptr(), gemm.error_word(q.device).data_ptr(), maps.group
     if maps.shortest * group <= FEW_ROWS:
-        splits = decode_splits(maps.n_seqs, cache.kv_heads, keys)
-        _check(_decode(cache.head_dim).llm_cache8_attention_decode(
-            q.data_ptr(), out.data_ptr(), at, decode_map, cache.pool_ptr, maps.lists, splits,
-            1 if maps.n_seqs * cache.kv_heads * splits > 2 * sm_count() else 0, min(maps.longest * group, FEW_ROWS), q_heads, scale, window, chunk, sink, gate, gate_stride, error_word, stream),
-            "cache8_attention_decode")
+        splits = decode_splits(maps.n_seqs, cache.kv_heads, launch.keys)
+        ordered = 1 if maps.n_seqs * cache.kv_heads * splits > 2 * sm_count() else 0
+        _check(launch.decode(q_at, out_at, launch.cache, launch.decode_map, cache.pool_ptr, maps.lists, splits, ordered,
+                             min(maps.longest * group, FEW_ROWS), q_heads, scale, window, *more, error_word, stream), "cache8_attention_decode")
     if maps.longest * group > FEW_ROWS:
-        _check(_prompt(cache.head_dim).llm_cache8_attention_prompt(
-            q.data_ptr(), out.data_ptr(), at, prompt_map, cache.pool_ptr, box_rows, maps.lists,
-            prompt_splits(maps.n_tiles, cache.kv_heads, keys), q_heads, scale, window, chunk, sink, gate, gate_stride, error_word, stream),
-            "cache8_attention_prompt")
+        _check(launch.prompt(q_at, out_at, launch.cache, launch.prompt_map, cache.pool_ptr, launch.box_rows, maps.lists,
+                             prompt_splits(maps.n_tiles, cache.kv_heads, launch.keys), q_heads, scale, window, *more, error_word, stream),
+               "cache8_attention_prompt")

@@ -77,13 +77,14 @@ class CacheView:
 
     __slots__ = ("k_ptr", "v_ptr", "block_table", "page_stride", "table_stride", "page_tokens",
                  "kv_heads", "head_dim", "dtype", "pool_ptr", "pool_elems", "v_dim", "k_scale_ptr", "v_scale_ptr", "scale_stride",
-                 "struct", "pool_map", "maps")
+                 "launch", "keeps", "maps")
 
     def __init__(self, k_ptr, v_ptr, block_table, page_stride, table_stride, page_tokens, kv_heads,
                  head_dim, dtype, pool_ptr=0, pool_elems=0, v_dim=None, k_scale_ptr=0, v_scale_ptr=0, scale_stride=0):
-        # a cache of 8-bit codes: its scales, floats from one page's to the next, and (made at first use) what its kernels take and the tensor map over its pool
+        # a cache of 8-bit codes: its scales, floats from one page's to the next; what its launchers hand on (made at first use); the
+        # tensors that it lies in, where the view has to keep them
         self.k_scale_ptr, self.v_scale_ptr, self.scale_stride = k_scale_ptr, v_scale_ptr, scale_stride
-        self.struct = self.pool_map = None
+        self.launch = self.keeps = None
         self.maps = None      # the step's maps (kernels.step_maps.StepMaps) where the step function keeps them for this cache
         self.v_dim = head_dim if v_dim is None else v_dim    # value head size (the key head's unless stated)
         self.pool_ptr, self.pool_elems = pool_ptr, pool_elems     # the group's whole storage (for TMA)

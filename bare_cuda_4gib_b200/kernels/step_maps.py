@@ -23,12 +23,20 @@ def lib():
     global _lib
     if _lib is None:
         l = build.load_library("step_maps.cu")
-        P, I = c_void_p, c_int
-        l.llm_step_maps.argtypes = [P, P, I, P, I, I, I, I, I, I, I, I, I] + [P] * 13
+        l.llm_step_maps.argtypes = [c_void_p, c_void_p]
         l.llm_step_maps.restype = c_int
         l.llm_step_maps_max_seqs.restype = c_int
         _lib = l
     return _lib
+
+
+class MapsArgs(ctypes.Structure):
+    """struct MapsArgs of csrc/step_maps.cu."""
+
+    _fields_ = [("cached", c_void_p), ("q_len", c_void_p), ("n_seqs", c_int), ("pages", c_void_p)] + [(name, c_int) for name in (
+        "n_pages", "n_rows", "page_tokens", "group", "tile_rows", "few_rows", "max_blocks", "n_writes", "n_tiles")] + [(name, c_void_p) for name in (
+            "seq_q_start", "seq_q_len", "seq_kv_len", "order", "positions", "row_seq", "slots", "block_table", "write_seq", "write_block",
+            "tile_seq", "tile_index")]
 
 
 class StepLists(ctypes.Structure):
@@ -44,6 +52,8 @@ class StepMaps:
 
     `group` query heads share a key/value head: a request with more than `few_rows` packed rows (tokens x group) is cut into tiles
     of `tile_rows`.
+
+    A `StepMaps` serves one stream: `build` writes what the kernels of the step before read, and waits for them in its stream's order.
 
     After `build`, for that step (S requests, T rows):
 
@@ -80,7 +90,9 @@ class StepMaps:
         self.device = self._table.device
         self.index = self.device.index
         self.table = self._table                       # the block tables whole, at the address that `block_table` keeps
-        self._out = tuple(t.data_ptr() for t in (*self._seqs, *self._rows, self._slots, self._table, *self._writes, *self._tiles))
+        self._args = MapsArgs(0, 0, 0, 0, 0, 0, page_tokens, group, tile_rows, few_rows, max_blocks, 0, 0,
+                              *(t.data_ptr() for t in (*self._seqs, *self._rows, self._slots, self._table, *self._writes, *self._tiles)))
+        self._args_at = ctypes.addressof(self._args)
         self._shape = None
         self.longest = self.shortest = 0
 
@@ -96,6 +108,8 @@ class StepMaps:
         self.write_seq, self.write_block = (t[:self.n_writes] for t in self._writes)
         self.tile_seq, self.tile_index = (t[:self.n_tiles] for t in self._tiles)
         self._shape = (seqs, rows)
+        a = self._args
+        a.n_seqs, a.n_rows, a.n_writes, a.n_tiles = seqs, rows, self.n_writes, self.n_tiles
         self._lists = StepLists(*(t.data_ptr() for t in (self.seq_q_start, self.seq_q_len, self.seq_kv_len, self.write_seq,
                                                          self.write_block, self.order, self.tile_seq,
                                                          self.tile_index)),
@@ -124,6 +138,6 @@ class StepMaps:
         if self._shape != (seqs, n_rows):
             self._arrays(seqs, n_rows)
         self.longest, self.shortest = int(longest), int(shortest)
-        _check(lib().llm_step_maps(cached.data_ptr(), q_len.data_ptr(), seqs, pages.data_ptr(), pages.numel(), n_rows, self.page_tokens,
-                                   self.group, self.tile_rows, self.few_rows, self.max_blocks, self.n_writes, self.n_tiles,
-                                   *self._out, stream if stream is not None else stream_handle()), "step_maps")
+        a = self._args
+        a.cached, a.q_len, a.pages, a.n_pages = cached.data_ptr(), q_len.data_ptr(), pages.data_ptr(), pages.numel()
+        _check(lib().llm_step_maps(self._args_at, stream if stream is not None else stream_handle()), "step_maps")

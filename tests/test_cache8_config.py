@@ -147,8 +147,9 @@ def test_a_launcher_turns_bad_sizes_away():
 
     assert prompt(cache(head_dim=128)) == 2 and prompt(cache(), splits=16) == 2 and prompt(cache(), box=32) == 2 and prompt(cache(), box=8) == 2
     assert prompt(cache(), scale=0.0) == 2 and prompt(cache(v=8208)) == 3
-    assert step_maps.lib().llm_step_maps(0, 0, 5000, 0, 0, 1, 16, 1, 128, 16, 1, 1, 1, *[0] * 12, 0) == 2
-    assert step_maps.lib().llm_step_maps(0, 0, 1, 0, 0, 1, 24, 1, 128, 16, 1, 1, 1, *[0] * 12, 0) == 2
+    for seqs, page in ((5000, 16), (1, 24), (1, 0)):
+        args = step_maps.MapsArgs(0, 0, seqs, 0, 0, 1, page, 1, 128, 16, 1, 1, 1, *[0] * 12)
+        assert step_maps.lib().llm_step_maps(ctypes.addressof(args), 0) == 2
     map_at = ctypes.addressof((ctypes.c_ubyte * 128)())
     for base, rows, box in ((4096, 1 << 40, 16), (4104, 64, 16), (4096, 0, 16), (4096, 64, 24), (4096, 64, 8)):
         assert cache8._prompt(64).llm_cache8_prompt_pool_map(map_at, base, rows, box) == 2

@@ -117,6 +117,16 @@ def test_step_maps_of_large_pools_and_short_tables():
     assert maps.block_table.tolist() == [[big, 5], [big - 1, -1]]
 
 
+def test_step_maps_of_lengths_that_are_not_the_steps():
+    """More rows than the step has are cut off at its end; pages that are not listed are not held."""
+    from bare_cuda_4gib_b200.kernels.step_maps import StepMaps
+    maps = StepMaps(20, 3, 4, 16, device=DEV)
+    maps.build(i32([3, 0, 7]), i32([5, 40, 6]), i32([4, 9]), 20, 20, 1)
+    assert maps.seq_q_start.tolist() == [0, 5, 25] and maps.seq_q_len.tolist() == [5, 15, 0] and maps.seq_kv_len.tolist() == [8, 15, 7]
+    assert maps.row_seq.tolist() == [0] * 5 + [1] * 15 and maps.slots.tolist() == [67, 68, 69, 70, 71] + [144 + i for i in range(15)]
+    assert maps.block_table.tolist() == [[4, -1, -1, -1], [9, -1, -1, -1], [-1] * 4]
+
+
 def test_step_maps_refuse():
     from bare_cuda_4gib_b200.errors import KernelLaunchError
     from bare_cuda_4gib_b200.kernels.step_maps import StepMaps
@@ -424,6 +434,40 @@ def test_pages_that_a_window_gave_back(dim):
 
 
 @pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("entry", [-1, -7, 2 ** 31 - 1, "first behind the pool"])
+def test_pages_outside_the_pool(dim, entry):
+    """A block whose entry of the table names no page of the pool: its positions are seen by no query, and the append writes nothing there."""
+    from bare_cuda_4gib_b200.kernels import cache8
+    from bare_cuda_4gib_b200.kernels.lib import Partials
+    requests, kept = [(200, 1), (150, 40), (300, 4), (64, 1), (70, 200)], []
+
+    def spoil(setup, plain):
+        kept.extend(plain)
+        setup.maps.table[:, 3] = setup.codes.shape[0] if isinstance(entry, str) else entry
+
+    setup, q, out = _attention(requests, 2, 4, dim, 16, seed=7, edit=spoil, check=False)
+    row = 0
+    for s, (c, n) in enumerate(requests):
+        k, v = (torch.cat([x[:, :48], x[:, 64:]], 1) for x in kept[s].values())      # [heads, positions, entries]
+        want, bound = pc.attention(q[row: row + n].double().cpu().view(n, 8, dim), k, v, c - 16, 1 / math.sqrt(dim), 0, 0, None, None)
+        off = (out[row: row + n].double().cpu().view(n, 8, dim) - want).abs() - (2.0 ** -8 * want.abs() + 2.0 ** -9 * bound)
+        assert (off <= 0).all(), s
+        row += n
+    requests = [(48, 3), (40, 20), (63, 1)]                # writes to blocks 2, 3 and (the second's) 3 again
+    setup = Setup(requests, 2, 4, dim, 16, seed=8)
+    setup.maps.table[:, 3] = setup.codes.shape[0] if isinstance(entry, str) else entry
+    before, scales = setup.codes.clone(), setup.scales.clone()
+    qkv = torch.randn(setup.rows, 12 * dim, device=DEV)
+    out = torch.zeros(setup.rows, 8 * dim, dtype=BF16, device=DEV)
+    cache8.append(Partials(qkv), out, setup.view, setup.maps, None, 8)
+    assert torch.equal(out, qkv[:, : 8 * dim].to(BF16))
+    page = setup.lists[1][2]                                # the one block that is held and written
+    others = [p for p in range(setup.codes.shape[0]) if p != page]
+    assert torch.equal(setup.codes[others], before[others]) and torch.equal(setup.scales[others].nan_to_num(-1), scales[others].nan_to_num(-1))
+    assert (setup.codes[page] != before[page]).any()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
 def test_scales_far_apart(dim):
     """Value blocks 2^20 apart and key blocks 2^12 apart, so that large and small ones meet in a row's sum and rows see small ones alone; values of
     1e30 and of 1e-28."""
@@ -434,6 +478,19 @@ def test_scales_far_apart(dim):
     _attention([(0, 1), (30, 1), (200, 1), (0, 100), (150, 70)], 2, 4, dim, 16, seed=1, keys=keys)
     _attention([(40, 1), (0, 90)], 2, 4, dim, 16, seed=2, keys=lambda k, v: (k, v * 1e30), check=True)
     _attention([(40, 1), (0, 90)], 2, 4, dim, 16, seed=2, keys=lambda k, v: (k, v * 1e-28), check=True)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("size", [1.0, 1e9, 1e16])
+def test_zeros_beside_large_values(dim, size):
+    """Three of four blocks hold values of zero (their scale is the least one) and keys of zero: many keys, each 2^-10 or so of the largest weight,
+    which add nothing to the output but their share of the sum."""
+    def keys(k, v):
+        holds = (torch.arange(k.shape[0])[:, None, None] // 16 % 4 == 1).double()
+        return k * holds * 4, v * holds * size
+
+    _attention([(900, 1), (30, 1), (500, 40), (0, 200), (100, 4)], 2, 4, dim, 16, seed=5, keys=keys)
+    _attention([(400, 1), (300, 90)], 2, 8, dim, 64, seed=6, window=130, keys=keys)
 
 
 @pytest.mark.parametrize("dim", [64, 128])
