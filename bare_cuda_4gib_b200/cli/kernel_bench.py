@@ -189,6 +189,8 @@ def bench_attention(a):
     ctx.max_q_len, ctx.max_kv_len = a.q_len, a.context
     q = torch.randn(rows, a.heads * a.head_dim, device="cuda").to(torch.bfloat16)
     out = torch.empty_like(q)
+    if a.cache_dtype == "float8_e4m3":
+        return _bench_attention_codes(a, storage, table, ctx, q, out)
     plan = fast.plan_for(a.head_dim, a.heads, a.kv_heads)
     scale = 1.0 / math.sqrt(a.head_dim)
     from ..kernels import gemm
@@ -200,6 +202,26 @@ def bench_attention(a):
     pairs = a.batch * (a.q_len * (a.context - a.q_len) + a.q_len * (a.q_len + 1) / 2)
     _report(f"attention batch={a.batch} q_len={a.q_len} context={a.context} heads={a.heads}/{a.kv_heads} d={a.head_dim}",
             us, kv_bytes + 2 * q.numel() * 2, 4.0 * a.heads * a.head_dim * pairs)
+
+
+def _bench_attention_codes(a, values, table, ctx, q, out):
+    """The same over a cache of e4m3 codes (scales of 2^-7)."""
+    import torch
+    from ..kernels import cache8, gemm
+    from ..kernels.step_maps import StepMaps
+    codes = (values.view(-1, 2, a.kv_heads, a.page, a.head_dim) * 128).to(cache8.DTYPE)
+    scales = torch.full((*codes.shape[:3], a.page // 16), 2.0 ** -7, device="cuda")
+    maps = StepMaps(q.shape[0], a.batch, table.shape[1], a.page, group=a.heads // a.kv_heads, tile_rows=cache8.tile_rows(a.head_dim),
+                    few_rows=cache8.FEW_ROWS)
+    maps.build(ctx.seq_kv_len - ctx.seq_q_len, ctx.seq_q_len, table.reshape(-1), q.shape[0], a.q_len, a.q_len)
+    view, scale = cache8.view(codes, scales, maps.table), 1.0 / math.sqrt(a.head_dim)
+    cache8.attention(q, out, view, maps, a.heads, scale)
+    gemm.check_errors()
+    us = _time(lambda: cache8.attention(q, out, view, maps, a.heads, scale), a.iters, a.warmup)
+    gemm.check_errors()
+    pairs = a.batch * (a.q_len * (a.context - a.q_len) + a.q_len * (a.q_len + 1) / 2)
+    _report(f"attention over e4m3 codes batch={a.batch} q_len={a.q_len} context={a.context} heads={a.heads}/{a.kv_heads} d={a.head_dim}",
+            us, a.batch * a.context * a.kv_heads * 2 * (a.head_dim + 4 / 16) + 2 * q.numel() * 2, 4.0 * a.heads * a.head_dim * pairs)
 
 
 def bench_norm(a):
@@ -265,6 +287,7 @@ def main(argv=None) -> int:
     for name, default in (("batch", 8), ("q-len", 1), ("context", 2048), ("heads", 32), ("kv-heads", 4),
                           ("head-dim", 64), ("page", 64)):
         t.add_argument(f"--{name}", type=int, default=default)
+    t.add_argument("--cache-dtype", default="bfloat16", choices=["bfloat16", "float8_e4m3"])
     n = sub.add_parser("norm", parents=[common])
     n.add_argument("--rows", type=int, default=2048)
     n.add_argument("--hidden", type=int, default=2048)

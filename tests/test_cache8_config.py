@@ -126,7 +126,7 @@ def test_a_launcher_turns_bad_sizes_away():
     at = ctypes.addressof(lists)
 
     def cache(**more):
-        c = dict(k=4096, v=8192, k_scale=0, v_scale=0, block_table=0, page_stride=4096, scale_stride=4, table_stride=1, page_tokens=16,
+        c = dict(k=4096, v=8192, k_scale=0, v_scale=0, block_table=0, page_stride=4096, scale_stride=4, n_pages=1, table_stride=1, page_tokens=16,
                  kv_heads=2, head_dim=64) | more
         return cache8._Cache8(*(c[name] for name, _ in cache8._Cache8._fields_))
 
