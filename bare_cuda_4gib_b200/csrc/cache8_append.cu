@@ -12,9 +12,9 @@
 // positions in registers (a thread 16 entries of each of one token), so they are read once, and it alone
 // settles the two scales: no atomics, no second pass.  The query heads that share the key/value head go through the same block:
 // their angles are the ones the keys need, computed once into shared memory; their first two rows are asked for together with the keys.
-// Bound by memory for prompts (projections in, queries out), by its trips to memory for decoding steps.  One B200, a call after
-// another from Python: 8 decoding requests (32 / 8 heads of 128) 13.2 us, 64 with three partial results (32 / 4 heads of 64) 13.6, a
-// prompt's 2,048 tokens 23.6 (1.95 TB/s).
+// Bound by memory for prompts (projections in, queries out), by its trips to memory for decoding steps.  One B200, in a graph: 8 decoding
+// requests (32 / 8 heads of 128) 2.4 us, 64 with three partial results (32 / 4 heads of 64) 4.1, a prompt's 2,048 tokens (32 / 8 heads of 128)
+// 9.2 (5.0 TB/s, most of it from L2).
 
 #include "cache8.cuh"
 
@@ -66,6 +66,23 @@ template <>
 __device__ __forceinline__ void load8<__nv_bfloat16, false>(float (&x)[8], const __nv_bfloat16* p, int n, long long stride) {
   load8_sum<__nv_bfloat16>(x, p, n, stride);
 }
+
+// The same eight entries on their way: as they were loaded where that is all there is to them, which takes half the registers.
+template <typename T, bool ONE>
+struct Eight {
+  float x[8];
+  __device__ __forceinline__ void load(const T* p, int n_partials, long long stride) { load8<T, ONE>(x, p, n_partials, stride); }
+  __device__ __forceinline__ void get(float (&y)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = x[i];
+  }
+};
+template <>
+struct Eight<__nv_bfloat16, true> {
+  uint4 raw;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p, int, long long) { raw = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void get(float (&y)[8]) const { load8<__nv_bfloat16, true>(y, reinterpret_cast<const __nv_bfloat16*>(&raw), 1, 0); }
+};
 
 // (lo, hi) turned by the angles of `cs` = (cos, sin) pairs.
 __device__ __forceinline__ void turn(float (&lo)[8], float (&hi)[8], const float2* cs) {
@@ -128,8 +145,10 @@ __device__ __forceinline__ uint4 bf16x8(const float (&x)[8]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// 896 threads an SM where there is one result to read (768: 2,048 tokens of 32 / 8 heads of 128 in 11.8 us instead of 9.2; 1,024: 9.7,
+// registers spilled), 768 with partial ones, which take more registers.
 template <int D, typename T, bool ONE>
-__global__ void __launch_bounds__(TOKENS * (D / 16), D == 128 ? 6 : 12) cache8_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(TOKENS * (D / 16), (D == 128 ? 1 : 2) * (ONE ? 7 : 6)) cache8_append_kernel(const AppendArgs a) {
   constexpr int CHUNKS = D / 16, HALF = D / 2, THREADS = TOKENS * CHUNKS, AHEAD = ONE ? 2 : 1;
   pdl_launch_dependents();
   __shared__ float2 angles[TOKENS][HALF];
@@ -181,15 +200,15 @@ __global__ void __launch_bounds__(TOKENS * (D / 16), D == 128 ? 6 : 12) cache8_a
   // the query heads of this key/value head: (head, token) pairs dealt to the groups of threads, tokens fastest, so that
   // a block with a single new token (a decoding request) turns up to 16 heads at once
   const int n_units = n_new * group;
-  float q_lo[AHEAD][8], q_hi[AHEAD][8];
+  Eight<T, ONE> q_lo[AHEAD], q_hi[AHEAD];
   auto load_queries = [&](int from) {
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       const int u = from + i * TOKENS;
       if (u >= n_units) break;
       const T* q = qkv + ((long long)(u % n_new) * n_heads + kvh * group + u / n_new) * D;
-      load8<T, ONE>(q_lo[i], q + 8 * c, a.n_partials, a.partial_stride);
-      load8<T, ONE>(q_hi[i], q + HALF + 8 * c, a.n_partials, a.partial_stride);
+      q_lo[i].load(q + 8 * c, a.n_partials, a.partial_stride);
+      q_hi[i].load(q + HALF + 8 * c, a.n_partials, a.partial_stride);
     }
   };
   auto store_queries = [&](int from) {
@@ -198,10 +217,12 @@ __global__ void __launch_bounds__(TOKENS * (D / 16), D == 128 ? 6 : 12) cache8_a
       const int u = from + i * TOKENS;
       if (u >= n_units) break;
       const int token = u % n_new, head = kvh * group + u / n_new;
-      if (a.inv_freq) turn(q_lo[i], q_hi[i], &angles[token][8 * c]);
+      float lo[8], hi[8];
+      q_lo[i].get(lo), q_hi[i].get(hi);
+      if (a.inv_freq) turn(lo, hi, &angles[token][8 * c]);
       __nv_bfloat16* out = a.q_out + ((row0 + token) * a.q_heads + head) * D;
-      *reinterpret_cast<uint4*>(out + 8 * c) = bf16x8(q_lo[i]);
-      *reinterpret_cast<uint4*>(out + HALF + 8 * c) = bf16x8(q_hi[i]);
+      *reinterpret_cast<uint4*>(out + 8 * c) = bf16x8(lo);
+      *reinterpret_cast<uint4*>(out + HALF + 8 * c) = bf16x8(hi);
     }
   };
   load_queries(group_of);
