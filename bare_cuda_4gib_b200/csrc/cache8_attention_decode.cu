@@ -27,7 +27,8 @@
 //    warps' states in shared memory and sends row r to block r % n_splits of the cluster, which merges in index order: no
 //    scratch in global memory, no atomics, no second launch.
 //  * Blocks of keys that lie wholly below the step's first new position are asked for before the kernel waits for the one before it.
-// One B200, 32 / 8 heads of 128: 8 requests of 8,192 positions 27.9 us (4.8 TB/s), 64 of 2,000 to 8,192 149.5 us (4.5 TB/s).
+// One B200, 32 / 8 heads of 128: 8 requests of 8,192 positions 24.1 us (5.6 TB/s, 0.86 of the copy rate; over a bfloat16 cache 44.7), 64 of 2,000
+// to 8,191 117 us (5.8 TB/s).  What is left is the start of a block (its lists, then its first pages, then its first keys) and its merge.
 
 #include "cache8.cuh"
 
@@ -176,11 +177,12 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&pool_map)) : "memory");
   }
   __syncwarp();
-  const int seq = a.ordered ? a.lists.order[blockIdx.x] : blockIdx.x, kvh = blockIdx.y;
+  const int seq = a.ordered ? a.lists.order[blockIdx.x] : blockIdx.x;
+  const int part = blockIdx.y / a.cache.kv_heads, kvh = blockIdx.y - part * a.cache.kv_heads, row0 = part * ROWS;   // row0: of the request's rows, this block's first
   const int group = a.q_heads / a.cache.kv_heads;
   const int q_start = a.lists.seq_q_start[seq], q_len = a.lists.seq_q_len[seq], kv_len = a.lists.seq_kv_len[seq], n_rows = q_len * group;
-  if (n_rows <= 0 || n_rows > FEW_ROWS) {                 // nothing, or the prompt kernel's: the same for the whole cluster
-    pdl_wait();
+  if (n_rows <= row0 || n_rows > FEW_ROWS) {              // nothing, or the prompt kernel's: the same for the whole cluster
+    if (blockIdx.x + blockIdx.y == 0) pdl_wait();      // (a kernel may not end ahead of those before it; the other blocks hold up none that has work)
     return;
   }
   if (smem_u32(ring) & 1023) {      // never seen; the swizzled blocks need it
@@ -252,7 +254,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
   int row_pos[NT][2], row_lo[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int R = n * 8 + g;
+    const int R = row0 + n * 8 + g;
     uint4 raw[KG][2];
 #pragma unroll
     for (int i = 0; i < KG; ++i) raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
@@ -277,7 +279,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
       qf[n][i >> 1][i & 1] = pack_half(__low2float(pairs[i]) * down, __high2float(pairs[i]) * down);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int col = 2 * t + h, C = n * 8 + col;
+      const int col = 2 * t + h, C = row0 + n * 8 + col;
       factor[n][h] = a.scale_log2 * power_of_two(__shfl_sync(0xffffffffu, e, col * 4));
       row_pos[n][h] = C < n_rows ? pos0 + C / group : -1;
       row_lo[n][h] = first_visible_key(row_pos[n][h], a.window, extras.chunk);
@@ -427,7 +429,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
   // ---- the block's warps merged, four channels a thread; row r goes to block r % n_splits
   for (int i = threadIdx.x; i < ROWS * (D / 4); i += THREADS) {
     const int r = i / (D / 4), c4 = i % (D / 4);
-    if (r >= n_rows) continue;
+    if (row0 + r >= n_rows) continue;
     float M = -INFINITY, L = 0.0f;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) M = fmaxf(M, st[((size_t)w * ROWS + r) * STATE + D]);
@@ -452,8 +454,8 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
   // ---- the rows this block owns, merged over the blocks in index order
   for (int i = threadIdx.x; i < owned_rows * (D / 4); i += THREADS) {
     const int slot = i / (D / 4), c4 = i % (D / 4), r = slot * n_splits + split;
-    if (r >= n_rows) continue;
-    const int token = r / group, head = kvh * group + r % group;
+    if (row0 + r >= n_rows) continue;
+    const int token = (row0 + r) / group, head = kvh * group + (row0 + r) % group;
     const float sink = sink_log2(extras, head);            // joins the row's sum here, once
     float M = sink;
 #pragma unroll 8
@@ -481,7 +483,7 @@ size_t smem_bytes(int rows, int n_splits) {
 }
 
 template <int NT>
-int launch(const CUtensorMap& map, const DecodeArgs& a, int n_splits, cudaStream_t stream) {
+int launch(const CUtensorMap& map, const DecodeArgs& a, int parts, int n_splits, cudaStream_t stream) {
   static unsigned long long met = 0;
   if (first_on_device(met)) {
     const int most = (int)(RING_BYTES + (8 * NT + 8) * STATE * 4 + WARPS * STAGES * 8);
@@ -490,7 +492,7 @@ int launch(const CUtensorMap& map, const DecodeArgs& a, int n_splits, cudaStream
       return met = 0, launch_status();
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.lists.n_seqs, a.cache.kv_heads, n_splits);
+  cfg.gridDim = dim3(a.lists.n_seqs, a.cache.kv_heads * parts, n_splits);
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = smem_bytes(8 * NT, n_splits);
   cfg.stream = stream;
@@ -550,16 +552,17 @@ extern "C" int llm_cache8_decode_pool_map(void* map_out, const void* base, long 
 }
 
 // Every request with 1 .. 16 packed rows (q_len * q_heads / kv_heads); the others' blocks return at once.  `rows`: the most packed rows
-// that such a request of the step brings (more than 8 take the kernel for 16).  n_splits (1, 2, 4 or 8) blocks share a
+// that such a request of the step brings.  More than 8 take the kernel for 16, or (`parts` 2) two blocks of the kernel for 8, of which
+// the second one of a request with no more than 8 returns at once.  n_splits (1, 2, 4 or 8) blocks share a
 // request's keys.  `ordered`: the longest requests' blocks start first
 // (worth its look-up where not all blocks run at once).  `pool_map`: llm_cache8_decode_pool_map over `pool_base`, in which the cache's codes lie.  chunk, sink, gate and gate_stride: `AttentionExtras`; 0 and null: none.
 extern "C" int llm_cache8_attention_decode(const void* q, void* out, const Cache8* cache, const void* pool_map, const void* pool_base,
-                                           const StepLists* lists, int n_splits, int ordered, int rows, int q_heads, float scale, int window, int chunk,
+                                           const StepLists* lists, int n_splits, int ordered, int rows, int parts, int q_heads, float scale, int window, int chunk,
                                            const float* sink, const void* gate, long long gate_stride, int* error_word,
                                            cudaStream_t stream) {
   if (lists->n_seqs <= 0) return 0;
   const Cache8& c = *cache;
-  if (c.head_dim != D || c.kv_heads <= 0 || q_heads <= 0 || q_heads % c.kv_heads || c.kv_heads > 65535 || c.page_tokens <= 0 ||
+  if (c.head_dim != D || c.kv_heads <= 0 || q_heads <= 0 || q_heads % c.kv_heads || c.kv_heads > 32767 || (parts != 1 && parts != 2) || c.page_tokens <= 0 ||
       c.page_tokens % SCALE_TOKENS || (n_splits != 1 && n_splits != 2 && n_splits != 4 && n_splits != 8) || rows < 1 || rows > FEW_ROWS)
     return ERR_BAD_SIZE;
   const uintptr_t all = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(c.k) |
@@ -571,5 +574,5 @@ extern "C" int llm_cache8_attention_decode(const void* q, void* out, const Cache
                v_off / D, *lists, q_heads, scale * 1.4426950408889634f, window, ordered, AttentionExtras{chunk, sink, gate, gate_stride}, error_word};
   CUtensorMap map;   // the caller's buffer need not be 64-byte aligned
   memcpy(&map, pool_map, sizeof(CUtensorMap));
-  return rows <= 8 ? launch<1>(map, a, n_splits, stream) : launch<2>(map, a, n_splits, stream);
+  return rows <= 8 || parts == 2 ? launch<1>(map, a, parts, n_splits, stream) : launch<2>(map, a, 1, n_splits, stream);
 }

@@ -31,8 +31,11 @@
 // the block get it; values are finite always, and behind the request's last key, or where no page is held, written as zeros.
 // Every mbarrier wait is bounded: on a timeout the thread sets the error word, all roles leave their loops, tensor memory is
 // released and the block returns.
-// One B200: a prompt of 2,048 tokens (32 / 4 heads of 64) 43.6 us, 2,048 tokens behind 2,048 (32 heads of 128) 117 us, 61 tokens behind 3,001
-// (32 / 8 heads of 128) 21.2 us.
+// One B200: a prompt of 2,048 tokens (32 / 4 heads of 64) 42.6 us, 2,048 tokens behind 2,048 (32 heads of 128) 118 us (0.88 PFLOP/s; over a
+// bfloat16 cache 137), 61 tokens behind 3,001 (32 / 8 heads of 128) 19.7 us (66).  What bounds it: a key block takes about 4,300 cycles for 256 rows,
+// of which the exponential unit is busy 1,540 and the tensor cores 1,000 to 2,000; the softmax warps (two a scheduler) wait for tensor-memory loads
+// and for their own chains of dependent instructions.  A block's start (queries staged: 7,000 cycles) and the merge of a cluster (9,000) weigh most
+// where there are few keys a block.
 
 #include "cache8.cuh"
 
@@ -355,8 +358,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
   // the most keys), then of the tile before it, ...
   const int tile = gridDim.y - 1 - blockIdx.y, kvh = blockIdx.x;
   const int seq = a.lists.tile_seq[tile];
-  if (seq < 0) {
-    pdl_wait();
+  if (seq < 0) {              // the end of the list; the blocks of its first entry stay for the kernels before (a kernel may not end ahead of them),
+    if (tile == 0) pdl_wait();  // the others hold up no block that has work
     return;
   }
   if (smem_u32(smem) & 1023) {   // never seen; refuse rather than compute with a broken layout

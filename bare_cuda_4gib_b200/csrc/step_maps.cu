@@ -17,8 +17,8 @@
 // the rows, table rows, blocks and tiles are dealt out over the grid.
 // It is an ordinary launch, not a dependent one: it waits for all kernels before it, and no kernel behind it
 // starts before it has ended, so kernels that read metadata ahead of their wait may read what it wrote.
-// One B200, a call after another from Python: 8 decoding requests 12.0 us, 256 requests of up to 30,000 positions beside four
-// prompts (3 MB of tables) 16.4 us.
+// One B200: 8 decoding requests 4.0 us in a graph (6.3 a call after another from Python), 256 requests of up to 30,000 positions beside four
+// prompts (3 MB of tables) 6.1 (8.2).
 
 #include "cache8.cuh"
 

@@ -22,6 +22,7 @@ DTYPE = torch.float8_e4m3fn
 HEAD_DIMS = (64, 128)
 FEW_ROWS = 16            # packed rows up to which the decode kernel takes a request
 KEY_BLOCK = 128          # positions that the prompt kernel takes at a time
+BLOCKS_AT_ONCE = {2: 148, 4: 132, 8: 120}     # of the prompt kernel on a B200, one an SM, by the size of a cluster (cudaOccupancyMaxActiveClusters)
 DECODE_WARPS = 8         # warps of a block of the decode kernel, which a request's scale blocks are dealt to
 _append_lib = None
 _decode_libs: Dict[int, object] = {}
@@ -56,7 +57,7 @@ def _decode(head_dim: int):
     if l is None:
         l = build.load_library("cache8_attention_decode.cu", (f"-DHEAD_DIM={head_dim}",))
         P, I, L, F = c_void_p, c_int, c_longlong, c_float
-        l.llm_cache8_attention_decode.argtypes = [P, P, P, P, P, P, I, I, I, I, F, I, I, P, P, L, P, P]
+        l.llm_cache8_attention_decode.argtypes = [P, P, P, P, P, P, I, I, I, I, I, F, I, I, P, P, L, P, P]
         l.llm_cache8_attention_decode.restype = c_int
         l.llm_cache8_decode_pool_map.argtypes = [P, P, L]
         l.llm_cache8_decode_pool_map.restype = c_int
@@ -205,9 +206,11 @@ def decode_splits(n_seqs: int, kv_heads: int, max_keys: int) -> int:
 
 @functools.lru_cache(maxsize=256)
 def prompt_splits(n_tiles: int, kv_heads: int, max_keys: int) -> int:
-    """How many blocks of the prompt kernel share a tile's keys: a power of two up to 8, as many as the SMs take at once."""
+    """How many blocks of the prompt kernel share a tile's keys: a power of two up to 8, as many as the SMs take at once in clusters of
+    that size (more start only when others have ended: 128 blocks by eights 27.6 us, by fours 64 of them 18.8), and none over four key blocks, where the
+    merge costs more than they save (389 tokens, 4 heads of 64, one block / two 11.9 / 13.4 us; behind 1,000 more 28.0 / 21.5)."""
     splits = 1
-    while splits < 8 and n_tiles * kv_heads * splits * 2 <= sm_count() and max_keys > splits * KEY_BLOCK:
+    while splits < 8 and n_tiles * kv_heads * splits * 2 <= BLOCKS_AT_ONCE[splits * 2] and max_keys > max(splits, 4) * KEY_BLOCK:
         splits *= 2
     return splits
 
@@ -234,9 +237,13 @@ def attention(q: torch.Tensor, out: torch.Tensor, cache: CacheView, maps: StepMa
     if maps.shortest * group <= FEW_ROWS:
         splits = decode_splits(maps.n_seqs, cache.kv_heads, launch.keys)
         ordered = 1 if maps.n_seqs * cache.kv_heads * splits > 2 * sm_count() else 0
+        # beside prompts only the shortest request is known: then most are taken to be like it, and one with more than 8 rows is read twice
+        parts = 2 if maps.longest * group > FEW_ROWS and maps.shortest * group <= FEW_ROWS // 2 else 1
         _check(launch.decode(q_at, out_at, launch.cache, launch.decode_map, cache.pool_ptr, maps.lists, splits, ordered,
-                             min(maps.longest * group, FEW_ROWS), q_heads, scale, window, *more, error_word, stream), "cache8_attention_decode")
+                             min(maps.longest * group, FEW_ROWS), parts, q_heads, scale, window, *more, error_word, stream), "cache8_attention_decode")
     if maps.longest * group > FEW_ROWS:
+        # the list of tiles has room for a last one of every request; taken as if all were like the longest they are fewer
+        tiles = min(maps.n_tiles, -(-maps.n_rows * -(-maps.longest * group // launch.tile_rows) // maps.longest))
         _check(launch.prompt(q_at, out_at, launch.cache, launch.prompt_map, cache.pool_ptr, launch.box_rows, maps.lists,
-                             prompt_splits(maps.n_tiles, cache.kv_heads, launch.keys), q_heads, scale, window, *more, error_word, stream),
+                             prompt_splits(tiles, cache.kv_heads, launch.keys), q_heads, scale, window, *more, error_word, stream),
                "cache8_attention_prompt")

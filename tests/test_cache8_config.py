@@ -137,7 +137,7 @@ def test_a_launcher_turns_bad_sizes_away():
     assert append(cache(), partials=0) == 2 and append(cache(), dtype=7) == 1 and append(cache(), qkv=4098) == 3 and append(cache(k=4100)) == 3
 
     def decode(c, splits=1, rows=4, q=4096):
-        return cache8._decode(64).llm_cache8_attention_decode(q, 4096, ctypes.addressof(c), 0, 4096, at, splits, 0, rows, 4, 0.125, 0, 0, 0, 0, 0, 0, 0)
+        return cache8._decode(64).llm_cache8_attention_decode(q, 4096, ctypes.addressof(c), 0, 4096, at, splits, 0, rows, 1, 4, 0.125, 0, 0, 0, 0, 0, 0, 0)
 
     assert decode(cache(head_dim=128)) == 2 and decode(cache(), splits=3) == 2 and decode(cache(), rows=17) == 2 and decode(cache(), q=4104) == 3
     assert decode(cache(k=1024)) == 3                                   # ahead of the pool's base

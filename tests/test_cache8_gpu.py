@@ -384,6 +384,14 @@ def test_decode_of_several_tokens(dim, group, each):
     _attention([(c, each) for c in (0, 1, 13, 16, 30, 100, 257)], 3, group, dim, 16, seed=each)
 
 
+@pytest.mark.parametrize("dim,group", [(64, 8), (128, 8), (64, 5), (128, 3), (128, 16), (64, 1)])
+@pytest.mark.parametrize("window", [0, 70])
+def test_few_rows_beside_prompts(dim, group, window):
+    """Requests of every number of packed rows up to 16 and just above beside prompts and idle rows: a block of 8 rows each, two for some."""
+    few = [(50 + 37 * n, n) for n in range(1, 18 // group + 2)]
+    _attention([(100, 1), (0, 90), *few, (-1, 1), (0, 1), (333, 1), (64, 20)], 2, group, dim, 32, seed=group, window=window, sink=True)
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("splits", [1, 2, 4, 8])
 def test_decode_long_and_split(monkeypatch, dim, splits):
