@@ -5,6 +5,7 @@
     bin/llm-kernel-bench attention --batch 8 --q-len 1 --context 2048 --heads 32 --kv-heads 4 --head-dim 64
     bin/llm-kernel-bench norm --rows 2048 --hidden 2048 --partials 1
     bin/llm-kernel-bench rope --rows 2048 --heads 32 --kv-heads 4 --head-dim 64
+    (attention and rope: --cache-dtype float8_e4m3 for a cache of e4m3 codes)
 
 It plays the part of the per-kernel table of cuongvng/bare-cuda-4gib's `llm-bench --kernels`
 (bench/src/bench_main.cc:208-254): time, achieved GB/s and TFLOP/s, and their fraction of the
@@ -252,8 +253,28 @@ def bench_rope(a):
     pos = torch.arange(a.rows, dtype=torch.int32, device="cuda")
     seq = torch.zeros(a.rows, dtype=torch.int32, device="cuda")
     inv = (1.0 / (10000.0 ** (torch.arange(d // 2, dtype=torch.float32) * 2.0 / d))).cuda()
+    if a.cache_dtype == "float8_e4m3":
+        return _bench_append_codes(a, page, table, qkv, q, inv)
     us = _time(lambda: K.rope_cache_write(K.Partials(qkv), q, view, pos, seq, inv, a.heads, True, a.rows), a.iters, a.warmup)
     _report(f"rope_cache_write rows={a.rows} heads={a.heads}/{a.kv_heads} d={d}", us, 2 * a.rows * width * 2, 0.0)
+
+
+def _bench_append_codes(a, page, table, qkv, q, inv):
+    """The same into a cache of e4m3 codes: a prompt's rows from position 0."""
+    import torch
+    from ..kernels import cache8
+    from ..kernels.lib import Partials
+    from ..kernels.step_maps import StepMaps
+    blocks, d = table.shape[1], a.head_dim
+    codes = torch.zeros(blocks, 2, a.kv_heads, page, d, device="cuda", dtype=torch.uint8)
+    scales = torch.zeros(*codes.shape[:3], page // 16, device="cuda")
+    maps = StepMaps(a.rows, 1, blocks, page, group=a.heads // a.kv_heads)
+    i32 = lambda x: torch.tensor([x], dtype=torch.int32, device="cuda")
+    maps.build(i32(0), i32(a.rows), table.reshape(-1), a.rows, a.rows, a.rows)
+    view = cache8.view(codes, scales, maps.table)
+    us = _time(lambda: cache8.append(Partials(qkv), q, view, maps, inv, a.heads), a.iters, a.warmup)
+    _report(f"append to e4m3 codes rows={a.rows} heads={a.heads}/{a.kv_heads} d={d}",
+            us, (qkv.numel() + q.numel()) * 2 + a.rows * a.kv_heads * 2 * (d + 4 / 16), 0.0)
 
 
 def main(argv=None) -> int:
@@ -295,6 +316,7 @@ def main(argv=None) -> int:
     r = sub.add_parser("rope", parents=[common])
     for name, default in (("rows", 2048), ("heads", 32), ("kv-heads", 4), ("head-dim", 64)):
         r.add_argument(f"--{name}", type=int, default=default)
+    r.add_argument("--cache-dtype", default="bfloat16", choices=["bfloat16", "float8_e4m3"])
     args = ap.parse_args(argv)
     GRAPH[0] = not args.no_graph
     {"gemm": bench_gemm, "gemv": bench_gemv, "attention": bench_attention, "norm": bench_norm, "rope": bench_rope}[args.kernel](args)

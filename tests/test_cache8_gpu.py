@@ -776,3 +776,41 @@ def test_engine_generates_and_reports(tmp_path, monkeypatch):
         LLMEngine(tmp_path, max_tokens=128, dtype="float32", cache_dtype="float8_e4m3")
     with pytest.raises(EngineError, match="e4m3"):
         LLMEngine(tmp_path, max_tokens=128, page_tokens=8, cache_dtype="float8_e4m3")
+
+
+def test_tools(tmp_path, monkeypatch):
+    """`llm-infer`, `llm-ppl` and `llm-kernel-bench` with such a cache, and the refusal of a float32 run."""
+    import json
+    import os
+    import pathlib
+    import subprocess
+    import sys
+    root = pathlib.Path(__file__).resolve().parents[1]
+
+    def run(tool, *args):
+        return subprocess.run([sys.executable, str(root / "bin" / tool), *map(str, args)], capture_output=True, text=True, timeout=600,
+                              env=dict(os.environ, PYTHONDONTWRITEBYTECODE="1"))
+
+    plain, pl = _engine_and_plain(tmp_path, monkeypatch, WIDE)
+    rng = random.Random(4)
+    prompt = [rng.randrange(515) for _ in range(40)]
+    args = ("--model", tmp_path, "--prompt", ",".join(map(str, prompt)), "--tokens", 9, "--cache-dtype", "float8_e4m3")
+    done = run("llm-infer", *args)
+    assert done.returncode == 0, done.stderr[-2000:]
+    tokens = [int(t) for t in next(line for line in done.stdout.splitlines() if line.startswith("generated:")).split(":")[1].split()]
+    logits = pl.forward_logits(plain, prompt + tokens[:-1])
+    assert len(tokens) == 9 and all(float(logits[39 + i].max() - logits[39 + i, t]) <= 3e-2 * float(logits[39 + i].abs().max()) for i, t in enumerate(tokens))
+    done = run("llm-infer", *args, "--dtype", "float32")
+    assert done.returncode == 1 and "bfloat16 runs" in done.stderr
+    (tmp_path / "text.ids").write_bytes(b"".join(rng.randrange(515).to_bytes(4, "little") for _ in range(140)))
+    args = ("--model", tmp_path, "--ids", tmp_path / "text.ids", "--ctx", 65, "--cache-dtype", "float8_e4m3")
+    done = run("llm-ppl", *args)
+    assert done.returncode == 0, done.stderr[-2000:]
+    done = run("llm-ppl", *args, "--dtype", "float32")
+    assert done.returncode == 1 and done.stderr.strip().splitlines()[-1].startswith("[llm] ") and "Traceback" not in done.stderr
+    for kernel, sizes, name in (("attention", ("--batch", 2, "--context", 100), "attention over e4m3 codes"), ("rope", ("--rows", 70), "append to e4m3 codes"),
+                                ("attention", ("--batch", 1, "--q-len", 50, "--context", 300, "--head-dim", 128, "--page", 16), "attention over e4m3 codes")):
+        done = run("llm-kernel-bench", kernel, *sizes, "--iters", 2, "--cache-dtype", "float8_e4m3")
+        assert done.returncode == 0, done.stderr[-2000:]
+        line = json.loads(done.stdout.strip().splitlines()[-1])
+        assert line["kernel"].startswith(name) and line["us"] > 0
