@@ -14,7 +14,7 @@
 // their angles are the ones the keys need, computed once into shared memory; their first two rows are asked for together with the keys.
 // Bound by memory for prompts (projections in, queries out), by its trips to memory for decoding steps.  One B200, in a graph: 8 decoding
 // requests (32 / 8 heads of 128) 2.4 us, 64 with three partial results (32 / 4 heads of 64) 4.1, a prompt's 2,048 tokens (32 / 8 heads of 128)
-// 9.2 (5.0 TB/s, most of it from L2).
+// 8.1 (5.7 TB/s, most of it from L2), 32,768 tokens 134 (5.5 TB/s).
 
 #include "cache8.cuh"
 
@@ -84,14 +84,17 @@ struct Eight<__nv_bfloat16, true> {
   __device__ __forceinline__ void get(float (&y)[8]) const { load8<__nv_bfloat16, true>(y, reinterpret_cast<const __nv_bfloat16*>(&raw), 1, 0); }
 };
 
-// (lo, hi) turned by the angles of `cs` = (cos, sin) pairs.
-__device__ __forceinline__ void turn(float (&lo)[8], float (&hi)[8], const float2* cs) {
+// (lo, hi) turned by the angles of `cs`: two (cos, sin) at a time, STEP apart.
+template <int STEP>
+__device__ __forceinline__ void turn(float (&lo)[8], float (&hi)[8], const float4* cs) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float a = lo[i], b = hi[i];
-    const float2 t = cs[i];
+  for (int i = 0; i < 8; i += 2) {
+    const float4 t = cs[i / 2 * STEP];
+    const float a = lo[i], b = hi[i], c = lo[i + 1], d = hi[i + 1];
     lo[i] = a * t.x - b * t.y;
     hi[i] = b * t.x + a * t.y;
+    lo[i + 1] = c * t.z - d * t.w;
+    hi[i + 1] = d * t.z + c * t.w;
   }
 }
 
@@ -145,13 +148,16 @@ __device__ __forceinline__ uint4 bf16x8(const float (&x)[8]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// 896 threads an SM where there is one result to read (768: 2,048 tokens of 32 / 8 heads of 128 in 11.8 us instead of 9.2; 1,024: 9.7,
+// 896 threads an SM where there is one result to read (768: 2,048 tokens of 32 / 8 heads of 128 in 11.8 us where this took 9.2; 1,024: 9.7,
 // registers spilled), 768 with partial ones, which take more registers.
 template <int D, typename T, bool ONE>
 __global__ void __launch_bounds__(TOKENS * (D / 16), (D == 128 ? 1 : 2) * (ONE ? 7 : 6)) cache8_append_kernel(const AppendArgs a) {
   constexpr int CHUNKS = D / 16, HALF = D / 2, THREADS = TOKENS * CHUNKS, AHEAD = ONE ? 2 : 1;
   pdl_launch_dependents();
-  __shared__ float2 angles[TOKENS][HALF];
+  // (cos, sin) of pairs 8 c + 2 k and 8 c + 2 k + 1 at [token][k][c], so that the threads of a token, and at head size 64 those of two, read side
+  // by side (pair after pair they would read a line in four turns: 8,192 tokens of 32 / 8 heads of 128 37.6 us, so 34.2; 32 / 4 heads of 64 15.8, 11.8)
+  constexpr int ROW = 4 * CHUNKS + (D == 64 ? 4 : 0);
+  __shared__ float4 angles[TOKENS][ROW];
   __shared__ float largest[2][THREADS / 32];
   const int tid = threadIdx.x, group_of = tid / CHUNKS, c = tid % CHUNKS, kvh = blockIdx.y;
   const int seq = a.lists.write_seq[blockIdx.x];
@@ -178,7 +184,8 @@ __global__ void __launch_bounds__(TOKENS * (D / 16), (D == 128 ? 1 : 2) * (ONE ?
       const float p = (float)(lo + i / HALF), f = a.inv_freq[i % HALF], hi = p * f, rest = fmaf(p, f, -hi);
       float s, co;
       sincosf(hi, &s, &co);
-      angles[i / HALF][i % HALF] = make_float2(fmaf(-rest, s, co), fmaf(rest, co, s));
+      const int pair = i % HALF;
+      reinterpret_cast<float2*>(&angles[i / HALF][pair % 8 / 2 * CHUNKS + pair / 8])[pair & 1] = make_float2(fmaf(-rest, s, co), fmaf(rest, co, s));
     }
   }
   __syncthreads();
@@ -219,7 +226,7 @@ __global__ void __launch_bounds__(TOKENS * (D / 16), (D == 128 ? 1 : 2) * (ONE ?
       const int token = u % n_new, head = kvh * group + u / n_new;
       float lo[8], hi[8];
       q_lo[i].get(lo), q_hi[i].get(hi);
-      if (a.inv_freq) turn(lo, hi, &angles[token][8 * c]);
+      if (a.inv_freq) turn<CHUNKS>(lo, hi, &angles[token][c]);
       __nv_bfloat16* out = a.q_out + ((row0 + token) * a.q_heads + head) * D;
       *reinterpret_cast<uint4*>(out + 8 * c) = bf16x8(lo);
       *reinterpret_cast<uint4*>(out + HALF + 8 * c) = bf16x8(hi);
@@ -228,7 +235,7 @@ __global__ void __launch_bounds__(TOKENS * (D / 16), (D == 128 ? 1 : 2) * (ONE ?
   load_queries(group_of);
   if (write) {        // the same for every thread of the block
     bool spoilt = false;
-    if (mine && a.inv_freq) turn(k_lo, k_hi, &angles[group_of][8 * c]);
+    if (mine && a.inv_freq) turn<CHUNKS>(k_lo, k_hi, &angles[group_of][c]);
     float k_most = fmaxf(largest_of(k_lo, spoilt), largest_of(k_hi, spoilt)), v_most = fmaxf(largest_of(v_lo, spoilt), largest_of(v_hi, spoilt));
     k_most = warp_max(k_most), v_most = warp_max(v_most);
     if ((tid & 31) == 0) largest[0][tid >> 5] = k_most, largest[1][tid >> 5] = v_most;
