@@ -15,7 +15,7 @@ import torch
 
 from . import build, gemm
 from ..errors import KernelLaunchError
-from .lib import AttentionExtras, CacheView, Partials, _check, _ptr, dtype_code, sm_count, stream_handle
+from .lib import AttentionExtras, CacheView, Partials, _check, _ptr, dtype_code, sm_count
 from .step_maps import SCALE_TOKENS, StepMaps
 
 DTYPE = torch.float8_e4m3fn
@@ -24,6 +24,7 @@ FEW_ROWS = 16            # packed rows up to which the decode kernel takes a req
 KEY_BLOCK = 128          # positions that the prompt kernel takes at a time
 BLOCKS_AT_ONCE = {2: 148, 4: 132, 8: 120}     # of the prompt kernel on a B200, one an SM, by the size of a cluster (cudaOccupancyMaxActiveClusters)
 DECODE_WARPS = 8         # warps of a block of the decode kernel, which a request's scale blocks are dealt to
+_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 _append_lib = None
 _decode_libs: Dict[int, object] = {}
 _prompt_libs: Dict[int, object] = {}
@@ -141,6 +142,7 @@ class _Launch:
                                                  _prompt(d).llm_cache8_attention_prompt)
         self.tile_rows, self.keys = tile_rows(d), cache.table_stride * cache.page_tokens
         self.device, self.table_rows = cache.block_table.get_device(), cache.block_table.shape[0]
+        self.error_word = gemm.error_word(cache.block_table.device).data_ptr()
 
 
 def _check_step(what: str, cache: CacheView, maps: StepMaps, q_heads: int, a: torch.Tensor, b: torch.Tensor) -> _Launch:
@@ -158,14 +160,13 @@ def _check_step(what: str, cache: CacheView, maps: StepMaps, q_heads: int, a: to
     index = maps.index
     if launch.device != index or a.get_device() != index or b.get_device() != index:
         raise KernelLaunchError(f"{what}: maps, cache and tensors must lie on one CUDA device")
-    if index != torch.cuda.current_device():
+    if index != _current_device():
         raise KernelLaunchError(f"{what}: the tensors lie on {maps.device}, the current device is cuda:{torch.cuda.current_device()}")
     return launch
 
 
 def _bf16_rows(t: torch.Tensor, rows: int, width: int) -> bool:
-    shape = t.shape
-    return t.dtype == torch.bfloat16 and shape[-1] == width and shape[0] >= rows and len(shape) == 2 and t.is_contiguous()
+    return t.dtype == torch.bfloat16 and t.dim() == 2 and t.size(1) == width and t.size(0) >= rows and t.is_contiguous()
 
 
 def append(qkv: Partials, q_out: torch.Tensor, cache: CacheView, maps: StepMaps, inv_freq: Optional[torch.Tensor], q_heads: int,
@@ -188,7 +189,7 @@ def append(qkv: Partials, q_out: torch.Tensor, cache: CacheView, maps: StepMaps,
         raise KernelLaunchError(f"cache8_append: the inverse frequencies must be {d // 2} contiguous float32 numbers")
     _check(launch.append(
         t.data_ptr(), dtype_code(t.dtype), qkv.n, qkv.stride, q_out.data_ptr(), launch.cache, maps.lists, _ptr(inv_freq), q_heads,
-        1 if write_cache else 0, stream if stream is not None else stream_handle()), "cache8_append")
+        1 if write_cache else 0, stream if stream is not None else _current_stream(maps.index)), "cache8_append")
 
 
 @functools.lru_cache(maxsize=256)
@@ -232,8 +233,8 @@ def attention(q: torch.Tensor, out: torch.Tensor, cache: CacheView, maps: StepMa
     if maps.few_rows != FEW_ROWS or maps.tile_rows != launch.tile_rows:
         raise KernelLaunchError(f"cache8_attention: the step's maps must be made with few_rows {FEW_ROWS} and tile_rows {launch.tile_rows}")
     more = extras.arguments(q_heads, q.dtype) if extras is not None else (0, 0, 0, 0)
-    stream = stream if stream is not None else stream_handle()
-    q_at, out_at, error_word, group = q.data_ptr(), out.data_ptr(), gemm.error_word(q.device).data_ptr(), maps.group
+    stream = stream if stream is not None else _current_stream(maps.index)
+    q_at, out_at, error_word, group = q.data_ptr(), out.data_ptr(), launch.error_word, maps.group
     if maps.shortest * group <= FEW_ROWS:
         splits = decode_splits(maps.n_seqs, cache.kv_heads, launch.keys)
         ordered = 1 if maps.n_seqs * cache.kv_heads * splits > 2 * sm_count() else 0
