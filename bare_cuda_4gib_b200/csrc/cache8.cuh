@@ -45,14 +45,11 @@ __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e 
 // The exponent of a normal positive power of two.
 __device__ __forceinline__ int exponent_of(float s) { return (__float_as_int(s) >> 23) - 127; }
 
-// Whether the current device is met for the first time (a kernel's attributes hold for one device); `met`: a bit a device.
-static inline bool first_on_device(unsigned long long& met) {
+// The current device's bit in the launchers' record of where a kernel's attributes are set (they hold for one device).
+static inline unsigned long long device_bit() {
   int device = 0;
   cudaGetDevice(&device);
-  const unsigned long long bit = 1ull << (device & 63);
-  const bool first = !(met & bit);
-  met |= bit;
-  return first;
+  return 1ull << (device & 63);
 }
 
 // The page that holds `position` (zero or more) of batch sequence `seq`, -1 if none does.

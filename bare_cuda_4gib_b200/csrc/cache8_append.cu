@@ -299,7 +299,7 @@ extern "C" int llm_cache8_append(const void* qkv, int in_dtype, int n_partials, 
   if (in_dtype != DT_F32 && in_dtype != DT_BF16) return ERR_BAD_DTYPE;
   const uintptr_t all = reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(c.k) |
                         reinterpret_cast<uintptr_t>(c.v) | (uintptr_t)c.page_stride;
-  if ((all & 15) || (n_partials > 1 && partial_stride % 4)) return ERR_BAD_ALIGN;
+  if ((all & 15) || (n_partials > 1 && partial_stride % (in_dtype == DT_F32 ? 4 : 8))) return ERR_BAD_ALIGN;
   AppendArgs a{qkv, n_partials, partial_stride, reinterpret_cast<__nv_bfloat16*>(q_out), c, *lists, inv_freq, q_heads, write_cache};
   if (c.head_dim == 64) return in_dtype == DT_F32 ? launch<64, float>(a, stream) : launch<64, __nv_bfloat16>(a, stream);
   return in_dtype == DT_F32 ? launch<128, float>(a, stream) : launch<128, __nv_bfloat16>(a, stream);

@@ -127,15 +127,15 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
       : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
   return ok != 0;
 }
-// Waits for a copy (about a second; then the error word is set and the warp goes on with what is there, to its barriers and its end).
-__device__ __forceinline__ void mbar_wait(uint64_t* bar, uint32_t parity, int* error_word) {
-  if (mbar_try_wait(bar, parity)) return;
+// Waits for a copy; false after about a second, with the error word set.
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* error_word) {
+  if (mbar_try_wait(bar, parity)) return true;
   const unsigned long long start = global_timer();
   for (unsigned spins = 0;; ++spins) {
-    if (mbar_try_wait(bar, parity)) return;
+    if (mbar_try_wait(bar, parity)) return true;
     if ((spins & 63u) == 63u && global_timer() - start > WAIT_LIMIT_NS) {
       atomicCAS(error_word, 0, ERR_DECODE);
-      return;
+      return false;
     }
   }
 }
@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
     const int ev = __shfl_sync(0xffffffffu, here.v_exponent, j & 31);
     const int later = j + STAGES;                          // the unit that takes this one's stage
     const int later_row = (later ^ j) & 32 ? __shfl_sync(0xffffffffu, ahead.row, later & 31) : __shfl_sync(0xffffffffu, here.row, later & 31);
-    mbar_wait(&my_full[j % STAGES], (uint32_t)(j / STAGES) & 1u, a.error_word);
+    const bool landed = mbar_wait(&my_full[j % STAGES], (uint32_t)(j / STAGES) & 1u, a.error_word);
     if (row < 0) {                  // a page that a window has given back: no row sees it
       __syncwarp();                 // (every lane has seen this phase)
       if (later < n_units) request(later, later_row);
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
         for (int n = 0; n < NT; ++n) mma_f16(w & 1 ? s_odd[n] : s[n], a0, a1, a2, a3, qf[n][i * 4 + w][0], qf[n][i * 4 + w][1]);
       }
     const bool all_visible = key0 + UNIT - 1 <= pos0 && key0 >= max_lo;
-    bool grown = false;
+    bool grown = !landed;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -346,6 +346,10 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
         grown |= v > m[n][h] + RESCALE_STEP;
       }
     if (__any_sync(0xffffffffu, grown)) {
+      if (!__all_sync(0xffffffffu, landed)) {      // the copies on their way land before the warp goes to its barriers and its end
+        for (int i = j; i < min(j + STAGES, n_units); ++i) mbar_wait(&my_full[i % STAGES], (uint32_t)(i / STAGES) & 1u, a.error_word);
+        break;
+      }
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -484,12 +488,14 @@ size_t smem_bytes(int rows, int n_splits) {
 
 template <int NT>
 int launch(const CUtensorMap& map, const DecodeArgs& a, int parts, int n_splits, cudaStream_t stream) {
-  static unsigned long long met = 0;
-  if (first_on_device(met)) {
+  static unsigned long long raised = 0;
+  const unsigned long long here = device_bit();
+  if (!(raised & here)) {
     const int most = (int)(RING_BYTES + (8 * NT + 8) * STATE * 4 + WARPS * STAGES * 8);
     if (cudaFuncSetAttribute(cache8_decode_kernel<NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess ||
         cudaFuncSetAttribute(cache8_decode_kernel<NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess)
-      return met = 0, launch_status();
+      return launch_status();
+    raised |= here;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.lists.n_seqs, a.cache.kv_heads * parts, n_splits);

@@ -959,11 +959,13 @@ extern "C" int llm_cache8_attention_prompt(const void* q, void* out, const Cache
   const long long v_off = reinterpret_cast<const char*>(c.v) - reinterpret_cast<const char*>(pool_base);
   if ((all & 15) || k_off < 0 || v_off < 0 || k_off % D || v_off % D || c.page_stride % D) return ERR_BAD_ALIGN;
   if (box_rows < SCALE_TOKENS || BN % box_rows || box_rows % SCALE_TOKENS || c.page_tokens % box_rows) return ERR_BAD_SIZE;
-  static unsigned long long met = 0;
-  if (first_on_device(met)) {
+  static unsigned long long raised = 0;
+  const unsigned long long here = device_bit();
+  if (!(raised & here)) {
     if (cudaFuncSetAttribute(cache8_prompt_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES) != cudaSuccess ||
         cudaFuncSetAttribute(cache8_prompt_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES) != cudaSuccess)
-      return met = 0, launch_status();
+      return launch_status();
+    raised |= here;
   }
   const AttnArgs a{reinterpret_cast<const __nv_bfloat16*>(q), reinterpret_cast<__nv_bfloat16*>(out), c, c.page_stride / D, k_off / D, v_off / D,
                    box_rows, *lists, q_heads,

@@ -165,10 +165,12 @@ extern "C" int llm_step_maps(const MapsArgs* args, cudaStream_t stream) {
       a.few_rows < 0 || a.n_rows < 0 || a.n_writes < 0 || a.n_tiles < 0 || a.n_pages < 0)
     return ERR_BAD_SIZE;
   const size_t smem = (size_t)5 * (a.n_seqs + 1) * 4;
-  static unsigned long long met = 0;
-  if (first_on_device(met)) {
+  static unsigned long long raised = 0;
+  const unsigned long long here = device_bit();
+  if (!(raised & here)) {
     if (cudaFuncSetAttribute(step_maps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 5 * (MAX_SEQS + 1) * 4) != cudaSuccess)
-      return met = 0, launch_status();
+      return launch_status();
+    raised |= here;
   }
   // four numbers a thread, one block an SM at most
   const long long numbers = (long long)a.n_rows + a.n_writes + a.n_tiles + (long long)a.n_seqs * a.max_blocks;

@@ -180,7 +180,8 @@ def append(qkv: Partials, q_out: torch.Tensor, cache: CacheView, maps: StepMaps,
     width, d = (q_heads + 2 * cache.kv_heads) * cache.head_dim, cache.head_dim
     launch = _check_step("cache8_append", cache, maps, q_heads, t, q_out)
     shape = t.shape
-    if shape[-1] != width or shape[-2] < maps.n_rows or t.stride(-1) != 1 or t.stride(-2) != width or (qkv.n > 1 and shape[0] < qkv.n):
+    if t.dim() not in (2, 3) or shape[-1] != width or shape[-2] < maps.n_rows or t.stride(-1) != 1 or t.stride(-2) != width or (
+            qkv.n != 1 and (qkv.n < 1 or t.dim() != 3 or shape[0] < qkv.n)):
         raise KernelLaunchError(f"cache8_append: projections of {tuple(shape)} for {maps.n_rows} dense rows of {width}")
     if not _bf16_rows(q_out, maps.n_rows, q_heads * d):
         raise KernelLaunchError(f"cache8_append: queries go to contiguous bfloat16 [rows, {q_heads * d}], not {tuple(q_out.shape)} of {q_out.dtype}")
@@ -228,11 +229,16 @@ def attention(q: torch.Tensor, out: torch.Tensor, cache: CacheView, maps: StepMa
     if not _bf16_rows(q, maps.n_rows, width) or not _bf16_rows(out, maps.n_rows, width):
         raise KernelLaunchError(f"cache8_attention: queries and outputs must be contiguous bfloat16 [{maps.n_rows} rows, {width}], not "
                                 f"{tuple(q.shape)} of {q.dtype} and {tuple(out.shape)} of {out.dtype}")
-    if not scale > 0.0 or window < 0:
+    if not 0.0 < scale < math.inf or window < 0:
         raise KernelLaunchError(f"cache8_attention: scale {scale} and window {window} are not supported (above zero; zero or more)")
     if maps.few_rows != FEW_ROWS or maps.tile_rows != launch.tile_rows:
         raise KernelLaunchError(f"cache8_attention: the step's maps must be made with few_rows {FEW_ROWS} and tile_rows {launch.tile_rows}")
-    more = extras.arguments(q_heads, q.dtype) if extras is not None else (0, 0, 0, 0)
+    more = (0, 0, 0, 0)
+    if extras is not None:
+        more = extras.arguments(q_heads, q.dtype)
+        if any(t is not None and t.get_device() != maps.index for t in (extras.sink, extras.gate)) or (
+                extras.gate is not None and (extras.gate.dim() != 2 or extras.gate.size(0) < maps.n_rows)):
+            raise KernelLaunchError(f"cache8_attention: sink and gate must lie on {maps.device}, the gate have two axes and {maps.n_rows} rows")
     stream = stream if stream is not None else _current_stream(maps.index)
     q_at, out_at, error_word, group = q.data_ptr(), out.data_ptr(), launch.error_word, maps.group
     if maps.shortest * group <= FEW_ROWS:

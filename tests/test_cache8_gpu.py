@@ -313,6 +313,12 @@ def test_append_refuses():
                                      (good.cpu(), q, setup.view, freq, 8), (torch.zeros(4, 24 * 64, device=DEV)[:, : 12 * 64], q, setup.view, freq, 8)):
         with pytest.raises(KernelLaunchError):
             cache8.append(Partials(t), out, view, setup.maps, inv, heads)
+    for n in (0, 2):           # two axes hold one result
+        with pytest.raises(KernelLaunchError):
+            cache8.append(Partials(good, n), q, setup.view, setup.maps, freq, 8)
+    parts = torch.zeros(2 * 4 * 12 * 64 + 4, dtype=BF16, device=DEV)        # partial results a whole number of 16 bytes apart, or refused
+    with pytest.raises(KernelLaunchError):
+        cache8.append(Partials(parts.as_strided((2, 4, 12 * 64), (4 * 12 * 64 + 4, 12 * 64, 1)), 2), q, setup.view, setup.maps, freq, 8)
     with pytest.raises(KernelLaunchError, match="have not been built"):
         from bare_cuda_4gib_b200.kernels.step_maps import StepMaps
         cache8.append(Partials(good), q, setup.view, StepMaps(4, 1, 1, 16, group=4, device=DEV), freq, 8)
@@ -552,6 +558,29 @@ def test_queries_that_are_no_numbers(dim):
     assert torch.equal(again[: setup.rows].view(setup.rows, 8, dim)[good], out[: setup.rows].view(setup.rows, 8, dim)[good])
 
 
+def test_pool_beyond_32_bits():
+    """The same pages at the end of a pool of 5 GB: the same outputs, and the same codes from the append."""
+    from bare_cuda_4gib_b200.kernels import cache8
+    from bare_cuda_4gib_b200.kernels.lib import Partials
+    requests = [(200, 1), (150, 40), (63, 2)]
+    setup, q, out = _attention(requests, 2, 4, 128, 64, seed=3, caches=1)
+    small, total = setup.codes.shape[0], (5 << 30) // (2 * 2 * 64 * 128)
+    codes = torch.empty((total, 2, 2, 64, 128), dtype=torch.uint8, device=DEV)
+    scales = torch.empty((total, 2, 2, 4), device=DEV)
+    codes[total - small:], scales[total - small:] = setup.codes[:, 0], setup.scales[:, 0]
+    near, table = setup.view, setup.maps.table
+    far_table = torch.where(table >= 0, table + (total - small), table)
+    far = cache8.view(codes, scales, far_table)
+    again = torch.zeros_like(out)
+    cache8.attention(q, again, far, setup.maps, 8, 1 / math.sqrt(128))
+    assert torch.equal(again[: setup.rows], out[: setup.rows])
+    qkv = torch.randn(setup.rows, 12 * 128, device=DEV) * 3
+    for view in (near, far):
+        cache8.append(Partials(qkv), again, view, setup.maps, None, 8)
+    assert torch.equal(codes[total - small:], setup.codes[:, 0])
+    assert torch.equal(scales[total - small:].nan_to_num(-1), setup.scales[:, 0].nan_to_num(-1))
+
+
 def test_attention_refuses():
     from bare_cuda_4gib_b200.errors import KernelLaunchError
     from bare_cuda_4gib_b200.kernels import cache8
@@ -562,7 +591,9 @@ def test_attention_refuses():
     wide = torch.zeros(4, 9 * 64, dtype=BF16, device=DEV)[:, 64:]
     for a, b, heads, scale, window, extras in ((q[:3], q, 8, 0.1, 0, None), (q, q[:3], 8, 0.1, 0, None), (q.float(), q, 8, 0.1, 0, None), (q, wide, 8, 0.1, 0, None),
                                                (q, q, 4, 0.1, 0, None), (q, q, 8, 0.0, 0, None), (q, q, 8, -1.0, 0, None), (q, q, 8, math.nan, 0, None),
-                                               (q, q, 8, 0.1, -1, None), (q.cpu(), q, 8, 0.1, 0, None), (q, q, 8, 0.1, 0, AttentionExtras(sink=torch.zeros(7, device=DEV)))):
+                                               (q, q, 8, 0.1, -1, None), (q.cpu(), q, 8, 0.1, 0, None), (q, q, 8, 0.1, 0, AttentionExtras(sink=torch.zeros(7, device=DEV))),
+                                               (q, q, 8, math.inf, 0, None), (q, q, 8, 0.1, 0, AttentionExtras(gate=torch.zeros(3, 8, dtype=BF16, device=DEV))),
+                                               (q, q, 8, 0.1, 0, AttentionExtras(gate=torch.zeros(8, dtype=BF16, device=DEV)))):
         with pytest.raises(KernelLaunchError):
             cache8.attention(a, b, setup.view, setup.maps, heads, scale, window, extras)
     other = StepMaps(4, 1, 1, 16, group=4, tile_rows=128, few_rows=16, device=DEV)
