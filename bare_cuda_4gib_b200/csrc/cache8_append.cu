@@ -13,7 +13,7 @@
 // settles the two scales: no atomics, no second pass.  The query heads that share the key/value head go through the same block:
 // their angles are the ones the keys need, computed once into shared memory; their first two rows are asked for together with the keys.
 // Bound by memory for prompts (projections in, queries out), by its trips to memory for decoding steps.  One B200, in a graph: 8 decoding
-// requests (32 / 8 heads of 128) 2.4 us, 64 with three partial results (32 / 4 heads of 64) 4.1, a prompt's 2,048 tokens (32 / 8 heads of 128)
+// requests (32 / 8 heads of 128) 2.4 us, 64 with three partial results (32 / 4 heads of 64) 3.3, a prompt's 2,048 tokens (32 / 8 heads of 128)
 // 8.1 (5.7 TB/s, most of it from L2), 32,768 tokens 134 (5.5 TB/s).
 
 #include "cache8.cuh"
@@ -35,53 +35,56 @@ struct AppendArgs {
   int q_heads, write_cache;
 };
 
-// Eight neighbouring entries of the sum of the partial results (ONE: there is one).
-template <typename T, bool ONE>
-__device__ __forceinline__ void load8(float (&x)[8], const T* p, int n_partials, long long stride);
-template <>
-__device__ __forceinline__ void load8<float, true>(float (&x)[8], const float* p, int, long long) {
+// Eight neighbouring entries.
+__device__ __forceinline__ void load8(float (&x)[8], const float* p) {
   const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
   x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
 }
-template <>
-__device__ __forceinline__ void load8<__nv_bfloat16, true>(float (&x)[8], const __nv_bfloat16* p, int, long long) {
+__device__ __forceinline__ void load8(float (&x)[8], const __nv_bfloat16* p) {
   const uint4 raw = *reinterpret_cast<const uint4*>(p);
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
 }
-template <typename T>
-__device__ __forceinline__ void load8_sum(float (&x)[8], const T* p, int n_partials, long long stride) {
-  load8<T, true>(x, p, 1, 0);
-  for (int i = 1; i < n_partials; ++i) {
-    float y[8];
-    load8<T, true>(y, p + i * stride, 1, 0);
+// N times eight entries of the sum of the partial results (ONE: there is one), a partial result's all on their way at once.
+template <typename T, bool ONE, int N>
+__device__ __forceinline__ void load_sums(float (&x)[N][8], const T* const (&p)[N], int n_partials, long long stride) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] += y[e];
+  for (int k = 0; k < N; ++k) load8(x[k], p[k]);
+  if (ONE) return;
+  for (int i = 1; i < n_partials; ++i) {
+    float y[N][8];
+#pragma unroll
+    for (int k = 0; k < N; ++k) load8(y[k], p[k] + i * stride);
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[k][e] += y[k][e];
   }
 }
-template <>
-__device__ __forceinline__ void load8<float, false>(float (&x)[8], const float* p, int n, long long stride) { load8_sum<float>(x, p, n, stride); }
-template <>
-__device__ __forceinline__ void load8<__nv_bfloat16, false>(float (&x)[8], const __nv_bfloat16* p, int n, long long stride) {
-  load8_sum<__nv_bfloat16>(x, p, n, stride);
-}
 
-// The same eight entries on their way: as they were loaded where that is all there is to them, which takes half the registers.
+// A query's two pieces on their way: as they were loaded where that is all there is to them, which takes half the registers.
 template <typename T, bool ONE>
-struct Eight {
-  float x[8];
-  __device__ __forceinline__ void load(const T* p, int n_partials, long long stride) { load8<T, ONE>(x, p, n_partials, stride); }
-  __device__ __forceinline__ void get(float (&y)[8]) const {
+struct Pieces {
+  float x[2][8];
+  __device__ __forceinline__ void load(const T* lo, const T* hi, int n_partials, long long stride) {
+    const T* const p[2] = {lo, hi};
+    load_sums<T, ONE>(x, p, n_partials, stride);
+  }
+  __device__ __forceinline__ void get(float (&lo)[8], float (&hi)[8]) const {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = x[i];
+    for (int i = 0; i < 8; ++i) lo[i] = x[0][i], hi[i] = x[1][i];
   }
 };
 template <>
-struct Eight<__nv_bfloat16, true> {
-  uint4 raw;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p, int, long long) { raw = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ void get(float (&y)[8]) const { load8<__nv_bfloat16, true>(y, reinterpret_cast<const __nv_bfloat16*>(&raw), 1, 0); }
+struct Pieces<__nv_bfloat16, true> {
+  uint4 raw[2];
+  __device__ __forceinline__ void load(const __nv_bfloat16* lo, const __nv_bfloat16* hi, int, long long) {
+    raw[0] = *reinterpret_cast<const uint4*>(lo), raw[1] = *reinterpret_cast<const uint4*>(hi);
+  }
+  __device__ __forceinline__ void get(float (&lo)[8], float (&hi)[8]) const {
+    load8(lo, reinterpret_cast<const __nv_bfloat16*>(&raw[0])), load8(hi, reinterpret_cast<const __nv_bfloat16*>(&raw[1]));
+  }
 };
 
 // (lo, hi) turned by the angles of `cs`: two (cos, sin) at a time, STEP apart.
@@ -149,9 +152,10 @@ __device__ __forceinline__ uint4 bf16x8(const float (&x)[8]) {
 }
 
 // 896 threads an SM where there is one result to read (768: 2,048 tokens of 32 / 8 heads of 128 in 11.8 us where this took 9.2; 1,024: 9.7,
-// registers spilled), 768 with partial ones, which take more registers.
+// registers spilled), 512 with partial ones, whose loads on their way take more (2,048 tokens with four results 33.3 us; 768 threads 34.0; a
+// piece's results one after another 54).
 template <int D, typename T, bool ONE>
-__global__ void __launch_bounds__(TOKENS * (D / 16), (D == 128 ? 1 : 2) * (ONE ? 7 : 6)) cache8_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(TOKENS * (D / 16), (D == 128 ? 1 : 2) * (ONE ? 7 : 4)) cache8_append_kernel(const AppendArgs a) {
   constexpr int CHUNKS = D / 16, HALF = D / 2, THREADS = TOKENS * CHUNKS, AHEAD = ONE ? 2 : 1;
   pdl_launch_dependents();
   // (cos, sin) of pairs 8 c + 2 k and 8 c + 2 k + 1 at [token][k][c], so that the threads of a token, and at head size 64 those of two, read side
@@ -195,27 +199,25 @@ __global__ void __launch_bounds__(TOKENS * (D / 16), (D == 128 ? 1 : 2) * (ONE ?
   const T* qkv = reinterpret_cast<const T*>(a.qkv) + row0 * n_heads * D;
   // ---- keys and values: token `group_of` of the new ones; pairs 8 c .. 8 c + 7 of the key, entries 16 c .. 16 c + 15 of the value
   const bool mine = write && group_of < n_new;
-  float k_lo[8] = {}, k_hi[8] = {}, v_lo[8] = {}, v_hi[8] = {};
+  float kv[4][8] = {};      // the key's two pieces, the value's
+  float (&k_lo)[8] = kv[0], (&k_hi)[8] = kv[1], (&v_lo)[8] = kv[2], (&v_hi)[8] = kv[3];
   if (mine) {
     const T* k = qkv + ((long long)group_of * n_heads + a.q_heads + kvh) * D;
     const T* v = k + (long long)a.cache.kv_heads * D;
-    load8<T, ONE>(k_lo, k + 8 * c, a.n_partials, a.partial_stride);
-    load8<T, ONE>(k_hi, k + HALF + 8 * c, a.n_partials, a.partial_stride);
-    load8<T, ONE>(v_lo, v + 16 * c, a.n_partials, a.partial_stride);
-    load8<T, ONE>(v_hi, v + 16 * c + 8, a.n_partials, a.partial_stride);
+    const T* const pieces[4] = {k + 8 * c, k + HALF + 8 * c, v + 16 * c, v + 16 * c + 8};
+    load_sums<T, ONE>(kv, pieces, a.n_partials, a.partial_stride);
   }
   // the query heads of this key/value head: (head, token) pairs dealt to the groups of threads, tokens fastest, so that
   // a block with a single new token (a decoding request) turns up to 16 heads at once
   const int n_units = n_new * group;
-  Eight<T, ONE> q_lo[AHEAD], q_hi[AHEAD];
+  Pieces<T, ONE> q_pieces[AHEAD];
   auto load_queries = [&](int from) {
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       const int u = from + i * TOKENS;
       if (u >= n_units) break;
       const T* q = qkv + ((long long)(u % n_new) * n_heads + kvh * group + u / n_new) * D;
-      q_lo[i].load(q + 8 * c, a.n_partials, a.partial_stride);
-      q_hi[i].load(q + HALF + 8 * c, a.n_partials, a.partial_stride);
+      q_pieces[i].load(q + 8 * c, q + HALF + 8 * c, a.n_partials, a.partial_stride);
     }
   };
   auto store_queries = [&](int from) {
@@ -225,7 +227,7 @@ __global__ void __launch_bounds__(TOKENS * (D / 16), (D == 128 ? 1 : 2) * (ONE ?
       if (u >= n_units) break;
       const int token = u % n_new, head = kvh * group + u / n_new;
       float lo[8], hi[8];
-      q_lo[i].get(lo), q_hi[i].get(hi);
+      q_pieces[i].get(lo, hi);
       if (a.inv_freq) turn<CHUNKS>(lo, hi, &angles[token][c]);
       __nv_bfloat16* out = a.q_out + ((row0 + token) * a.q_heads + head) * D;
       *reinterpret_cast<uint4*>(out + 8 * c) = bf16x8(lo);
