@@ -56,7 +56,7 @@ def run_once(engine, prompt, tokens, batch):
 def kernel_report(engine_factory, prompt, tokens, batch):
     """Device time of one request by kernel: every launcher call between two CUDA events."""
     import torch
-    from ..kernels import attention, gemm, gemv
+    from ..kernels import attention, cache8, gemm, gemv, step_maps
     from ..kernels import lib as K
 
     records = {}
@@ -81,7 +81,8 @@ def kernel_report(engine_factory, prompt, tokens, batch):
                                 (K, "argmax_rows", "argmax"), (K, "sample_rows", "sampling"),
                                 (K, "matmul_plain", "matmul (plain)"), (K, "attention_plain", "attention (plain)"),
                                 (gemm, "run", "matmul (tcgen05)"), (gemv, "run", "few-token product"),
-                                (attention, "run", "attention")]:
+                                (attention, "run", "attention"), (step_maps.StepMaps, "build", "step maps"),
+                                (cache8, "append", "append (codes)"), (cache8, "attention", "attention (codes)")]:
         saved.append((module, name, timed(module, name, label)))
     try:
         engine = engine_factory(False)

@@ -810,7 +810,7 @@ def test_engine_generates_and_reports(tmp_path, monkeypatch):
 
 
 def test_tools(tmp_path, monkeypatch):
-    """`llm-infer`, `llm-ppl` and `llm-kernel-bench` with such a cache, and the refusal of a float32 run."""
+    """`llm-infer`, `llm-ppl`, `llm-bench` and `llm-kernel-bench` with such a cache, and the refusal of a float32 run."""
     import json
     import os
     import pathlib
@@ -839,6 +839,9 @@ def test_tools(tmp_path, monkeypatch):
     assert done.returncode == 0, done.stderr[-2000:]
     done = run("llm-ppl", *args, "--dtype", "float32")
     assert done.returncode == 1 and done.stderr.strip().splitlines()[-1].startswith("[llm] ") and "Traceback" not in done.stderr
+    done = run("llm-bench", "--model", tmp_path, "--prompt-len", 40, "--tokens", 3, "--runs", 1, "--warmup", 1, "--batch", 2, "--kernels",
+               "--cache-dtype", "float8_e4m3")
+    assert done.returncode == 0 and all(f"  {label}  " in done.stdout for label in ("step maps", "append (codes)", "attention (codes)")), done.stderr[-2000:]
     for kernel, sizes, name in (("attention", ("--batch", 2, "--context", 100), "attention over e4m3 codes"), ("rope", ("--rows", 70), "append to e4m3 codes"),
                                 ("attention", ("--batch", 1, "--q-len", 50, "--context", 300, "--head-dim", 128, "--page", 16), "attention over e4m3 codes")):
         done = run("llm-kernel-bench", kernel, *sizes, "--iters", 2, "--cache-dtype", "float8_e4m3")
