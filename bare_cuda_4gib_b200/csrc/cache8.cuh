@@ -52,6 +52,11 @@ static inline unsigned long long device_bit() {
   return 1ull << (device & 63);
 }
 
+// What a sink (base-2 units) adds to a row's sum against the maximum m, infinite ones and rows without a maximum included.
+__device__ __forceinline__ float sink_share(float sink, float m) {
+  return sink == -INFINITY ? 0.0f : sink == INFINITY ? INFINITY : exp2f(sink - m);
+}
+
 // The page that holds `position` (zero or more) of batch sequence `seq`, -1 if none does.
 __device__ __forceinline__ int page_of(const Cache8& c, int seq, int position) {
   const int block = position / c.page_tokens;

@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
 #pragma unroll 8
     for (int z = 0; z < n_splits; ++z) M = fmaxf(M, recv[((size_t)z * owned_rows + slot) * STATE + D]);
     const float M_use = M == -INFINITY ? 0.0f : M;
-    float L = exp2f(sink - M_use);
+    float L = sink_share(sink, M_use);
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8
     for (int z = 0; z < n_splits; ++z) {

@@ -814,7 +814,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
       // at a time.  Heads that share a key/value head lie side by side in a token's output row, as their
       // rows do in the tile.  (The loads are warp-wide, so rows without an output still take part.)
       // the sink joins the sum, taken against the same maximum (far above it the sum is infinite, the row zero)
-      if (extras.sink && row_valid) l += exp2f(sink_log2(extras, head) - m);
+      if (extras.sink && row_valid) l += sink_share(sink_log2(extras, head), m);
       const float inv = l == 0.0f ? 0.0f : (row_valid ? head_gate<__nv_bfloat16>(extras, q_start + token, head) : 1.0f) / l;
       uint4* dst = reinterpret_cast<uint4*>(a.out + ((long long)(q_start + token) * a.q_heads + head) * D);
 #pragma unroll
@@ -881,7 +881,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
       const float M_use = M == -INFINITY ? 0.0f : M;
       const float h_mine = ml.x == -INFINITY ? 1.0f : exp2f(0.5f * (ml.x - M_use));      // without a maximum: zeros, or NaN to be handed on
       const float part_mine = ml.y * h_mine * h_mine, f_mine = h_mine * h_mine;
-      float L = exp2f(sink - M_use);
+      float L = sink_share(sink, M_use);
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int z = 0; z < MAX_SPLITS; ++z) {

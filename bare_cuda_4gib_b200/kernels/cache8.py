@@ -174,8 +174,8 @@ def append(qkv: Partials, q_out: torch.Tensor, cache: CacheView, maps: StepMaps,
     """Rows [q | k | v] of the step (`qkv`, dense, bfloat16 or float32, possibly a sum of partial results): q turned by
     position into `q_out` (bfloat16 [rows, q_heads * head size]), k turned by position and v into the cache (left alone unless
     `write_cache`).  `inv_freq` (float32 [head size / 2]) None: no rotation.  Positions of a written block that earlier steps filled
-    keep their numbers, but for a rounding where the new ones need a larger scale.  Rows of no request and idle ones are
-    left as they were in `q_out`."""
+    keep their numbers, but for a rounding where the new ones need a larger scale.  Requests may share pages that they read, not
+    pages that a step writes.  Rows of no request and idle ones are left as they were in `q_out`."""
     t = qkv.tensor
     width, d = (q_heads + 2 * cache.kv_heads) * cache.head_dim, cache.head_dim
     launch = _check_step("cache8_append", cache, maps, q_heads, t, q_out)

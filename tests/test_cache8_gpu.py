@@ -442,6 +442,25 @@ def test_windows_blocks_sinks_gates(dim, more):
 
 
 @pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("splits", [1, 4])
+def test_infinite_sinks(monkeypatch, dim, splits):
+    """A sink of -inf is none, one of +inf leaves nothing of its head, and a row without a key is zero whatever its sink."""
+    from bare_cuda_4gib_b200.kernels import cache8
+    from bare_cuda_4gib_b200.kernels.lib import AttentionExtras
+    monkeypatch.setattr(cache8, "prompt_splits", lambda *a: splits)
+    monkeypatch.setattr(cache8, "decode_splits", lambda *a: splits)
+    setup, q, out = _attention([(700, 1), (600, 60), (0, 1)], 2, 4, dim, 16, seed=9)
+    again, sinks = torch.zeros_like(out), torch.tensor([-math.inf, math.inf] * 4, device=DEV)
+    cache8.attention(q, again, setup.view, setup.maps, 8, 1 / math.sqrt(dim), 0, AttentionExtras(sink=sinks))
+    got, want = (x[: setup.rows].double().view(setup.rows, 8, dim) for x in (again, out))
+    assert (got[:, 1::2] == 0).all() and ((got - want)[:, ::2].abs() <= 2.0 ** -7 * want[:, ::2].abs() + 2.0 ** -12).all()
+    setup.maps.table.fill_(-1)
+    for sink in (None, sinks, torch.zeros(8, device=DEV)):
+        cache8.attention(q, again, setup.view, setup.maps, 8, 1 / math.sqrt(dim), 0, AttentionExtras(sink=sink) if sink is not None else None)
+        assert (again[: setup.rows] == 0).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
 def test_pages_that_a_window_gave_back(dim):
     """Blocks without a page in front of the window; the pool is full of NaN codes and scales."""
     _attention([(100, 1), (85, 3), (200, 40), (16, 1)], 2, 4, dim, 16, window=33, dropped=[4, 3, 10, 0])
