@@ -25,7 +25,7 @@ from ..weights.loader import load_weights, random_weights
 RUN_DTYPES = {"float32": torch.float32, "fp32": torch.float32, "bfloat16": torch.bfloat16, "bf16": torch.bfloat16}
 
 
-CACHE_DTYPES = {"float8_e4m3": torch.float8_e4m3fn, "e4m3": torch.float8_e4m3fn}
+CACHE_DTYPES = {"float8_e4m3": torch.float8_e4m3fn}
 
 
 def run_dtype(name) -> torch.dtype:
