@@ -246,15 +246,21 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+// Maxima that keep a NaN.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max2(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
 // 2^x for both of a pair without the exponential unit, which takes eight cycles a warp and is what the softmax would wait for: x = n + f with
 // n the nearest whole number (found by adding 1.5 * 2^23), 2^f by a polynomial that was fitted to it on [-1/2, 1/2] for the least
-// relative error (2.9e-6) with 1 at 0, n added to its exponent.  Up to x = -127: zero, as that exponent says of a one.  One pair of four goes
-// this way: the 7b portion below 122 -> 117 us.
+// relative error (2.9e-6) with 1 at 0, n added to its exponent.  Up to x = -127: zero, as that exponent says of a one.  A NaN becomes zero too:
+// the row's maximum keeps it.  One pair of four goes this way: the 7b portion below 122 -> 117 us.
 __device__ __forceinline__ void exp2_by_products(uint64_t x, float& p0, float& p1) {
   float a, b;
   unpair(x, a, b);
@@ -765,13 +771,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
               even = max3(even, __uint_as_float(w[k]), __uint_as_float(w[k + 1]));
               odd = max3(odd, __uint_as_float(w[k + 2]), __uint_as_float(w[k + 3]));
             }
-            const float most = max3(fmaxf(even, odd), __uint_as_float(w[SCALE_TOKENS - 2]), __uint_as_float(w[SCALE_TOKENS - 1]));
-            m_new = fmaxf(m_new, fmaf(most, c, ev));   // c > 0: the maximum commutes with it
+            const float most = max3(max2(even, odd), __uint_as_float(w[SCALE_TOKENS - 2]), __uint_as_float(w[SCALE_TOKENS - 1]));
+            m_new = max2(m_new, fmaf(most, c, ev));   // c > 0: the maximum commutes with it
             if (j & 1) tmem_store16(s_addr + h * S_PIECE + (j >> 1) * 16, packed);      // over the scores that they were made of
           }
           // tensor-memory loads and stores are warp-wide: the warp moves its maxima together, as soon as one of
-          // its rows has outgrown its own by the step (a row that has not may follow the true maximum just as well)
-          if (settled || !__any_sync(0xffffffffu, m_new > m + RESCALE_STEP)) {
+          // its rows has outgrown its own by the step (a row that has not may follow the true maximum just as well).  A row that
+          // sees a score that is no number has no number as its maximum either, and from here on as its sum.
+          if (settled || !__any_sync(0xffffffffu, !(m_new <= m + RESCALE_STEP))) {
             l2 = sum;
             break;
           }
@@ -803,6 +810,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
     float l_odd;
     unpair(l2, l, l_odd);
     l += l_odd;
+    if (m == INFINITY) l = __int_as_float(0x7fc00000);      // scores beyond float32
     if (ok && my_n > 0) ok = wait_pv(my_n - 1, 1) && !*abort_flag;
     if (!ok) {
       *abort_flag = 1;
