@@ -52,6 +52,7 @@ constexpr int VW = D / 32;                     // 32-bit words of a value that a
 constexpr int FEW_ROWS = 16;
 constexpr float RESCALE_STEP = 8.0f;           // base-2 units
 constexpr int FAR_VALUES = -40;
+constexpr float MOST_FACTOR = 3.40282347e38f;
 constexpr int UNIT_BYTES = UNIT * D;           // keys, or values, of one scale block
 constexpr int STAGES = D == 128 ? 3 : 6;       // scale blocks a warp has in flight: 96 KB a thread block, two of which share an SM
 constexpr int RING_BYTES = WARPS * STAGES * 2 * UNIT_BYTES;
@@ -331,13 +332,18 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
         for (int n = 0; n < NT; ++n) mma_f16(w & 1 ? s_odd[n] : s[n], a0, a1, a2, a3, qf[n][i * 4 + w][0], qf[n][i * 4 + w][1]);
       }
     const bool all_visible = key0 + UNIT - 1 <= pos0 && key0 >= max_lo;
+    float c[NT][2];       // infinite times a score of zero would be no number (a NaN of the keys' scale stays one)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) c[n][h] = factor[n][h] * ks, c[n][h] = c[n][h] > MOST_FACTOR ? MOST_FACTOR : c[n][h];
     bool grown = !landed;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int h = e & 1;
-        float v = fmaf(s[n][e] + s_odd[n][e], factor[n][h] * ks, (float)ev);
+        float v = fmaf(s[n][e] + s_odd[n][e], c[n][h], (float)ev);
         if (!all_visible) {
           const int key = key0 + key_of(g) + 8 * (e >> 1);
           if (key > row_pos[n][h] || key < row_lo[n][h]) v = -INFINITY;

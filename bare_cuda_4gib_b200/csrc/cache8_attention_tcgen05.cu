@@ -68,6 +68,9 @@ constexpr int S_PIECE = 64;      // columns of S a softmax thread holds in regis
 constexpr int TMEM_COLS = 512, O_COL = TILES * BN;
 constexpr unsigned long long WAIT_LIMIT_NS = 1000000000ull;
 constexpr float RESCALE_STEP = 8.0f;
+// What the factor of 16 scores is kept within: at 0 a hidden score (-inf) would be no longer hidden (2^-126 more changes none above 2^-102, and
+// ones below make nothing of any score), and an infinite factor times a score of zero would be no number.
+constexpr float LEAST_FACTOR = 1.17549435e-38f, MOST_FACTOR = 3.40282347e38f;
 constexpr int CHUNKS = D / 16;              // 16-byte chunks of a key's codes; also how many of them a converter thread takes of a tile
 constexpr int BLOCKS = BN / SCALE_TOKENS;   // scale blocks of a key block
 constexpr int MAX_SPLITS = 8;               // blocks that may share a tile's keys
@@ -748,7 +751,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
 #pragma unroll
           for (int j = 0; j < S_PIECE / SCALE_TOKENS; ++j) {
             const uint32_t* w = v + j * SCALE_TOKENS;
-            const float c = factor * of_block->key[h * 4 + j], ev = of_block->value[h * 4 + j], back = of_block->back[h * 4 + j];
+            const float c = fminf(fmaf(factor, of_block->key[h * 4 + j], LEAST_FACTOR), MOST_FACTOR), ev = of_block->value[h * 4 + j], back = of_block->back[h * 4 + j];
             const uint64_t c2 = pair(c, c), shift2 = pair(ev - m_use, ev - m_use);
             uint64_t part = 0;
 #pragma unroll

@@ -63,3 +63,42 @@ def test_queries_without_a_number_that_see_few_keys(monkeypatch, dim, splits, mo
     assert wrong.nonzero().tolist() == [[r, i % 8] for i, r in enumerate(rows)]
     good = ~wrong
     assert torch.equal(again[: setup.rows].view(setup.rows, 8, dim)[good], out[: setup.rows].view(setup.rows, 8, dim)[good])
+
+
+# ------------------------------------------------------------------------------ factors of the scores at the ends of float32's range
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("splits", [1, 4])
+@pytest.mark.parametrize("q_scale", [1e-20, 1e-30, 1e-37])
+def test_small_queries_over_keys_of_zero(monkeypatch, dim, splits, q_scale):
+    """A key block of zeros has the least scale, which times a small query's own is below float32: hidden keys stay hidden, the row is the
+    mean of the values that it sees."""
+    _split(monkeypatch, splits)
+
+    def keys(k, v):
+        return k * (torch.arange(k.shape[0])[:, None, None] // 16 % 3 == 1).double(), v
+
+    _attention([(0, 90), (100, 70), (30, 1), (64, 3)], 2, 4, dim, 16, seed=4, keys=keys, q_scale=q_scale)
+    _attention([(0, 90), (100, 70), (30, 1), (64, 3)], 2, 4, dim, 16, seed=4, keys=keys, q_scale=q_scale, window=20)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("splits", [1, 4])
+def test_large_queries_over_large_keys_that_are_hidden(monkeypatch, dim, splits):
+    """The first key is zero, the others so large that a query's scores of them are beyond float32: the first row sees only the zero, and is the
+    first value."""
+    from bare_cuda_4gib_b200.kernels import cache8
+    _split(monkeypatch, splits)
+    kept = []
+
+    def keys(k, v):
+        return k * (torch.arange(k.shape[0])[:, None, None] > 0).double() * 2.0 ** 100, v
+
+    requests = [(0, 30), (0, 2), (0, 3)]        # of the prompt kernel and of the decode kernel
+    setup, q, out = _attention(requests, 2, 4, dim, 16, seed=4, keys=keys, q_scale=2.0 ** 70, check=False, edit=lambda _s, plain: kept.extend(plain))
+    row = 0
+    for s, (_c, n) in enumerate(requests):
+        v = kept[s].values()[1][:, 0].repeat_interleave(4, 0)         # [heads, dim]
+        got = out[row].double().cpu().view(8, dim)
+        assert ((got - v).abs() <= (2.0 ** -8 + 2.0 ** -9) * v.abs()).all(), s
+        row += n
