@@ -19,9 +19,10 @@
 //                  running maximum and sum in float32 (base 2), write P as halves back into tensor memory.
 // The scales cost the softmax nothing but their constants: the keys' joins the factor of 16 scores, and a weight goes into P together with the
 // scale of its values: P = 2^(s + e_V - m) with m the running maximum of s + e_V, while the sum takes P 2^-e_V.  So a half of P is relative to
-// what the row's keys can add to its output, and O needs no factor of its own.  A block whose values are all below 2^-60 of the
-// largest so far (one of zeros, say, whose scale is the least one) would leave of such a P nothing to take a sum from; its values count as zeros and
-// its e_V as the largest so far.
+// what the row's keys can add to its output, and O needs no factor of its own.  Of a block whose values are all below 2^-60 of the
+// largest so far (one of zeros, say, whose scale is the least one) such a P may leave nothing to take a sum from: for those the sum takes 2^(s - m)
+// itself, a second exponential, where the maximum is moved (2 % for the code's presence; behind the first ones 4 %, in a loop of its own 8 %).
+// Larger values that are hidden from a row do not matter to it: the second way is right for any values.
 // m follows the true maximum only when that has grown by more than 2^8 (a half reaches 2^15), so O is rescaled rarely.
 // A half of P takes the columns of the scores it was made of (S 2 x 128, O 2 x head size columns of the 512), and the next key block's half of S is
 // issued when P has been read, while the softmax is at the other half: it waits for no product.
@@ -75,7 +76,7 @@ constexpr int CHUNKS = D / 16;              // 16-byte chunks of a key's codes; 
 constexpr int BLOCKS = BN / SCALE_TOKENS;   // scale blocks of a key block
 constexpr int MAX_SPLITS = 8;               // blocks that may share a tile's keys
 constexpr int KNOWN = 8;                    // key blocks whose scales are kept (a key tile's slot is free again at most five blocks on)
-constexpr int VALUE_RANGE = 60;             // how far below the largest exponent of a value scale another one counts (base 2)
+constexpr int VALUE_RANGE = 60;             // how far below the largest exponent of a value scale a sum still takes its part from P (base 2)
 constexpr int STATE = D + 4;                // floats of a row's state in a merge: D sums, the maximum, the sum
 constexpr size_t TILES_BYTES = (size_t)(TILES * 2 + K_SLOTS + C_SLOTS) * CODES + (size_t)V_SLOTS * VALUES;
 static_assert((size_t)BLOCK_ROWS * STATE * 4 <= TILES_BYTES, "the states of a merge lie over the tiles");
@@ -83,8 +84,8 @@ static_assert((size_t)BLOCK_ROWS * STATE * 4 <= TILES_BYTES, "the states of a me
 struct Scales {
   float key[BLOCKS];       // 2^e_K (1 where it is lost)
   float value[BLOCKS];     // e_V
-  float back[BLOCKS];      // 2^-e_V
-  uint32_t special, unused[3];   // bits b, 8 + b: scale block b has no number as its keys' scale, has no page
+  float back[BLOCKS];      // 2^-e_V; 0 where the sum takes its part another way
+  uint32_t special, unused[3];   // bits b, 8 + b, 16 + b: scale block b has no number as its keys' scale, has no page, has values far below others
 };
 
 // barriers (two to a slot, 14 of the groups, one to a block of scales), scales, rows' exponents, what is held, two words; 16 for alignment
@@ -286,6 +287,8 @@ __device__ __forceinline__ void halves(uint32_t codes, uint32_t& lo, uint32_t& h
   asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
       : "=r"(lo), "=r"(hi) : "r"(codes));
 }
+// The factor of 16 scores.
+__device__ __forceinline__ float score_factor(float of_row, float of_keys) { return fminf(fmaf(of_row, of_keys, LEAST_FACTOR), MOST_FACTOR); }
 // Two numbers as two e4m3 codes.
 __device__ __forceinline__ uint32_t codes2(float lo, float hi) {
   uint16_t d;
@@ -542,9 +545,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
     for (int jj = 0; jj < n_kb; ++jj) {
       int ev = now.row >= 0 ? max(exponent_of(now.v_scale), SCALE_LEAST) : SCALE_LEAST;      // (a scale that nothing has written is zero)
       most = max(most, __reduce_max_sync(0xffffffffu, ev));
-      const bool small = ev < most - VALUE_RANGE;
-      if (small) ev = most;
-      const uint32_t there = __ballot_sync(0xffffffffu, now.row >= 0 && !small), copies = __popc(__ballot_sync(0xffffffffu, leads && now.row >= 0));
+      if (now.row < 0) ev = most;
+      const bool far = ev < most - VALUE_RANGE;
+      const uint32_t there = __ballot_sync(0xffffffffu, now.row >= 0), copies = __popc(__ballot_sync(0xffffffffu, leads && now.row >= 0));
       const int ks = jj % K_SLOTS, cs = jj % C_SLOTS;
       ok = jj < K_SLOTS || mbar_wait(&k_empty[ks], (uint32_t)(jj / K_SLOTS - 1) & 1u, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
@@ -566,11 +569,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
       if (lane < BLOCKS) {
         to->key[lane] = now.row >= 0 && !lost ? fmaxf(now.k_scale, power_of_two(SCALE_LEAST)) : 1.0f;
         to->value[lane] = (float)ev;
-        to->back[lane] = power_of_two(-ev);
+        to->back[lane] = far ? 0.0f : power_of_two(-ev);
       }
+      const uint32_t all_far = __ballot_sync(0xffffffffu, far);
       const uint32_t all_lost = __ballot_sync(0xffffffffu, lost && now.row >= 0);
       const uint32_t all_absent = __ballot_sync(0xffffffffu, lane < BLOCKS && now.row < 0 && (kb_lo + jj) * BN + lane * SCALE_TOKENS < kv_len);
-      if (lane == 0) to->special = all_lost | all_absent << 8;
+      if (lane == 0) to->special = all_lost | all_absent << 8 | all_far << 16;
       __syncwarp();
       if (lane == 0) mbar_arrive(&known[jj % KNOWN]);
       now = next;
@@ -726,7 +730,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
         for (int k = 0; k < S_PIECE; k += 32) tmem_load32_nowait(s_addr + h * S_PIECE + k, v + k);
         tmem_wait_loads();
         const uint32_t special = of_block->special >> (h * 4);
-        if (special & 0x0f0fu) {
+        float limit = m + RESCALE_STEP;      // what a row's maximum may grow to before its sums follow
+        if (special & 0x0f0f0fu) {
+          if (special & 0x0f0000u) limit = __int_as_float(0x7fc00000);      // (they follow in any case)
 #pragma unroll
           for (int k = 0; k < S_PIECE; ++k) {
             if ((special >> (k / SCALE_TOKENS)) & 1u) v[k] = 0x7fc00000u;
@@ -751,7 +757,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
 #pragma unroll
           for (int j = 0; j < S_PIECE / SCALE_TOKENS; ++j) {
             const uint32_t* w = v + j * SCALE_TOKENS;
-            const float c = fminf(fmaf(factor, of_block->key[h * 4 + j], LEAST_FACTOR), MOST_FACTOR), ev = of_block->value[h * 4 + j], back = of_block->back[h * 4 + j];
+            const float c = score_factor(factor, of_block->key[h * 4 + j]), ev = of_block->value[h * 4 + j], back = of_block->back[h * 4 + j];
             const uint64_t c2 = pair(c, c), shift2 = pair(ev - m_use, ev - m_use);
             uint64_t part = 0;
 #pragma unroll
@@ -781,13 +787,23 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
           // tensor-memory loads and stores are warp-wide: the warp moves its maxima together, as soon as one of
           // its rows has outgrown its own by the step (a row that has not may follow the true maximum just as well).  A row that
           // sees a score that is no number has no number as its maximum either, and from here on as its sum.
-          if (settled || !__any_sync(0xffffffffu, !(m_new <= m + RESCALE_STEP))) {
+          if (settled || !__any_sync(0xffffffffu, !(m_new <= limit))) {
             l2 = sum;
             break;
           }
           const float down = m - (m_new == -INFINITY ? 0.0f : m_new), half_way = fast_exp2(0.5f * down), corr = fast_exp2(down);   // m = -inf gives 0
           m = m_new;
           l2 = fma2(fma2(l2, pair(half_way, half_way), 0), pair(half_way, half_way), 0);
+          const uint32_t far = of_block->special >> (16 + h * 4);
+          if (far & 0x0fu) {        // the shares of blocks whose values are far below others
+            const float m_use = m == -INFINITY ? 0.0f : m;
+            float share = 0.0f;
+#pragma unroll
+            for (int k = 0; k < S_PIECE; ++k)
+              if ((far >> (k / SCALE_TOKENS)) & 1u)
+                share += fast_exp2(fmaf(__uint_as_float(v[k]), score_factor(factor, of_block->key[h * 4 + k / SCALE_TOKENS]), -m_use));
+            l2 = add2(l2, pair(share, 0.0f));
+          }
           if (i > 0 || h > 0) {     // O = O * corr in tensor memory, when every product issued so far is complete
             ok = h > 0 ? wait_pv(i, 0) : wait_pv(i - 1, 1);
             if (!ok) break;

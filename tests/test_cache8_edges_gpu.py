@@ -102,3 +102,36 @@ def test_large_queries_over_large_keys_that_are_hidden(monkeypatch, dim, splits)
         got = out[row].double().cpu().view(8, dim)
         assert ((got - v).abs() <= (2.0 ** -8 + 2.0 ** -9) * v.abs()).all(), s
         row += n
+
+
+# ------------------------------------------------------------------------------ values far apart
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("splits", [1, 2, 4])
+@pytest.mark.parametrize("more", [dict(), dict(window=20), dict(chunk=48), dict(window=40, sink=True)])
+def test_small_values_count_for_rows_that_see_no_larger_ones(monkeypatch, dim, splits, more):
+    """Values of ordinary size between values 2^-72 of them: rows ahead of the ordinary ones, and rows whose window has left them behind, are made of
+    the small ones alone, rows that see both take the small ones' share of the sum into account."""
+    _split(monkeypatch, splits)
+
+    def keys(k, v):
+        ordinary = (torch.arange(k.shape[0])[:, None, None] // 16 % 8 == 3).double()
+        return k, v * torch.where(ordinary > 0, 1.0, 2.0 ** -72)
+
+    _attention([(0, 90), (100, 170), (0, 17), (30, 1), (44, 6), (300, 1)], 2, 4, dim, 16, seed=5, keys=keys, **more)
+    _attention([(500, 61), (0, 130)], 1, 8, dim, 64, seed=6, keys=keys, **more)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_later_tokens_change_no_earlier_row(dim):
+    """Behind them a token's values are 2^90 times as large or not: the rows are the same, but for a sum that is taken from other terms (2^-16 of
+    it at most), so that an output may be the other neighbour in bfloat16.  (Rows that see keys of the large values' own block are another
+    matter: the block's codes are off by 2^-10 of its scale.)"""
+    outs = []
+    for size in (1.0, 2.0 ** 90):
+        def keys(k, v):
+            return k, v * torch.where(torch.arange(k.shape[0])[:, None, None] >= 50, size, 1.0)
+
+        _setup, _q, out = _attention([(0, 60)], 2, 4, dim, 16, seed=7, keys=keys, check=size == 1.0)
+        outs.append(out[:48].double())
+    assert ((outs[0] - outs[1]).abs() <= 2.0 ** -7 * outs[0].abs()).all()
