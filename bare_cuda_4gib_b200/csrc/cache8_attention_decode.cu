@@ -14,8 +14,10 @@
 //    four at a time; of a value, the eight threads of a column take an eighth of the channels each.  Row g of the left operand is key
 //    g, or g ^ 4 for odd g: then the swizzled loads of keys and values meet every bank once (values of head size 64 twice).
 //  * A code becomes a half by one conversion for two; halves hold e4m3 exactly.  The scale of the keys joins the factor of
-//    the scores.  A weight goes into P together with its block's value scale: P = 2^(s + e_V - m) with m the running maximum of s + e_V,
-//    while the sum takes P 2^-e_V; so a half of P is relative to what the row's keys can add to its output, and O needs no factor.
+//    the scores.  A weight goes into P together with its block's value scale: P = 2^(s + e_V - m + 7) with m the running maximum of s + e_V,
+//    while the sum takes P 2^(-e_V - 7); so a half of P is relative to what the row's keys can add to its output, and O needs no factor but the 2^-7 at
+//    the end.  (The 2^7: weights keep a half's eleven bits down to 2^-21 of the row's largest, 15 nats below it, have an absolute step of 2^-31 of it from there on,
+//    and are lost from O below 2^-32.)
 //    Float32 drops a P below 2^-126, and with it a share of that times 2^(largest e_V - e_V) of the sum: nothing where e_V is of the size of the
 //    others', all of it for a block of zeros (e_V = -100) beside values in the millions.  Blocks with e_V below FAR_VALUES take 2^(s - m) itself, so
 //    that no share above 2^-26 is lost while the largest value is below 448 * 2^60.  (A test a block, which costs nothing here.)  For the same reason a
@@ -51,6 +53,9 @@ constexpr int TILES = D / 16;                  // 16-channel tiles of the output
 constexpr int VW = D / 32;                     // 32-bit words of a value that a thread takes (an eighth of its channels)
 constexpr int FEW_ROWS = 16;
 constexpr float RESCALE_STEP = 8.0f;           // base-2 units
+constexpr int HEADROOM = 7;                    // with the step above, what a half can hold over one: 2^15
+constexpr float P_UNIT = 1.0f / (1 << HEADROOM);
+static_assert(HEADROOM <= 126 - SCALE_MOST, "the sum takes 2^(-e_V - HEADROOM)");
 constexpr int FAR_VALUES = -40;
 constexpr float MOST_FACTOR = 3.40282347e38f;
 constexpr int UNIT_BYTES = UNIT * D;           // keys, or values, of one scale block
@@ -374,13 +379,13 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
     uint32_t pf[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const float m0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
+      const float m0 = m[n][0] == -INFINITY ? 0.0f : m[n][0] - HEADROOM, m1 = m[n][1] == -INFINITY ? 0.0f : m[n][1] - HEADROOM;
       const float p0 = fast_exp2(s[n][0] - m0), p1 = fast_exp2(s[n][1] - m1), p2 = fast_exp2(s[n][2] - m0), p3 = fast_exp2(s[n][3] - m1);
       if (ev >= FAR_VALUES) {       // the same for the whole warp
-        l[n][0] = fmaf(p0 + p2, power_of_two(-ev), l[n][0]);
-        l[n][1] = fmaf(p1 + p3, power_of_two(-ev), l[n][1]);
+        l[n][0] = fmaf(p0 + p2, power_of_two(-ev - HEADROOM), l[n][0]);
+        l[n][1] = fmaf(p1 + p3, power_of_two(-ev - HEADROOM), l[n][1]);
       } else {
-        const float e = (float)ev;
+        const float e = (float)(ev + HEADROOM);
         l[n][0] += fast_exp2(s[n][0] - e - m0) + fast_exp2(s[n][2] - e - m0);
         l[n][1] += fast_exp2(s[n][1] - e - m1) + fast_exp2(s[n][3] - e - m1);
       }
@@ -481,7 +486,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
       L += from[D + 1] * half_way * half_way;
       acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
     }
-    const float inv = L == 0.0f ? 0.0f : head_gate<__nv_bfloat16>(extras, q_start + token, head) / L;
+    const float inv = L == 0.0f ? 0.0f : head_gate<__nv_bfloat16>(extras, q_start + token, head) * P_UNIT / L;
     *reinterpret_cast<uint2*>(a.out + ((long long)(q_start + token) * a.q_heads + head) * D + c4 * 4) =
         make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
   }

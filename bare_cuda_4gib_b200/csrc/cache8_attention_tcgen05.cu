@@ -18,8 +18,10 @@
 //   softmax (8)    a group of four warps per tile, one thread per row.  First it stages Q_g.  Then, per half of 64 keys: read the row of S, mask,
 //                  running maximum and sum in float32 (base 2), write P as halves back into tensor memory.
 // The scales cost the softmax nothing but their constants: the keys' joins the factor of 16 scores, and a weight goes into P together with the
-// scale of its values: P = 2^(s + e_V - m) with m the running maximum of s + e_V, while the sum takes P 2^-e_V.  So a half of P is relative to
-// what the row's keys can add to its output, and O needs no factor of its own.  Of a block whose values are all below 2^-60 of the
+// scale of its values: P = 2^(s + e_V - m + 7) with m the running maximum of s + e_V, while the sum takes P 2^(-e_V - 7).  So a half of P is relative to
+// what the row's keys can add to its output, and O needs no factor of its own but the 2^-7 at the end.  The 2^7 is for rows of which one token takes
+// most of the weight: weights keep a half's eleven bits down to 2^-21 of the largest (15 nats below it),
+// have an absolute step of 2^-31 of it from there on, and are lost from O below 2^-32.  Of a block whose values are all below 2^-60 of the
 // largest so far (one of zeros, say, whose scale is the least one) such a P may leave nothing to take a sum from: for those the sum takes 2^(s - m)
 // itself, a second exponential, where the maximum is moved (2 % for the code's presence; behind the first ones 4 %, in a loop of its own 8 %).
 // Larger values that are hidden from a row do not matter to it: the second way is right for any values.
@@ -69,6 +71,9 @@ constexpr int S_PIECE = 64;      // columns of S a softmax thread holds in regis
 constexpr int TMEM_COLS = 512, O_COL = TILES * BN;
 constexpr unsigned long long WAIT_LIMIT_NS = 1000000000ull;
 constexpr float RESCALE_STEP = 8.0f;
+constexpr int HEADROOM = 7;      // with the step above, what a half can hold over one: 2^15
+constexpr float P_UNIT = 1.0f / (1 << HEADROOM);
+static_assert(HEADROOM <= 126 - SCALE_MOST, "the sum takes 2^(-e_V - HEADROOM)");
 // What the factor of 16 scores is kept within: at 0 a hidden score (-inf) would be no longer hidden (2^-126 more changes none above 2^-102, and
 // ones below make nothing of any score), and an infinite factor times a score of zero would be no number.
 constexpr float LEAST_FACTOR = 1.17549435e-38f, MOST_FACTOR = 3.40282347e38f;
@@ -84,7 +89,7 @@ static_assert((size_t)BLOCK_ROWS * STATE * 4 <= TILES_BYTES, "the states of a me
 struct Scales {
   float key[BLOCKS];       // 2^e_K (1 where it is lost)
   float value[BLOCKS];     // e_V
-  float back[BLOCKS];      // 2^-e_V; 0 where the sum takes its part another way
+  float back[BLOCKS];      // 2^(-e_V - HEADROOM); 0 where the sum takes its part another way
   uint32_t special, unused[3];   // bits b, 8 + b, 16 + b: scale block b has no number as its keys' scale, has no page, has values far below others
 };
 
@@ -569,7 +574,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
       if (lane < BLOCKS) {
         to->key[lane] = now.row >= 0 && !lost ? fmaxf(now.k_scale, power_of_two(SCALE_LEAST)) : 1.0f;
         to->value[lane] = (float)ev;
-        to->back[lane] = far ? 0.0f : power_of_two(-ev);
+        to->back[lane] = far ? 0.0f : power_of_two(-ev - HEADROOM);
       }
       const uint32_t all_far = __ballot_sync(0xffffffffu, far);
       const uint32_t all_lost = __ballot_sync(0xffffffffu, lost && now.row >= 0);
@@ -750,7 +755,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
         // The exponentials are taken against the maximum so far while the scores' own is being found, which needs them only when it has
         // outgrown the other by the step: then they are taken again (twice or so for a row of many blocks).
         for (bool settled = false;; settled = true) {
-          const float m_use = m == -INFINITY ? 0.0f : m;
+          const float m_use = m == -INFINITY ? 0.0f : m - HEADROOM;
           float m_new = m;
           uint64_t sum = l2;
           uint32_t packed[16];
@@ -837,12 +842,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
     }
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (n_splits == 1 && ok && my_n > 0) {
-      // ---- every thread finishes its own row: O / l out of tensor memory, rounded to bfloat16, 64 bytes
+      // ---- every thread finishes its own row: O / l (less the headroom) out of tensor memory, rounded to bfloat16, 64 bytes
       // at a time.  Heads that share a key/value head lie side by side in a token's output row, as their
       // rows do in the tile.  (The loads are warp-wide, so rows without an output still take part.)
       // the sink joins the sum, taken against the same maximum (far above it the sum is infinite, the row zero)
       if (extras.sink && row_valid) l += sink_share(sink_log2(extras, head), m);
-      const float inv = l == 0.0f ? 0.0f : (row_valid ? head_gate<__nv_bfloat16>(extras, q_start + token, head) : 1.0f) / l;
+      const float inv = l == 0.0f ? 0.0f : (row_valid ? head_gate<__nv_bfloat16>(extras, q_start + token, head) : 1.0f) * P_UNIT / l;
       uint4* dst = reinterpret_cast<uint4*>(a.out + ((long long)(q_start + token) * a.q_heads + head) * D);
 #pragma unroll
       for (int c0 = 0; c0 < D; c0 += 32) {
@@ -916,7 +921,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) cache8_prompt_kernel(const __g
         L += part;
         acc.x += v[z].x * f, acc.y += v[z].y * f, acc.z += v[z].z * f, acc.w += v[z].w * f;
       }
-      const float inv = L == 0.0f ? 0.0f : head_gate<__nv_bfloat16>(extras, q_start + tok, hd) / L;
+      const float inv = L == 0.0f ? 0.0f : head_gate<__nv_bfloat16>(extras, q_start + tok, hd) * P_UNIT / L;
       if (there)
         *reinterpret_cast<uint2*>(a.out + ((long long)(q_start + tok) * a.q_heads + hd) * D + c4 * 4) =
             make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));

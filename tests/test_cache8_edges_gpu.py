@@ -135,3 +135,40 @@ def test_later_tokens_change_no_earlier_row(dim):
         _setup, _q, out = _attention([(0, 60)], 2, 4, dim, 16, seed=7, keys=keys, check=size == 1.0)
         outs.append(out[:48].double())
     assert ((outs[0] - outs[1]).abs() <= 2.0 ** -7 * outs[0].abs()).all()
+
+
+# ------------------------------------------------------------------------------ one token that takes most of the weight
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("splits", [1, 4])
+@pytest.mark.parametrize("sink", [False, True])
+def test_a_first_token_that_takes_most_of_the_weight(monkeypatch, dim, splits, sink):
+    """Its value is next to nothing, so that the other tokens, each 8 to 20 nats below it, make the output.  A weight is a half in units of 2^-7 of
+    the row's largest or more: where it lies below the half's normal range it is off by at most 2^-25 of that, 2^-32 of the largest weight."""
+    from bare_cuda_4gib_b200.kernels import cache8
+    from bare_cuda_4gib_b200.kernels.lib import AttentionExtras
+    _split(monkeypatch, splits)
+    kept, requests = [], [(0, 1), (2000, 1), (500, 3), (1500, 40), (0, 200)]
+
+    def keys(k, v):
+        t = torch.arange(k.shape[0])[:, None, None]
+        u = torch.rand(v.shape, generator=torch.Generator().manual_seed(3), dtype=torch.float64)
+        return torch.where(t == 0, 2.0, 0.0) + 0 * k, torch.where(t == 0, 2.0 ** -9, 1 + 0.7 * u)
+
+    setup, _q, out = _attention(requests, 2, 4, dim, 16, seed=1, keys=keys, check=False, edit=lambda _s, plain: kept.extend(plain))
+    gen = torch.Generator().manual_seed(5)
+    gap = 8 + 12 * torch.rand(setup.rows, 8, 1, generator=gen)                       # nats
+    q = (gap / (2 * math.sqrt(dim)) * (0.5 + torch.rand(setup.rows, 8, dim, generator=gen))).view(setup.rows, -1).to(BF16).to(DEV)
+    sinks = (torch.rand(8, generator=gen) * 20).to(DEV) if sink else None
+    again = torch.zeros_like(out)
+    cache8.attention(q, again, setup.view, setup.maps, 8, 1 / math.sqrt(dim), 0, AttentionExtras(sink=sinks) if sink else None)
+    row = 0
+    for s, (c, n) in enumerate(requests):
+        k, v = kept[s].values()
+        want, bound = pc.attention(q[row: row + n].double().cpu().view(n, 8, dim), k, v, c, 1 / math.sqrt(dim), 0, 0, sinks.double().cpu() if sink else None, None)
+        got = again[row: row + n].double().cpu().view(n, 8, dim)
+        # (the sum of a row's weights is at least the largest of them)
+        lost = 2.0 ** -32 * v.abs().sum(1).repeat_interleave(4, 0)
+        off = (got - want).abs() - (2.0 ** -8 * want.abs() + 2.0 ** -9 * bound + lost)
+        assert (off <= 0).all(), (s, float(((got - want).abs() / want.abs()).max()))
+        row += n
