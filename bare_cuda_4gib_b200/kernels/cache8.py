@@ -118,6 +118,7 @@ def view(codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, i
                     DTYPE, codes.data_ptr(), codes.numel(), k_scale_ptr=s, v_scale_ptr=s + per_cache_scales // 2 * 4,
                     scale_stride=caches * per_cache_scales)
     out.keeps = (codes, scales)
+    gemm.error_word(codes.device)      # made here, so that a captured call, if it is the first, need not
     return out
 
 

@@ -18,7 +18,7 @@ from .lib import DT_BF16, DT_F32, AddTo, glu_defines, LazyNorm, Partials, Prenor
 BM, BK = 128, 64
 SPLIT_MAX_ROWS = 256          # steps with more rows never split K
 _libs = {}
-_error_word: Optional[torch.Tensor] = None
+_error_words: Dict[torch.device, torch.Tensor] = {}
 
 
 def lib(activation: str = "silu"):
@@ -45,18 +45,19 @@ def lib(activation: str = "silu"):
 
 
 def error_word(device) -> torch.Tensor:
-    global _error_word
-    if _error_word is None:
-        _error_word = torch.zeros(1, dtype=torch.int32, device=device)
-    return _error_word
+    """The word of the device that its kernels report to."""
+    word = _error_words.get(device)
+    if word is None:
+        word = _error_words[device] = torch.zeros(1, dtype=torch.int32, device=device)
+    return word
 
 
 def check_errors() -> None:
-    """Reads the device error word (synchronises); raises if a kernel gave up on a wait."""
-    if _error_word is not None:
-        code = int(_error_word.item())
+    """Reads the devices' error words (synchronises); raises if a kernel gave up on a wait."""
+    for word in _error_words.values():
+        code = int(word.item())
         if code:
-            _error_word.zero_()
+            word.zero_()
             role = {1: "gemm TMA producer", 2: "gemm MMA issuer", 3: "gemm epilogue", 11: "attention loader",
                     12: "attention MMA issuer", 13: "attention softmax",
                     14: "attention (shared memory not 1024-byte aligned)", 21: "few-token product, producer",

@@ -154,3 +154,18 @@ def test_a_launcher_turns_bad_sizes_away():
     for base, rows, box in ((4096, 1 << 40, 16), (4104, 64, 16), (4096, 0, 16), (4096, 64, 24), (4096, 64, 8)):
         assert cache8._prompt(64).llm_cache8_prompt_pool_map(map_at, base, rows, box) == 2
     assert cache8._decode(64).llm_cache8_decode_pool_map(map_at, 4096, 1 << 31) == 2
+
+
+def test_every_device_has_an_error_word_of_its_own(monkeypatch):
+    """What a kernel reports to lies on its own device; a report on any of them is found, once."""
+    from bare_cuda_4gib_b200.errors import KernelLaunchError
+    from bare_cuda_4gib_b200.kernels import gemm
+    monkeypatch.setattr(gemm, "_error_words", {}, raising=False)
+    monkeypatch.setattr(gemm, "_error_word", None, raising=False)
+    first, second = (gemm.error_word(d) for d in (torch.device("cpu"), torch.device("cpu", 0)))
+    assert first is not second and gemm.error_word(torch.device("cpu", 0)) is second
+    gemm.check_errors()
+    second.fill_(46)
+    with pytest.raises(KernelLaunchError, match="decode attention over 8-bit codes"):
+        gemm.check_errors()
+    gemm.check_errors()

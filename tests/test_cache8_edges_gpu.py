@@ -172,3 +172,22 @@ def test_a_first_token_that_takes_most_of_the_weight(monkeypatch, dim, splits, s
         off = (got - want).abs() - (2.0 ** -8 * want.abs() + 2.0 ** -9 * bound + lost)
         assert (off <= 0).all(), (s, float(((got - want).abs() / want.abs()).max()))
         row += n
+
+
+# ------------------------------------------------------------------------------ a captured call that is the first one
+
+def test_a_view_makes_what_a_captured_call_reports_to(monkeypatch):
+    """A graph that made the error word itself would set it to zero at every replay."""
+    from bare_cuda_4gib_b200.kernels import cache8, gemm
+    from test_cache8_gpu import Setup
+    monkeypatch.setattr(gemm, "_error_words", {})
+    setup = Setup([(40, 1)], 2, 4, 64, 16)
+    assert list(gemm._error_words) == [setup.codes.device]
+    word = gemm._error_words[setup.codes.device]
+    q = torch.zeros(1, 8 * 64, dtype=BF16, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache8.attention(q, q, setup.view, setup.maps, 8, 0.125)
+    word.fill_(46)
+    graph.replay()
+    assert gemm._error_words[setup.codes.device] is word and int(word) == 46
