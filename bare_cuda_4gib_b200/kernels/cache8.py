@@ -23,6 +23,7 @@ HEAD_DIMS = (64, 128)
 FEW_ROWS = 16            # packed rows up to which the decode kernel takes a request
 KEY_BLOCK = 128          # positions that the prompt kernel takes at a time
 BLOCKS_AT_ONCE = {2: 148, 4: 132, 8: 120}     # of the prompt kernel on a B200, one an SM, by the size of a cluster (cudaOccupancyMaxActiveClusters)
+LEAST_SCALE, MOST_SCALE = 2.0 ** -126, 2.0 ** 127      # of the scores: what float32 has
 DECODE_WARPS = 8         # warps of a block of the decode kernel, which a request's scale blocks are dealt to
 _current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 _append_lib = None
@@ -230,8 +231,9 @@ def attention(q: torch.Tensor, out: torch.Tensor, cache: CacheView, maps: StepMa
     if not _bf16_rows(q, maps.n_rows, width) or not _bf16_rows(out, maps.n_rows, width):
         raise KernelLaunchError(f"cache8_attention: queries and outputs must be contiguous bfloat16 [{maps.n_rows} rows, {width}], not "
                                 f"{tuple(q.shape)} of {q.dtype} and {tuple(out.shape)} of {out.dtype}")
-    if not 0.0 < scale < math.inf or window < 0:
-        raise KernelLaunchError(f"cache8_attention: scale {scale} and window {window} are not supported (above zero; zero or more)")
+    if not LEAST_SCALE <= scale < MOST_SCALE or not 0 <= window < 1 << 31 or extras is not None and not 0 <= extras.chunk < 1 << 31:
+        raise KernelLaunchError(f"cache8_attention: scale {scale}, window {window} and blocks of {extras.chunk if extras is not None else 0} are not "
+                                f"supported (above zero; zero or more; in 32 bits)")
     if maps.few_rows != FEW_ROWS or maps.tile_rows != launch.tile_rows:
         raise KernelLaunchError(f"cache8_attention: the step's maps must be made with few_rows {FEW_ROWS} and tile_rows {launch.tile_rows}")
     more = (0, 0, 0, 0)

@@ -191,3 +191,35 @@ def test_a_view_makes_what_a_captured_call_reports_to(monkeypatch):
     word.fill_(46)
     graph.replay()
     assert gemm._error_words[setup.codes.device] is word and int(word) == 46
+
+
+# ------------------------------------------------------------------------------ bounds beyond 32 bits
+
+@pytest.mark.parametrize("window,chunk,scale", [(1 << 31, 0, 0.125), ((1 << 32) + 5, 0, 0.125), (0, 1 << 31, 0.125), (0, (1 << 32) + 16, 0.125), (0, -16, 0.125),
+                                                (0, 0, 1e-50), (0, 0, 1e39)])
+def test_bounds_and_scales_beyond_32_bits_are_refused(window, chunk, scale):
+    """They went to the kernel modulo 2^32, as zero or as infinity: a window of 2^32 + 5 positions was one of 5."""
+    from bare_cuda_4gib_b200.errors import KernelLaunchError
+    from bare_cuda_4gib_b200.kernels import cache8
+    from bare_cuda_4gib_b200.kernels.lib import AttentionExtras
+    setup, q, out = _attention([(40, 1), (0, 30)], 2, 4, 64, 16)
+    with pytest.raises(KernelLaunchError, match="in 32 bits"):
+        cache8.attention(q, out, setup.view, setup.maps, 8, scale, window, AttentionExtras(chunk) if chunk else None)
+    again = torch.zeros_like(out)
+    most = (1 << 31) - 1
+    for args in ((most, None), (0, AttentionExtras(most))):
+        cache8.attention(q, again, setup.view, setup.maps, 8, 1 / 8, *args)
+        assert torch.equal(again[: setup.rows], out[: setup.rows])
+
+
+# ------------------------------------------------------------------------------ twice
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_call_repeats_itself(dim):
+    """The same call twice, also split over a cluster: the same to the bit."""
+    from bare_cuda_4gib_b200.kernels import cache8
+    setup, q, out = _attention([(2000, 1), (700, 3), (1500, 61), (0, 300)], 2, 4, dim, 16, window=900, sink=False)
+    for _ in range(5):
+        again = torch.zeros_like(out)
+        cache8.attention(q, again, setup.view, setup.maps, 8, 1 / math.sqrt(dim), 900)
+        assert torch.equal(again[: setup.rows], out[: setup.rows])
