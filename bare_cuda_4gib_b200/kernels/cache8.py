@@ -92,6 +92,12 @@ def prepare(head_dim: int) -> None:
     _append(), _decode(head_dim), _prompt(head_dim)
 
 
+def _check_table(table: torch.Tensor) -> None:
+    # (in a part of a wider table a request longer than the part would find its neighbours' entries, or what lies behind the table)
+    if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
+        raise KernelLaunchError("cache8: the block table must be contiguous int32 with two axes")
+
+
 def view(codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, index: int = 0) -> CacheView:
     """The cache that lies in `codes` (uint8 or float8_e4m3fn, [pages, (caches,) keys | values, kv heads, page tokens, head size])
     and `scales` (float32, [pages, (caches,) keys | values, kv heads, page tokens / 16]): with caches, the one at `index`."""
@@ -108,14 +114,13 @@ def view(codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, i
     if not supports(head_dim, None, page_tokens):
         raise KernelLaunchError(f"cache8: head size {head_dim} in pages of {page_tokens} positions is not supported (head sizes "
                                 f"{HEAD_DIMS}, pages of a multiple of {SCALE_TOKENS})")
+    _check_table(block_table)
     if not codes.is_cuda or scales.device != codes.device or block_table.device != codes.device:
         raise KernelLaunchError("cache8: codes, scales and block table must lie on one CUDA device")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
-        raise KernelLaunchError("cache8: the block table must be int32 with dense rows")
     per_cache, per_cache_scales = 2 * kv_heads * page_tokens * head_dim, 2 * kv_heads * (page_tokens // SCALE_TOKENS)
     k = codes.data_ptr() + index * per_cache
     s = scales.data_ptr() + index * per_cache_scales * 4
-    out = CacheView(k, k + per_cache // 2, block_table, caches * per_cache, block_table.stride(0), page_tokens, kv_heads, head_dim,
+    out = CacheView(k, k + per_cache // 2, block_table, caches * per_cache, block_table.shape[1], page_tokens, kv_heads, head_dim,
                     DTYPE, codes.data_ptr(), codes.numel(), k_scale_ptr=s, v_scale_ptr=s + per_cache_scales // 2 * 4,
                     scale_stride=caches * per_cache_scales)
     out.keeps = (codes, scales)
@@ -130,6 +135,7 @@ class _Launch:
     def __init__(self, cache: CacheView):
         if cache.dtype != DTYPE:
             raise KernelLaunchError(f"cache8: a cache of {cache.dtype} is not one of e4m3 codes")
+        _check_table(cache.block_table)
         d = cache.head_dim
         self._struct = _Cache8(cache.k_ptr, cache.v_ptr, cache.k_scale_ptr, cache.v_scale_ptr, cache.block_table.data_ptr(),
                                cache.page_stride, cache.scale_stride, cache.pool_elems // cache.page_stride, cache.table_stride, cache.page_tokens,

@@ -169,3 +169,21 @@ def test_every_device_has_an_error_word_of_its_own(monkeypatch):
     with pytest.raises(KernelLaunchError, match="decode attention over 8-bit codes"):
         gemm.check_errors()
     gemm.check_errors()
+
+
+def test_a_view_refuses_parts_of_tables():
+    """A request longer than its table's columns must find no page there; in a part of a wider table it would find the neighbouring columns', and
+    behind the last row what lies behind the table."""
+    from bare_cuda_4gib_b200.errors import KernelLaunchError
+    from bare_cuda_4gib_b200.kernels import cache8
+    from bare_cuda_4gib_b200.kernels.lib import CacheView
+    codes, scales = torch.zeros(4, 2, 1, 16, 64, dtype=torch.uint8), torch.zeros(4, 2, 1, 1)
+    table = torch.zeros(3, 8, dtype=torch.int32)
+    for part in (table[:, 2:], table[:, :4], table.t(), table[::2], table[0], table.long(), table[:1].expand(3, 8)):
+        with pytest.raises(KernelLaunchError, match="block table must be contiguous"):
+            cache8.view(codes, scales, part)
+        with pytest.raises(KernelLaunchError, match="block table must be contiguous"):      # a view made by a cache's manager, at its first use
+            cache8._Launch(CacheView(0, 0, part, 4096, 8, 16, 1, 64, cache8.DTYPE))
+    for whole in (table, table[:2], table[1:2]):
+        with pytest.raises(KernelLaunchError, match="one CUDA device"):
+            cache8.view(codes, scales, whole)
