@@ -14,7 +14,7 @@
 // their angles are the ones the keys need, computed once into shared memory; their first two rows are asked for together with the keys.
 // Bound by memory for prompts (projections in, queries out), by its trips to memory for decoding steps.  One B200, in a graph: 8 decoding
 // requests (32 / 8 heads of 128) 2.4 us, 64 with three partial results (32 / 4 heads of 64) 3.3, a prompt's 2,048 tokens (32 / 8 heads of 128)
-// 8.1 (5.7 TB/s, most of it from L2), 32,768 tokens 134 (5.5 TB/s).
+// 8.3 (5.6 TB/s, most of it from L2), 32,768 tokens 136 (5.4 TB/s).
 
 #include "cache8.cuh"
 
@@ -183,13 +183,16 @@ __global__ void __launch_bounds__(TOKENS * (D / 16), (D == 128 ? 1 : 2) * (ONE ?
   const long long at = (long long)page * a.cache.page_stride + ((long long)kvh * a.cache.page_tokens + in_page) * D;
   const long long scale_at = (long long)page * a.cache.scale_stride + (long long)kvh * (a.cache.page_tokens / TOKENS) + in_page / TOKENS;
   if (a.inv_freq) {
-    // the angle's product in two parts, p f = hi + lo exactly, sin(hi + lo) = sin hi + lo cos hi: far positions keep their angle
+    // The angle's product in two parts, p f = hi + lo exactly: far positions keep their angle.  lo is at most half a step of hi, 1/2 at 2^24, to which
+    // positions are float32 numbers; its sine and cosine by their series, off by 1.6e-6 there and by 1e-8 up to 2^22.
     for (int i = tid; i < n_new * HALF; i += THREADS) {
       const float p = (float)(lo + i / HALF), f = a.inv_freq[i % HALF], hi = p * f, rest = fmaf(p, f, -hi);
+      const float r2 = rest * rest, rs = rest * fmaf(r2, fmaf(r2, 1.0f / 120, -1.0f / 6), 1.0f),
+                  rc = fmaf(r2, fmaf(r2, fmaf(r2, -1.0f / 720, 1.0f / 24), -0.5f), 1.0f);
       float s, co;
       sincosf(hi, &s, &co);
       const int pair = i % HALF;
-      reinterpret_cast<float2*>(&angles[i / HALF][pair % 8 / 2 * CHUNKS + pair / 8])[pair & 1] = make_float2(fmaf(-rest, s, co), fmaf(rest, co, s));
+      reinterpret_cast<float2*>(&angles[i / HALF][pair % 8 / 2 * CHUNKS + pair / 8])[pair & 1] = make_float2(co * rc - s * rs, s * rc + co * rs);
     }
   }
   __syncthreads();

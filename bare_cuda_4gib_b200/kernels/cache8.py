@@ -24,6 +24,7 @@ FEW_ROWS = 16            # packed rows up to which the decode kernel takes a req
 KEY_BLOCK = 128          # positions that the prompt kernel takes at a time
 BLOCKS_AT_ONCE = {2: 148, 4: 132, 8: 120}     # of the prompt kernel on a B200, one an SM, by the size of a cluster (cudaOccupancyMaxActiveClusters)
 LEAST_SCALE, MOST_SCALE = 2.0 ** -126, 2.0 ** 127      # of the scores: what float32 has
+MOST_POSITIONS = 1 << 24       # that angles are taken for: float32 has their numbers
 DECODE_WARPS = 8         # warps of a block of the decode kernel, which a request's scale blocks are dealt to
 _current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 _append_lib = None
@@ -196,6 +197,8 @@ def append(qkv: Partials, q_out: torch.Tensor, cache: CacheView, maps: StepMaps,
     if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.numel() != d // 2 or not inv_freq.is_contiguous()
                                  or inv_freq.get_device() != maps.index):
         raise KernelLaunchError(f"cache8_append: the inverse frequencies must be {d // 2} contiguous float32 numbers")
+    if inv_freq is not None and launch.keys > MOST_POSITIONS:
+        raise KernelLaunchError(f"cache8_append: a block table for {launch.keys} positions, angles are taken for {MOST_POSITIONS}")
     _check(launch.append(
         t.data_ptr(), dtype_code(t.dtype), qkv.n, qkv.stride, q_out.data_ptr(), launch.cache, maps.lists, _ptr(inv_freq), q_heads,
         1 if write_cache else 0, stream if stream is not None else _current_stream(maps.index)), "cache8_append")

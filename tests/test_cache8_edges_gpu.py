@@ -223,3 +223,45 @@ def test_a_call_repeats_itself(dim):
         again = torch.zeros_like(out)
         cache8.attention(q, again, setup.view, setup.maps, 8, 1 / math.sqrt(dim), 900)
         assert torch.equal(again[: setup.rows], out[: setup.rows])
+
+
+# ------------------------------------------------------------------------------ far positions
+
+def _far(page, length, new, width):
+    """One request of `length` positions of which only the last two pages are held, and the plain statement of its new rows."""
+    from bare_cuda_4gib_b200.kernels import cache8
+    from bare_cuda_4gib_b200.kernels.lib import Partials
+    from bare_cuda_4gib_b200.kernels.step_maps import StepMaps
+    dim = 128
+    maps = StepMaps(new, 1, width, page, group=1, tile_rows=cache8.tile_rows(dim), few_rows=16, device=DEV)
+    blocks = -(-(length + new) // page)
+    pages = torch.full((blocks,), -1, dtype=torch.int32)
+    pages[-2:] = torch.tensor([1, 0])
+    maps.build(torch.tensor([length], dtype=torch.int32, device=DEV), torch.tensor([new], dtype=torch.int32, device=DEV), pages.to(DEV), new, new, new)
+    codes = torch.zeros(2, 2, 1, page, dim, dtype=torch.uint8, device=DEV)
+    scales = torch.full((2, 2, 1, page // 16), 2.0 ** -100, device=DEV)
+    inv_freq = (10000.0 ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)).float().to(DEV)
+    qkv = torch.randn(new, 3 * dim, generator=torch.Generator().manual_seed(length)).to(DEV)
+    q = torch.zeros(new, dim, dtype=BF16, device=DEV)
+    cache8.append(Partials(qkv), q, cache8.view(codes, scales, maps.table), maps, inv_freq, 1)
+    want = pc.rotate(qkv.double().cpu().view(new, 3, dim)[:, :2], torch.arange(length, length + new), inv_freq.cpu())
+    return q.double().cpu(), want[:, 0], (maps, codes, scales, inv_freq, qkv)
+
+
+@pytest.mark.parametrize("length", [1000, 130001, 1 << 20, 3000001, (1 << 23) - 9, (1 << 23) + 12345, (1 << 24) - 40])
+def test_append_turns_by_the_angle_of_far_positions(length):
+    """To the last position that a float32 holds: 2^-20 of the entries a rotation mixes, and the rounding to bfloat16."""
+    q, want, _ = _far(128, length, 37, (1 << 24) // 128)
+    assert ((q - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -20 * (1 + want.abs().amax())).all()
+
+
+def test_append_refuses_angles_of_positions_beyond_that():
+    from bare_cuda_4gib_b200.errors import KernelLaunchError
+    from bare_cuda_4gib_b200.kernels import cache8
+    from bare_cuda_4gib_b200.kernels.lib import Partials
+    with pytest.raises(KernelLaunchError, match="angles are taken for"):
+        _far(128, 1000, 2, (1 << 24) // 128 + 1)
+    _q, _want, (maps, codes, scales, _inv_freq, qkv) = _far(128, 1000, 2, 100)
+    q = torch.zeros(2, 128, dtype=BF16, device=DEV)
+    cache8.append(Partials(qkv), q, cache8.view(codes, scales, maps.table), maps, None, 1)       # without angles there is no such bound
+    assert torch.equal(q, qkv[:, :128].to(BF16))
