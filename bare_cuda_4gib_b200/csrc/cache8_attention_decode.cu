@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) cache8_decode_kernel
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
     const int e = most > 0.0f ? min(max(exponent_of(most) - 10, -100), 116) : 0;
-    const float down = power_of_two(-e);
+    const float down = most < INFINITY ? power_of_two(-e) : __int_as_float(0x7fc00000);      // (an infinite entry makes the row NaN, as in the prompt kernel)
 #pragma unroll
     for (int i = 0; i < KG * 8; ++i)
       qf[n][i >> 1][i & 1] = pack_half(__low2float(pairs[i]) * down, __high2float(pairs[i]) * down);

@@ -265,3 +265,23 @@ def test_append_refuses_angles_of_positions_beyond_that():
     q = torch.zeros(2, 128, dtype=BF16, device=DEV)
     cache8.append(Partials(qkv), q, cache8.view(codes, scales, maps.table), maps, None, 1)       # without angles there is no such bound
     assert torch.equal(q, qkv[:, :128].to(BF16))
+
+
+# ------------------------------------------------------------------------------ infinite queries
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("entry", [math.inf, -math.inf])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_a_query_with_an_infinite_entry_is_lost_whatever_the_keys_signs(dim, entry, sign):
+    """Rows of the decode kernel and of the prompt kernel alike, also where every score of the row would be minus infinity."""
+    from bare_cuda_4gib_b200.kernels import cache8
+    setup, q, out = _attention([(100, 1), (40, 3), (0, 40), (0, 1)], 2, 4, dim, 16, seed=3, keys=lambda k, v: (sign * (k.abs() + 1), v))
+    bad, again = q.clone(), torch.zeros_like(out)
+    rows = [0, 2, 4 + 17, 44]
+    for i, r in enumerate(rows):
+        bad[r, i * dim + 5] = entry
+    cache8.attention(bad, again, setup.view, setup.maps, 8, 1 / math.sqrt(dim))
+    wrong = again[: setup.rows].view(setup.rows, 8, dim).isnan().all(-1)
+    assert wrong.nonzero().tolist() == [[r, i] for i, r in enumerate(rows)]
+    good = ~wrong
+    assert torch.equal(again[: setup.rows].view(setup.rows, 8, dim)[good], out[: setup.rows].view(setup.rows, 8, dim)[good])
