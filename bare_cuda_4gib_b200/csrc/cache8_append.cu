@@ -152,7 +152,7 @@ __device__ __forceinline__ uint4 bf16x8(const float (&x)[8]) {
 }
 
 // 896 threads an SM where there is one result to read (768: 2,048 tokens of 32 / 8 heads of 128 in 11.8 us where this took 9.2; 1,024: 9.7,
-// registers spilled), 512 with partial ones, whose loads on their way take more (2,048 tokens with four results 33.3 us; 768 threads 34.0; a
+// registers spilled; a single float32 result spills 76 to 80 bytes already), 512 with partial ones, whose loads on their way take more (2,048 tokens with four results 33.3 us; 768 threads 34.0; a
 // piece's results one after another 54).
 template <int D, typename T, bool ONE>
 __global__ void __launch_bounds__(TOKENS * (D / 16), (D == 128 ? 1 : 2) * (ONE ? 7 : 4)) cache8_append_kernel(const AppendArgs a) {

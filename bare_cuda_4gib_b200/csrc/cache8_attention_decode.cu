@@ -29,8 +29,10 @@
 //    warps' states in shared memory and sends row r to block r % n_splits of the cluster, which merges in index order: no
 //    scratch in global memory, no atomics, no second launch.
 //  * Blocks of keys that lie wholly below the step's first new position are asked for before the kernel waits for the one before it.
-// One B200, 32 / 8 heads of 128: 8 requests of 8,192 positions 24.1 us (5.6 TB/s, 0.86 of the copy rate; over a bfloat16 cache 44.7), 64 of 2,000
-// to 8,191 117 us (5.8 TB/s).  What is left is the start of a block (its lists, then its first pages, then its first keys) and its merge.
+// One B200, 32 / 8 heads of 128: 8 requests of 8,192 positions 24.0 us (5.6 TB/s, 0.86 of the copy rate; over a bfloat16 cache 44.5), 64 of 2,000
+// to 8,191 115 us (5.9 TB/s).  What is left is the start of a block (its lists, then its first pages, then its first keys) and its merge.  Where a warp
+// has few keys they are most of it: 64 requests of 2,047 (32 / 4 heads of 64) 17.6 us (3.9 TB/s), 32 of 1,900 11.1 (2.8; over bfloat16 12.2).
+// 9 to 16 rows (NT 2) leave one block an SM: 64 requests of 8,192 with 16 heads on one of 128 49.6 us (2.7 TB/s), 8 of them 14.4 (1.2).
 
 #include "cache8.cuh"
 

@@ -11,7 +11,7 @@
 //                  pool, a box per piece of a page), and hands the block's scales to the softmax;
 //   converters (4) write the value codes as halves (which hold e4m3 exactly, two a conversion) into 128-byte-swizzled tiles;
 //   MMA issuers (2, one a tile)  S_g = Q_g K^T (M 128, N 64, twice a key block) with the keys as the codes they are: an 8-bit product.  Q_g is the sum of two
-//                  e4m3 tiles, which together hold a bfloat16's eight bits exactly (but for entries 2^10 below their row's largest; those are 2^-18 of it off), times a power of
+//                  e4m3 tiles, which together hold a bfloat16's eight bits exactly (but for entries below 2^-9 of their row's largest, which are off by at most 2^-17 of it), times a power of
 //                  two of the row's own; two products at twice the rate of one in 16 bits, and no key is ever converted.
 //                  O_g (+)= P_g V in halves of 64 keys, each as soon as its half of P is there, with P_g as the operand in tensor memory and V as it
 //                  lies ([key][channel], MN-major): P never goes through shared memory, whose bandwidth bounds a block that has it there;
@@ -34,8 +34,8 @@
 // the block get it; values are finite always, and behind the request's last key, or where no page is held, written as zeros.
 // Every mbarrier wait is bounded: on a timeout the thread sets the error word, all roles leave their loops, tensor memory is
 // released and the block returns.
-// One B200: a prompt of 2,048 tokens (32 / 4 heads of 64) 42.6 us, 2,048 tokens behind 2,048 (32 heads of 128) 118 us (0.88 PFLOP/s; over a
-// bfloat16 cache 137), 61 tokens behind 3,001 (32 / 8 heads of 128) 19.7 us (66).  What bounds it: a key block takes about 4,300 cycles for 256 rows,
+// One B200: a prompt of 2,048 tokens (32 / 4 heads of 64) 43.9 us (over a bfloat16 cache 41.3), 2,048 tokens behind 2,048 (32 heads of 128) 117 us
+// (0.88 PFLOP/s; 136), 61 tokens behind 3,001 (32 / 8 heads of 128) 20.6 us (66).  What bounds it: a key block takes about 4,300 cycles for 256 rows,
 // of which the exponential unit is busy 1,540 and the tensor cores 1,000 to 2,000; the softmax warps (two a scheduler) wait for tensor-memory loads
 // and for their own chains of dependent instructions.  A block's start (queries staged: 7,000 cycles) and the merge of a cluster (9,000) weigh most
 // where there are few keys a block.
@@ -132,7 +132,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
-// Byte offset of the 16-byte chunk `chunk` (0..7) of row `row` inside a [rows x 64 bf16] sub-tile
+// Byte offset of the 16-byte chunk `chunk` (0..7) of row `row` inside a [rows x 64 halves] sub-tile
 // with the 128-byte swizzle: rows are 128 bytes, groups of 8 rows are 1024 bytes, and the chunk
 // index is XORed with the row's index inside its group.
 __device__ __forceinline__ uint32_t swizzled(int row, int chunk) {

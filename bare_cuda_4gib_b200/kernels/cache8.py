@@ -184,7 +184,8 @@ def append(qkv: Partials, q_out: torch.Tensor, cache: CacheView, maps: StepMaps,
     position into `q_out` (bfloat16 [rows, q_heads * head size]), k turned by position and v into the cache (left alone unless
     `write_cache`).  `inv_freq` (float32 [head size / 2]) None: no rotation.  Positions of a written block that earlier steps filled
     keep their numbers, but for a rounding where the new ones need a larger scale.  Requests may share pages that they read, not
-    pages that a step writes.  Rows of no request and idle ones are left as they were in `q_out`."""
+    pages that a step writes.  Rows of no request and idle ones are left as they were in `q_out`.  With `inv_freq` the block table has columns for
+    2^24 positions at most."""
     t = qkv.tensor
     width, d = (q_heads + 2 * cache.kv_heads) * cache.head_dim, cache.head_dim
     launch = _check_step("cache8_append", cache, maps, q_heads, t, q_out)
@@ -209,7 +210,8 @@ def decode_splits(n_seqs: int, kv_heads: int, max_keys: int) -> int:
     """How many blocks of the decode kernel share a request's keys: a power of two up to 8, about two blocks an SM in all, and no more
     than have a scale block for every warp.  With long caches twice that: requests of different lengths then leave fewer SMs idle at the
     end than a block's start and merge cost (one / two blocks: 64 requests of 2,000 to 8,191 positions, 8 heads of 128, 128 / 118 us; of 500 to
-    2,047 positions 37 / 44).  The number goes by what the cache holds, not by the lengths at hand, so a captured graph stays valid."""
+    2,047 positions 37 / 44).  `max_keys` is what the block table has columns for, not the lengths at hand, so that a captured graph stays valid: short
+    requests in wide tables are split for nothing (8 of 100 positions, 4 heads of 64: 4.0 us in a table for 128, 5.8 in one for 8,192)."""
     splits = 1
     while splits < 8 and max_keys > splits * DECODE_WARPS * SCALE_TOKENS and (
             n_seqs * kv_heads * splits * 2 <= 2 * sm_count() or (max_keys >= splits * 2 * 2560 and n_seqs * kv_heads * splits <= 4 * sm_count())):
@@ -221,7 +223,9 @@ def decode_splits(n_seqs: int, kv_heads: int, max_keys: int) -> int:
 def prompt_splits(n_tiles: int, kv_heads: int, max_keys: int) -> int:
     """How many blocks of the prompt kernel share a tile's keys: a power of two up to 8, as many as the SMs take at once in clusters of
     that size (more start only when others have ended: 128 blocks by eights 27.6 us, by fours 64 of them 18.8), and none over four key blocks, where the
-    merge costs more than they save (389 tokens, 4 heads of 64, one block / two 11.9 / 13.4 us; behind 1,000 more 28.0 / 21.5)."""
+    merge costs more than they save (389 tokens, 4 heads of 64, one block / two 11.9 / 13.4 us; behind 1,000 more 28.0 / 21.5).  `max_keys` is what
+    the block table has columns for: a short prompt in a wide table is split all the same (61 tokens behind nothing, 8 heads of 128: 11.4 us in a table
+    for 64 positions, 16.0 in one for 8,192)."""
     splits = 1
     while splits < 8 and n_tiles * kv_heads * splits * 2 <= BLOCKS_AT_ONCE[splits * 2] and max_keys > max(splits, 4) * KEY_BLOCK:
         splits *= 2
@@ -234,7 +238,13 @@ def attention(q: torch.Tensor, out: torch.Tensor, cache: CacheView, maps: StepMa
     `window` of them), q and out contiguous bfloat16 [rows, q_heads * head size].  `extras`: blocks of positions, sink, gate.
     Requests of few packed rows go to the decode kernel, the others to the prompt kernel, which a step may launch both of; rows
     of no request and idle ones are left as they were in `out`, a row that sees no key is zero.  A position whose page is not held (an entry of the
-    block table outside the pool) is seen by no query."""
+    block table outside the pool) is seen by no query.
+
+    Positions below the step's first new ones are read ahead of the wait for the kernels before, so between what wrote them and this call there has to
+    be an ordinary operation of the stream (a copy, a kernel of torch's, the step's own `build`).  The step's maps are that where they are built
+    behind the appends of the step before; a program that builds the maps of two steps ahead of both puts a copy or a synchronisation there.
+
+    Weights are halves: 2^-32 of a row's largest is lost of any one of them, where a bfloat16 cache's kernels keep eight bits."""
     launch = _check_step("cache8_attention", cache, maps, q_heads, q, out)
     width = q_heads * cache.head_dim
     if not _bf16_rows(q, maps.n_rows, width) or not _bf16_rows(out, maps.n_rows, width):
